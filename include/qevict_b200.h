@@ -250,6 +250,82 @@ size_t qv_prefill_workspace_bytes(const qv_dims* d, int32_t seq_len);
  * qv_prefill_attention.  Synchronises the stream. */
 int qv_prefill_read_error(const void* workspace, size_t workspace_bytes, int32_t* host_err, qv_stream_t stream);
 
+/* ---- paged KV cache --------------------------------------------------------
+ * Not part of the reference, whose cache is one tensor per layer: full-context
+ * K/V of many sequences in pages of one pool, for prompts that arrive in
+ * chunks and for full-cache decode beside the Sticky layout.
+ *
+ * Pool: k, v [pages][kv_heads][page_size][head_dim] in dtype, or (bits = 8)
+ * INT8 codes with one fp32 scale per row, k_scale / v_scale
+ * [pages][kv_heads][page_size]: value = code * scale.  Token j of a sequence b
+ * lives in page block_table[b][j / page_size] at offset j % page_size.
+ * Calls check what the device-side tables hold and stay inside their buffers;
+ * what they find wrong sets bits of *err (when not NULL): a page id or a
+ * position outside its table QV_DERR_TABLE (attention then reads page 0, the
+ * read-back leaves the row), a slot behind the pool or a length above its
+ * bound QV_DERR_CAPACITY (not written / cut to the bound). */
+typedef struct qv_paged_cache {
+    void* k;
+    void* v;
+    float* k_scale;      /* bits = 8 only */
+    float* v_scale;
+    int32_t* err;        /* [1] device error word, or NULL */
+    int32_t pages;
+    int32_t kv_heads;
+    int32_t page_size;   /* 16, 32, 64 or 128 */
+    int32_t head_dim;    /* a multiple of 8 up to 256; attention: 64 or 128 */
+    int32_t dtype;       /* QV_*: new rows, queries, outputs (and pages, bits = 0) */
+    int32_t bits;        /* 0: pages in dtype; 8: INT8 */
+} qv_paged_cache;
+
+/* Per-head RMS norm and rotation of query and key heads in one pass, fp32
+ * arithmetic rounded once.  q [tokens][q_heads][head_dim], k
+ * [tokens][kv_heads][head_dim] with token strides in elements (views of a packed
+ * projection; 16-byte aligned rows); q_out, k_out contiguous (they may be q
+ * and k where those are contiguous).  q_weight / k_weight [head_dim] in dtype, or
+ * NULL: y = x * rsqrt(mean(x^2) + eps) * w.  table [max_pos][rot_dim] fp32, cos
+ * then sin of rot_dim/2 angles each, or NULL (no rotation): the first rot_dim
+ * (a multiple of 8) elements turn in pairs (i, i + rot_dim/2), or (2i, 2i + 1)
+ * with interleaved; positions [tokens].  A position outside the table gives NaN. */
+int qv_qk_norm_rope(int32_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, const void* q,
+                    int64_t q_stride, const void* k, int64_t k_stride, const void* q_weight, const void* k_weight,
+                    float eps, const float* table, int32_t max_pos, int32_t rot_dim, int32_t interleaved,
+                    const int32_t* positions, void* q_out, void* k_out, qv_stream_t stream);
+/* The same, with the new keys and the values v [tokens][kv_heads][head_dim]
+ * written into the pool: token t to slot slots[t] = page * page_size + offset, a
+ * negative slot writes nothing (a padded batch).  bits = 8: scale = max|row| / 127,
+ * code = rint(row / scale), from the fp32 row; a row that is not finite reads
+ * back as NaN.  A slot must appear at most once per call. */
+int qv_paged_append(const qv_paged_cache* c, int32_t tokens, int32_t q_heads, const void* q, int64_t q_stride,
+                    const void* k, int64_t k_stride, const void* v, int64_t v_stride, const void* q_weight,
+                    const void* k_weight, float eps, const float* table, int32_t max_pos, int32_t rot_dim,
+                    int32_t interleaved, const int32_t* positions, const int64_t* slots, void* q_out,
+                    qv_stream_t stream);
+/* The cached rows as contiguous tensors: k_out, v_out [total][kv_heads][head_dim] in
+ * dtype, sequence b's first kv_lens[b] tokens from row cu_kv[b] (cu_kv [batch + 1],
+ * ascending); other rows are left as they were. */
+int qv_paged_gather(const qv_paged_cache* c, int32_t batch, const int32_t* block_table, int32_t max_pages,
+                    const int32_t* kv_lens, const int32_t* cu_kv, int32_t total, void* k_out, void* v_out,
+                    qv_stream_t stream);
+/* Attention of a ragged batch of chunks over the pool.  Sequence b's new tokens
+ * are rows cu_q[b] .. cu_q[b+1] of q [total_q][q_heads][head_dim] (token stride in
+ * elements) and the last of its kv_lens[b] cached tokens; causal: each sees the
+ * keys up to its own, otherwise all.  A row that sees no key gives 0; rows
+ * outside every chunk are left as they were.  max_q and max_kv are upper bounds
+ * of the chunk and cached lengths (max_kv <= max_pages * page_size): they size
+ * the launch, so a captured call serves any lengths below them.  Of a longer
+ * chunk the rows past max_q are left as they were, a longer sequence is cut.  out [total_q][q_heads][head_dim].  head_dim 64
+ * or 128, q_heads / kv_heads up to 16.  Sums run in a fixed order.  Rows of one
+ * tile share their P.V products, so a K or V row that is not finite can reach
+ * rows of its own sequence that do not see it; what lies behind a sequence's
+ * last token, in its pages or others, is never used. */
+size_t qv_paged_attention_workspace_bytes(const qv_paged_cache* c, int32_t batch, int32_t q_heads, int32_t total_q,
+                                          int32_t max_q, int32_t max_kv);
+int qv_paged_attention(const qv_paged_cache* c, int32_t batch, int32_t q_heads, const int32_t* block_table,
+                       int32_t max_pages, const int32_t* kv_lens, const int32_t* cu_q, int32_t total_q, int32_t max_q,
+                       int32_t max_kv, const void* q, int64_t q_stride, float scale, int32_t causal, void* out,
+                       void* workspace, size_t workspace_bytes, qv_stream_t stream);
+
 /* ---- codec (the reference's static methods) ----------------------------- */
 
 /* quantize_k_per_window / quantize_v_per_window / dequantize_from_quant

@@ -35,6 +35,11 @@ class QvLayer(ctypes.Structure):
         "arch_ks", "arch_kz", "arch_vs", "arch_vz", "seq", "step", "err")]
 
 
+class QvPagedCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "err")] + [
+        (n, ctypes.c_int32) for n in ("pages", "kv_heads", "page_size", "head_dim", "dtype", "bits")]
+
+
 class QevictError(RuntimeError):
     pass
 
@@ -54,7 +59,8 @@ def lib():
     L = ctypes.CDLL(_LIB_PATH)
     P = ctypes.POINTER
     vp, i32, i64, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
-    D, Lp = P(QvDims), P(QvLayer)
+    D, Lp, Cp = P(QvDims), P(QvLayer), P(QvPagedCache)
+    f32 = ctypes.c_float
     sig = {
         "qv_ring_windows": (i32, [D]),
         "qv_main_capacity": (i32, [D]),
@@ -75,6 +81,14 @@ def lib():
         "qv_prefill_attention": (ctypes.c_int, [D, vp, vp, vp, i32, vp, vp, vp, sz, vp]),
         "qv_prefill_workspace_bytes": (sz, [D, i32]),
         "qv_prefill_read_error": (ctypes.c_int, [vp, sz, P(i32), vp]),
+        "qv_qk_norm_rope": (ctypes.c_int, [i32, i32, i32, i32, i32, vp, i64, vp, i64, vp, vp, f32, vp, i32, i32, i32,
+                                           vp, vp, vp, vp]),
+        "qv_paged_append": (ctypes.c_int, [Cp, i32, i32, vp, i64, vp, i64, vp, i64, vp, vp, f32, vp, i32, i32, i32,
+                                           vp, vp, vp, vp]),
+        "qv_paged_gather": (ctypes.c_int, [Cp, i32, vp, i32, vp, vp, i32, vp, vp, vp]),
+        "qv_paged_attention_workspace_bytes": (sz, [Cp, i32, i32, i32, i32, i32]),
+        "qv_paged_attention": (ctypes.c_int, [Cp, i32, i32, vp, i32, vp, vp, i32, i32, i32, vp, i64, f32, i32, vp, vp,
+                                              sz, vp]),
         "qv_quantize_k": (ctypes.c_int, [i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]),
         "qv_quantize_v": (ctypes.c_int, [i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]),
         "qv_dequantize": (ctypes.c_int, [i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]),
@@ -112,6 +126,8 @@ def exported_symbols():
             "qv_decode_attention_noalloc", "qv_decode_attention_nofold", "qv_decode_fold", "qv_evict_cycle",
             "qv_evict_cycle_count", "qv_evict_cycle_ext",
             "qv_prefill_build", "qv_prefill_attention", "qv_prefill_workspace_bytes", "qv_prefill_read_error",
+            "qv_qk_norm_rope", "qv_paged_append", "qv_paged_gather", "qv_paged_attention_workspace_bytes",
+            "qv_paged_attention",
             "qv_quantize_k", "qv_quantize_v", "qv_dequantize", "qv_add_rmsnorm", "qv_silu_mul", "qv_gemv",
             "qv_argmax_workspace_bytes", "qv_argmax", "qv_track_prefill", "qv_track_decode",
             "qv_track_positions", "qv_read_error",

@@ -1,0 +1,397 @@
+// The paged KV cache: norm and rotation of query / key heads, the same with
+// the new keys and values written into pages, and pages read back.
+//
+// Per head row x of D elements, in fp32 throughout and rounded once at the
+// store:
+//   norm      y = x * (mean(x^2) + eps)^(-1/2) * w          (optional)
+//   rotation  pair (a, b) -> (a c - b s, b c + a s), i < rot/2, with (a, b) =
+//             (y[i], y[i + rot/2]) or, interleaved, (y[2i], y[2i+1]); (c, s)
+//             from the fp32 table row of the token's position
+//   8 bits    scale = max|y| / 127 (fp32), code = rint(y / scale)
+//
+// All three are bound by HBM: every row is read and written once.  A block
+// takes one token, and each of its threads one 8-element chunk position of
+// all the token's heads, so that the table row and the norm weights are
+// loaded once per token into registers (a table row is two to four times a
+// 16-bit head row) and the rows of up to four heads are in flight per thread.
+#include <math.h>
+
+#include "paged.cuh"
+
+namespace qv {
+
+constexpr int PH_THREADS = 256;
+constexpr int PH_ROWS = 4;   // head rows in flight per thread
+
+struct HeadArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t qs, ks, vs;          // token strides in elements
+    const void* qw;              // [D] or null
+    const void* kw;
+    float eps;
+    const float* table;          // [max_pos][rot]: cos | sin, or null
+    const int32_t* pos;
+    int max_pos, rot, interleaved;
+    int Hq, H, D;
+    void* q_out;                 // [tokens][Hq][D]
+    void* k_out;                 // [tokens][H][D] (no pages)
+    void* kp;                    // pages
+    void* vp;
+    float* k_scale;
+    float* v_scale;
+    const int64_t* slots;
+    int64_t n_slots;
+    int page_shift;
+    int32_t* err;
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+enum { PH_ROWS_ONLY = 0, PH_PAGES = 1, PH_PAGES8 = 2 };
+
+// TPR threads share a head row (8 elements each, TPR a power of two >= D/8).
+template <int DT, int TPR, int MODE>
+__global__ void __launch_bounds__(PH_THREADS) heads_kernel(const HeadArgs a) {
+    constexpr int HPB = PH_THREADS / TPR;
+    const size_t t = blockIdx.x;
+    const int c = threadIdx.x & (TPR - 1), hl = threadIdx.x / TPR;
+    const int lane = threadIdx.x & 31;
+    const bool on = 8 * c < a.D;
+    const int rows = MODE == PH_ROWS_ONLY ? a.Hq + a.H : a.Hq + 2 * a.H;
+
+    int64_t slot = -1;
+    if (MODE != PH_ROWS_ONLY) {
+        slot = a.slots[t];
+        if (slot >= a.n_slots) {
+            if (threadIdx.x == 0 && a.err) set_err(a.err, QV_DERR_CAPACITY);
+            slot = -1;
+        }
+    }
+    float qw[8], kw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qw[i] = kw[i] = 1.f;
+    if (a.qw && on) widen8<DT>(load8<DT>(a.qw, 8 * c), qw);
+    if (a.kw && on) widen8<DT>(load8<DT>(a.kw, 8 * c), kw);
+
+    // the thread's rotation factors and where its partner elements sit: 4-element
+    // sub-chunk u = 2c + s of a half-layout head pairs with u +- rot/8
+    float cs[8], sn[8];
+    bool turn[2] = {false, false};
+    int src[2] = {lane, lane};
+    const int r8 = a.rot >> 3;
+    if (a.table) {
+        const int p = a.pos[t];
+        const bool ok = (unsigned)p < (unsigned)a.max_pos;
+        if (MODE != PH_ROWS_ONLY && !ok && threadIdx.x == 0 && a.err) set_err(a.err, QV_DERR_TABLE);
+        const float* row = a.table + (size_t)(ok ? p : 0) * a.rot;
+        const float bad = ok ? 0.f : NAN;   // a position outside the table shows as NaN
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int u = 2 * c + s;
+            turn[s] = 4 * u < a.rot;
+            float4 cv = make_float4(0.f, 0.f, 0.f, 0.f), sv = cv;
+            if (turn[s]) {
+                // interleaved: both sub-chunks of a thread read their two pairs of the same 4
+                const int i0 = a.interleaved ? 4 * c : 4 * (u < r8 ? u : u - r8);
+                cv = *reinterpret_cast<const float4*>(row + i0);
+                sv = *reinterpret_cast<const float4*>(row + a.rot / 2 + i0);
+                if (!a.interleaved) src[s] = lane - c + ((u < r8 ? u + r8 : u - r8) >> 1);
+            }
+            const float* ce = reinterpret_cast<const float*>(&cv);
+            const float* se = reinterpret_cast<const float*>(&sv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = a.interleaved ? 2 * s + (i >> 1) : i;
+                const bool first = a.interleaved ? (i & 1) == 0 : u < r8;
+                cs[4 * s + i] = ce[j] + bad;
+                sn[4 * s + i] = (first ? -se[j] : se[j]) + bad;
+            }
+        }
+    }
+
+    for (int r0 = 0; r0 < rows; r0 += HPB * PH_ROWS) {
+        Chunk8<DT> raw[PH_ROWS];
+#pragma unroll
+        for (int i = 0; i < PH_ROWS; ++i) {
+            const int r = r0 + i * HPB + hl;
+#pragma unroll
+            for (int w = 0; w < (DT == QV_F32 ? 2 : 1); ++w) raw[i].u[w] = make_uint4(0, 0, 0, 0);
+            if (r < rows && on) {
+                if (r < a.Hq) raw[i] = load8<DT>(a.q, t * a.qs + (size_t)r * a.D + 8 * c);
+                else if (r < a.Hq + a.H) raw[i] = load8<DT>(a.k, t * a.ks + (size_t)(r - a.Hq) * a.D + 8 * c);
+                else raw[i] = load8<DT>(a.v, t * a.vs + (size_t)(r - a.Hq - a.H) * a.D + 8 * c);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PH_ROWS; ++i) {
+            if (r0 + i * HPB >= rows) break;   // the same for the whole block
+            const int r = r0 + i * HPB + hl;
+            const bool is_q = r < a.Hq, is_v = r >= a.Hq + a.H;
+            float x[8];
+            widen8<DT>(raw[i], x);
+            if (a.qw || a.kw) {
+                float ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+#pragma unroll
+                for (int o = TPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if (!is_v && (is_q ? a.qw : a.kw)) {
+                    const float inv = rsqrtf(ss / (float)a.D + a.eps);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * (is_q ? qw[j] : kw[j]);
+                }
+            }
+            if (a.table) {
+                float y[8];
+                if (a.interleaved) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
+                } else {
+                    const bool swap = r8 & 1;   // partners sit in the other sub-chunk
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        y[j] = __shfl_sync(0xffffffffu, swap ? x[4 + j] : x[j], src[0]);
+                        y[4 + j] = __shfl_sync(0xffffffffu, swap ? x[j] : x[4 + j], src[1]);
+                    }
+                }
+                if (!is_v) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (turn[j >> 2]) x[j] = fmaf(x[j], cs[j], y[j] * sn[j]);
+                }
+            }
+            float scale = 0.f;
+            if (MODE == PH_PAGES8) {
+                float m = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(x[j]));
+#pragma unroll
+                for (int o = TPR / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                scale = __fdiv_rn(m, 127.f);
+            }
+            if (r >= rows || !on) continue;    // no shuffle follows in this row
+            if (is_q) {
+                store8<DT>(a.q_out, (t * a.Hq + r) * a.D + 8 * c, x);
+                continue;
+            }
+            const int h = r - a.Hq - (is_v ? a.H : 0);
+            if (MODE == PH_ROWS_ONLY) {
+                store8<DT>(a.k_out, (t * a.H + h) * a.D + 8 * c, x);
+            } else if (slot >= 0) {
+                const size_t pg = (size_t)(slot >> a.page_shift), off = (size_t)slot & ((1u << a.page_shift) - 1);
+                const size_t row = ((pg * a.H + h) << a.page_shift) + off;
+                void* pages = is_v ? a.vp : a.kp;
+                if (MODE == PH_PAGES) {
+                    store8<DT>(pages, row * a.D + 8 * c, x);
+                } else {
+                    uint2 u;
+                    int8_t* e = reinterpret_cast<int8_t*>(&u);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        // a row that is not finite: codes of 0 and a scale that is not finite read back as NaN
+                        const float f = scale > 0.f && scale < INFINITY ? __fdiv_rn(x[j], scale) : 0.f;
+                        e[j] = (int8_t)__float2int_rn(fminf(fmaxf(f, -127.f), 127.f));
+                    }
+                    *reinterpret_cast<uint2*>(reinterpret_cast<int8_t*>(pages) + row * a.D + 8 * c) = u;
+                    if (c == 0) (is_v ? a.v_scale : a.k_scale)[row] = scale;
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- read back
+constexpr int PG_TOKENS = 8;     // tokens per block
+constexpr int PG_THREADS = 256;
+constexpr int PG_FLIGHT = 4;     // K chunks, and V chunks, in flight per thread
+
+struct GatherArgs {
+    const void* k;
+    const void* v;
+    const float* k_scale;
+    const float* v_scale;
+    int32_t* err;
+    const int32_t* block_table;
+    const int32_t* kv_lens;
+    const int32_t* cu_kv;
+    void* k_out;
+    void* v_out;
+    int pages, H, D, page_shift, max_pages, B, total;
+};
+
+template <int DT, bool Q8>
+__global__ void __launch_bounds__(PG_THREADS) gather_kernel(const GatherArgs a) {
+    __shared__ int64_t s_row[PG_TOKENS];   // the token's row of head 0 in the pages, or -1
+    const int t0 = blockIdx.x * PG_TOKENS;
+    if (threadIdx.x < PG_TOKENS) {
+        const int t = t0 + threadIdx.x;
+        int64_t row = -1;
+        if (t < a.total) {
+            const int b = paged_find_token(a.cu_kv, a.B, t);
+            const int pos = t - a.cu_kv[b];
+            if (t < a.cu_kv[a.B] && pos >= 0 && pos < a.kv_lens[b]) {
+                const int pi = pos >> a.page_shift;
+                const int pg = pi < a.max_pages ? a.block_table[(size_t)b * a.max_pages + pi] : -1;
+                if ((unsigned)pg < (unsigned)a.pages)
+                    row = (((int64_t)pg * a.H) << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+                else if (a.err)
+                    set_err(a.err, pi < a.max_pages ? QV_DERR_TABLE : QV_DERR_CAPACITY);
+            }
+        }
+        s_row[threadIdx.x] = row;
+    }
+    __syncthreads();
+    const int per_row = a.D >> 3, per_tok = a.H * per_row, n = PG_TOKENS * per_tok;
+    for (int i0 = threadIdx.x; i0 < n; i0 += PG_THREADS * PG_FLIGHT) {
+        int64_t src[PG_FLIGHT], dst[PG_FLIGHT];
+        Chunk8<DT> kr[PG_FLIGHT], vr[PG_FLIGHT];
+        uint2 kc[PG_FLIGHT], vc[PG_FLIGHT];
+        float kscale[PG_FLIGHT], vscale[PG_FLIGHT];
+#pragma unroll
+        for (int f = 0; f < PG_FLIGHT; ++f) {
+            const int i = i0 + f * PG_THREADS;
+            src[f] = -1;
+            if (i >= n) continue;
+            const int tt = i / per_tok, rem = i - tt * per_tok, h = rem / per_row, c = rem - h * per_row;
+            if (s_row[tt] < 0) continue;
+            const int64_t row = s_row[tt] + ((int64_t)h << a.page_shift);
+            src[f] = row * a.D + 8 * c;
+            dst[f] = ((int64_t)(t0 + tt) * a.H + h) * a.D + 8 * c;
+            if (Q8) {
+                kc[f] = *reinterpret_cast<const uint2*>(reinterpret_cast<const int8_t*>(a.k) + src[f]);
+                vc[f] = *reinterpret_cast<const uint2*>(reinterpret_cast<const int8_t*>(a.v) + src[f]);
+                kscale[f] = a.k_scale[row];
+                vscale[f] = a.v_scale[row];
+            } else {
+                kr[f] = load8<DT>(a.k, src[f]);
+                vr[f] = load8<DT>(a.v, src[f]);
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < PG_FLIGHT; ++f) {
+            if (src[f] < 0) continue;
+            float x[8];
+            if (Q8) widen8_codes(kc[f], kscale[f], x); else widen8<DT>(kr[f], x);
+            store8<DT>(a.k_out, dst[f], x);
+            if (Q8) widen8_codes(vc[f], vscale[f], x); else widen8<DT>(vr[f], x);
+            store8<DT>(a.v_out, dst[f], x);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host
+static bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool dtype_ok(int dt) { return dt == QV_F32 || dt == QV_BF16 || dt == QV_F16; }
+
+// The checks every entry point makes of a cache.
+int paged_cache_check(const qv_paged_cache* c) {
+    if (!c || !c->k || !c->v || !al16(c->k) || !al16(c->v)) return QV_EINVAL;
+    if (c->pages <= 0 || c->kv_heads <= 0 || c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8) return QV_EINVAL;
+    if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return QV_EINVAL;
+    if (!dtype_ok(c->dtype) || (c->bits != 0 && c->bits != 8)) return QV_EINVAL;
+    if (c->bits == 8 && (!c->k_scale || !c->v_scale)) return QV_EINVAL;
+    return QV_OK;
+}
+
+int paged_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+
+static int heads_check(const HeadArgs& a, int64_t tokens, int dt) {
+    if (tokens < 0 || tokens > 0x7fffffff || a.Hq <= 0 || a.H <= 0 || !dtype_ok(dt)) return QV_EINVAL;
+    if (a.D < 8 || a.D > 256 || a.D % 8) return QV_EINVAL;
+    const int64_t per16 = 16 / (int64_t)elt_size(dt);
+    if (!a.q || !a.k || !a.q_out || !al16(a.q) || !al16(a.k) || !al16(a.q_out)) return QV_EINVAL;
+    if (a.qs < (int64_t)a.Hq * a.D || a.ks < (int64_t)a.H * a.D || a.qs % per16 || a.ks % per16) return QV_EINVAL;
+    if ((a.qw && !al16(a.qw)) || (a.kw && !al16(a.kw))) return QV_EINVAL;
+    if (a.table && (!a.pos || !al16(a.table) || a.max_pos <= 0 || a.rot < 8 || a.rot > a.D || a.rot % 8)) return QV_EINVAL;
+    return QV_OK;
+}
+
+template <int DT, int MODE> static int heads_launch(const HeadArgs& a, int64_t tokens, cudaStream_t s) {
+    const int g = (int)tokens;
+    if (a.D <= 64) heads_kernel<DT, 8, MODE><<<g, PH_THREADS, 0, s>>>(a);
+    else if (a.D <= 128) heads_kernel<DT, 16, MODE><<<g, PH_THREADS, 0, s>>>(a);
+    else heads_kernel<DT, 32, MODE><<<g, PH_THREADS, 0, s>>>(a);
+    return check_launch();
+}
+template <int MODE> static int heads_dispatch(const HeadArgs& a, int64_t tokens, int dt, cudaStream_t s) {
+    if (dt == QV_F32) return heads_launch<QV_F32, MODE>(a, tokens, s);
+    if (dt == QV_BF16) return heads_launch<QV_BF16, MODE>(a, tokens, s);
+    return heads_launch<QV_F16, MODE>(a, tokens, s);
+}
+
+}  // namespace qv
+
+using namespace qv;
+
+extern "C" int qv_qk_norm_rope(int32_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t dtype,
+                               const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* q_weight,
+                               const void* k_weight, float eps, const float* table, int32_t max_pos, int32_t rot_dim,
+                               int32_t interleaved, const int32_t* positions, void* q_out, void* k_out,
+                               qv_stream_t stream) {
+    HeadArgs a = {};
+    a.q = q; a.k = k; a.qs = q_stride; a.ks = k_stride; a.qw = q_weight; a.kw = k_weight; a.eps = eps;
+    a.table = table; a.pos = positions; a.max_pos = max_pos; a.rot = rot_dim; a.interleaved = interleaved != 0;
+    a.Hq = q_heads; a.H = kv_heads; a.D = head_dim; a.q_out = q_out; a.k_out = k_out;
+    if (tokens == 0) return QV_OK;
+    const int rc = heads_check(a, tokens, dtype);
+    if (rc != QV_OK) return rc;
+    if (!k_out || !al16(k_out)) return QV_EINVAL;
+    return heads_dispatch<PH_ROWS_ONLY>(a, tokens, dtype, (cudaStream_t)stream);
+}
+
+extern "C" int qv_paged_append(const qv_paged_cache* c, int32_t tokens, int32_t q_heads, const void* q,
+                               int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                               const void* q_weight, const void* k_weight, float eps, const float* table,
+                               int32_t max_pos, int32_t rot_dim, int32_t interleaved, const int32_t* positions,
+                               const int64_t* slots, void* q_out, qv_stream_t stream) {
+    int rc = paged_cache_check(c);
+    if (rc != QV_OK) return rc;
+    HeadArgs a = {};
+    a.q = q; a.k = k; a.v = v; a.qs = q_stride; a.ks = k_stride; a.vs = v_stride;
+    a.qw = q_weight; a.kw = k_weight; a.eps = eps;
+    a.table = table; a.pos = positions; a.max_pos = max_pos; a.rot = rot_dim; a.interleaved = interleaved != 0;
+    a.Hq = q_heads; a.H = c->kv_heads; a.D = c->head_dim; a.q_out = q_out;
+    a.kp = c->k; a.vp = c->v; a.k_scale = c->k_scale; a.v_scale = c->v_scale; a.err = c->err;
+    a.slots = slots; a.page_shift = paged_shift(c->page_size);
+    a.n_slots = (int64_t)c->pages * c->page_size;
+    if (tokens == 0) return QV_OK;
+    rc = heads_check(a, tokens, c->dtype);
+    if (rc != QV_OK) return rc;
+    const int64_t per16 = 16 / (int64_t)elt_size(c->dtype);
+    if (!v || !al16(v) || !slots || v_stride < (int64_t)a.H * a.D || v_stride % per16) return QV_EINVAL;
+    return c->bits == 8 ? heads_dispatch<PH_PAGES8>(a, tokens, c->dtype, (cudaStream_t)stream)
+                        : heads_dispatch<PH_PAGES>(a, tokens, c->dtype, (cudaStream_t)stream);
+}
+
+extern "C" int qv_paged_gather(const qv_paged_cache* c, int32_t batch, const int32_t* block_table, int32_t max_pages,
+                               const int32_t* kv_lens, const int32_t* cu_kv, int32_t total, void* k_out, void* v_out,
+                               qv_stream_t stream) {
+    const int rc = paged_cache_check(c);
+    if (rc != QV_OK) return rc;
+    if (batch < 0 || total < 0) return QV_EINVAL;
+    if (batch == 0 || total == 0) return QV_OK;
+    if (!block_table || max_pages <= 0 || !kv_lens || !cu_kv || !k_out || !v_out) return QV_EINVAL;
+    if (!al16(k_out) || !al16(v_out)) return QV_EINVAL;
+    GatherArgs a = {c->k, c->v, c->k_scale, c->v_scale, c->err, block_table, kv_lens, cu_kv, k_out, v_out,
+                    c->pages, c->kv_heads, c->head_dim, paged_shift(c->page_size), max_pages, batch, total};
+    const int g = (int)(((int64_t)total + PG_TOKENS - 1) / PG_TOKENS);
+    cudaStream_t s = (cudaStream_t)stream;
+    const bool q8 = c->bits == 8;
+    if (c->dtype == QV_F32) {
+        if (q8) gather_kernel<QV_F32, true><<<g, PG_THREADS, 0, s>>>(a);
+        else gather_kernel<QV_F32, false><<<g, PG_THREADS, 0, s>>>(a);
+    } else if (c->dtype == QV_BF16) {
+        if (q8) gather_kernel<QV_BF16, true><<<g, PG_THREADS, 0, s>>>(a);
+        else gather_kernel<QV_BF16, false><<<g, PG_THREADS, 0, s>>>(a);
+    } else {
+        if (q8) gather_kernel<QV_F16, true><<<g, PG_THREADS, 0, s>>>(a);
+        else gather_kernel<QV_F16, false><<<g, PG_THREADS, 0, s>>>(a);
+    }
+    return check_launch();
+}

@@ -1,0 +1,135 @@
+// Shared by the paged-cache kernels: 8-element row chunks, the sequence that a
+// token or tile belongs to, and the arguments of the attention kernels.
+#pragma once
+
+#include "common.cuh"
+
+namespace qv {
+
+// Eight consecutive elements as loaded (16 bytes of a 16-bit type, 32 of fp32).
+template <int DT> struct Chunk8 { uint4 u[DT == QV_F32 ? 2 : 1]; };
+
+template <int DT> __device__ __forceinline__ Chunk8<DT> load8(const void* base, size_t elt) {
+    Chunk8<DT> c;
+    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const typename Elt<DT>::T*>(base) + elt);
+    c.u[0] = p[0];
+    if constexpr (DT == QV_F32) c.u[1] = p[1];
+    return c;
+}
+
+template <int DT> __device__ __forceinline__ void widen8(const Chunk8<DT>& c, float* x) {
+    const typename Elt<DT>::T* e = reinterpret_cast<const typename Elt<DT>::T*>(c.u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Elt<DT>::f(e[i]);
+}
+
+template <int DT> __device__ __forceinline__ void store8(void* base, size_t elt, const float* x) {
+    Chunk8<DT> c;
+    typename Elt<DT>::T* e = reinterpret_cast<typename Elt<DT>::T*>(c.u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = Elt<DT>::t(x[i]);
+    uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<typename Elt<DT>::T*>(base) + elt);
+    p[0] = c.u[0];
+    if constexpr (DT == QV_F32) p[1] = c.u[1];
+}
+
+// Eight INT8 codes times their row's scale.
+__device__ __forceinline__ void widen8_codes(uint2 u, float scale, float* x) {
+    const int8_t* e = reinterpret_cast<const int8_t*>(&u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)e[i] * scale;
+}
+
+struct PagedArgs {
+    const void* k;               // [pages][H][page][D], dtype or int8
+    const void* v;
+    const float* k_scale;        // [pages][H][page] (int8 pages)
+    const float* v_scale;
+    int32_t* err;                // may be null
+    const int32_t* block_table;  // [B][max_pages]
+    const int32_t* kv_lens;      // [B]
+    const int32_t* cu_q;         // [B + 1]
+    const void* q;               // [total_q][G*H][D], token stride q_stride elements
+    void* out;                   // [total_q][G*H][D]
+    float* part_o;               // [splits][total_q*G*H][D]
+    float* part_ml;              // [splits][total_q*G*H][2]: row maximum (base-2 logits), sum
+    int64_t q_stride;
+    int pages, H, G, page_shift, max_pages, B, total_q, max_q, max_kv, causal, splits, chunk;
+    float scale_log2;            // softmax scale * log2(e)
+};
+
+// One sequence of the batch, clamped so that no address leaves its buffer
+// whatever the device-side lengths hold.
+struct PagedSeq {
+    int q0, n, kv;   // first row of the chunk, its tokens, cached tokens (the chunk's own included)
+    int live;        // tokens of the chunk that are computed: min(n, max_q)
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
+    PagedSeq s;
+    const int lo = min(max(a.cu_q[b], 0), a.total_q), hi = min(max(a.cu_q[b + 1], 0), a.total_q);
+    s.q0 = lo;
+    s.n = max(hi - lo, 0);
+    const int kv = a.kv_lens[b];
+    s.kv = min(max(kv, 0), a.max_kv);
+    s.live = min(s.n, a.max_q);
+    if ((kv != s.kv || s.live != s.n) && a.err) set_err(a.err, QV_DERR_CAPACITY);
+    return s;
+}
+
+// Keys that token i of the chunk sees.
+__device__ __forceinline__ int paged_limit(const PagedArgs& a, const PagedSeq& s, int i) {
+    return a.causal ? min(s.kv, s.kv - s.n + i + 1) : s.kv;
+}
+
+// Page that holds a key; an id outside the pool raises the error word and reads page 0.
+__device__ __forceinline__ int paged_page(const PagedArgs& a, int b, int key) {
+    int p = a.block_table[(size_t)b * a.max_pages + (key >> a.page_shift)];
+    if ((unsigned)p >= (unsigned)a.pages) {
+        if (a.err) set_err(a.err, QV_DERR_TABLE);
+        p = 0;
+    }
+    return p;
+}
+
+// The sequence that holds tile `tile` when every chunk of n tokens (up to
+// max_q) is cut into ceil(n * rows_per_token / tile_rows) tiles: (sequence,
+// tile within it), or sequence -1 past the last tile.  Called by one full warp.
+__device__ __forceinline__ int2 paged_find_tile(const PagedArgs& a, int tile, int rows_per_token, int tile_rows) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int b = b0 + lane;
+        int n = 0;
+        if (b < a.B) {
+            const int lo = min(max(a.cu_q[b], 0), a.total_q), hi = min(max(a.cu_q[b + 1], 0), a.total_q);
+            const long long rows = (long long)min(max(hi - lo, 0), a.max_q) * rows_per_token;
+            n = (int)((rows + tile_rows - 1) / tile_rows);
+        }
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > tile);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            const int start = before + __shfl_sync(0xffffffffu, incl - n, src);
+            return make_int2(b0 + src, tile - start);
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return make_int2(-1, 0);
+}
+
+// Index of the last entry of the ascending cu[0..B] that is <= t, below B.
+__device__ __forceinline__ int paged_find_token(const int32_t* cu, int B, int t) {
+    int lo = 0, hi = B;   // cu[lo] <= t, and hi is past it
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid] <= t) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+}  // namespace qv

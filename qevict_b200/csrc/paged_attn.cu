@@ -1,0 +1,188 @@
+// Attention of a ragged batch of chunks of new tokens over a paged KV cache:
+// how the work is cut, the launches, and the merge of key splits.
+//
+// Token i of a chunk of n, in a sequence of L cached tokens (the chunk's own
+// included), sees the keys j < L - n + i + 1 (causal) or j < L:
+//   o = sum_j softmax_j(scale q.k_j) v_j,  and 0 where it sees none.
+// Where the tiles of query rows alone would not fill the GPU, the key axis is
+// cut into splits of equal length; each split leaves its unnormalised output,
+// row maximum and sum in fp32, and paged_combine_kernel merges them in split
+// order (the same bits for the same call, whatever finished first).
+#include <math.h>
+
+#include "paged.cuh"
+#include "paged_simt.cuh"
+
+namespace qv {
+
+int paged_cache_check(const qv_paged_cache* c);
+int paged_shift(int page);
+
+constexpr int PC_THREADS = 128;
+
+// One block per (token, query head): its four warps take the splits in turn,
+// lane i holds columns of the row, and the warps' sums join in shared memory.
+template <int DT, int D>
+__global__ void __launch_bounds__(PC_THREADS) paged_combine_kernel(const PagedArgs a) {
+    constexpr int E = D / 32;
+    __shared__ float s_o[4][D], s_l[4], s_m[4];
+    const int Hq = a.H * a.G;
+    const int t = blockIdx.x / Hq, hq = blockIdx.x % Hq;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = paged_find_token(a.cu_q, a.B, t);
+    const PagedSeq s = paged_seq(a, b);
+    const int i = t - s.q0;
+    if (i < 0 || i >= s.live || s.kv <= a.chunk) return;   // behind the last sequence, or written by its only split
+    const int limit = paged_limit(a, s, i);
+    const int n = limit > 0 ? (limit + a.chunk - 1) / a.chunk : 0;
+    const size_t row = (size_t)t * Hq + hq, step = (size_t)a.total_q * Hq;
+    float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int sp = warp; sp < n; sp += 4) {
+        const size_t p = sp * step + row;
+        const float ms = a.part_ml[2 * p], ls = a.part_ml[2 * p + 1];
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = a.part_o[p * D + E * lane + e];
+        const float mn = fmaxf(m, ms), base = mn == -INFINITY ? 0.f : mn;
+        const float f = exp2f(m - base), g = exp2f(ms - base);
+        l = l * f + ls * g;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = o[e] * f + v[e] * g;
+        m = mn;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_o[warp][E * lane + e] = o[e];
+    if (lane == 0) { s_l[warp] = l; s_m[warp] = m; }
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    const float mm = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    const float base = mm == -INFINITY ? 0.f : mm;
+    float sum = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = exp2f(s_m[w] - base);
+        sum += s_l[w] * f;
+        x += s_o[w][threadIdx.x] * f;
+    }
+    st<DT>(a.out, row * D + threadIdx.x, sum > 0.f ? x / sum : sum);
+}
+
+// ---------------------------------------------------------------- plan
+struct PagedPlan {
+    int bm;        // query rows per tile
+    int64_t tiles; // upper bound of the query tiles of a KV head
+    int splits, chunk;
+};
+
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static PagedPlan paged_plan(int B, int H, int G, int total_q, int max_q, int max_kv) {
+    PagedPlan p;
+    p.bm = (int64_t)max_q * G <= 16 ? 16 : 64;
+    // every sequence ends in at most one partial tile, and none is longer than max_q
+    p.tiles = (int64_t)total_q * G / p.bm + (B < total_q ? B : total_q);
+    const int64_t by_len = (int64_t)B * ceil_div((int64_t)max_q * G, p.bm);
+    if (p.tiles > by_len) p.tiles = by_len;
+    // splits: enough blocks for two per SM, of at least 256 keys
+    const int64_t blocks = p.tiles * H;
+    int64_t n = blocks > 0 ? ceil_div(2 * 148, blocks) : 1;
+    const int64_t most = ceil_div(max_kv, 256);
+    if (n > most) n = most;
+    if (n < 1) n = 1;
+    p.chunk = (int)(ceil_div(ceil_div(max_kv, n), 128) * 128);
+    if (p.chunk < 128) p.chunk = 128;
+    p.splits = (int)ceil_div(max_kv, p.chunk);
+    if (p.splits < 1) p.splits = 1;
+    return p;
+}
+
+static size_t paged_ws_bytes(const PagedPlan& p, int total_q, int Hq, int D) {
+    return p.splits > 1 ? (size_t)p.splits * total_q * Hq * (D + 2) * sizeof(float) : 0;
+}
+
+// ---------------------------------------------------------------- launch
+template <int DT, int D, bool Q8, int BM>
+static int simt_launch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
+    constexpr size_t bytes = paged_simt_smem<D, BM>();
+    if (bytes > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(paged_simt_kernel<DT, D, Q8, BM>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return set_cuda_error(e);
+    }
+    paged_simt_kernel<DT, D, Q8, BM><<<dim3((unsigned)p.tiles, a.H, p.splits), PS_THREADS, bytes, s>>>(a);
+    return check_launch();
+}
+
+template <int DT, int D, bool Q8> static int simt_dispatch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
+    return p.bm == 16 ? simt_launch<DT, D, Q8, 16>(a, p, s) : simt_launch<DT, D, Q8, 64>(a, p, s);
+}
+
+template <int DT, int D> static int paged_launch(const PagedArgs& a, const PagedPlan& p, bool q8, cudaStream_t s) {
+    const int rc = q8 ? simt_dispatch<DT, D, true>(a, p, s) : simt_dispatch<DT, D, false>(a, p, s);
+    if (rc != QV_OK || p.splits == 1) return rc;
+    paged_combine_kernel<DT, D><<<(unsigned)((int64_t)a.total_q * a.H * a.G), PC_THREADS, 0, s>>>(a);
+    return check_launch();
+}
+
+}  // namespace qv
+
+using namespace qv;
+
+static bool attn_dims_ok(const qv_paged_cache* c, int32_t batch, int32_t q_heads, int32_t total_q, int32_t max_q,
+                         int32_t max_kv) {
+    if (batch < 0 || total_q < 0 || max_q < 0 || max_kv < 0 || q_heads <= 0) return false;
+    if (c->head_dim != 64 && c->head_dim != 128) return false;
+    if (q_heads % c->kv_heads || q_heads / c->kv_heads > 16 || c->kv_heads > 65535) return false;
+    return (int64_t)total_q * q_heads <= 0x7fffffff;
+}
+
+extern "C" size_t qv_paged_attention_workspace_bytes(const qv_paged_cache* c, int32_t batch, int32_t q_heads,
+                                                     int32_t total_q, int32_t max_q, int32_t max_kv) {
+    if (paged_cache_check(c) != QV_OK || !attn_dims_ok(c, batch, q_heads, total_q, max_q, max_kv)) return 0;
+    if (batch == 0 || total_q == 0 || max_q == 0) return 0;
+    return paged_ws_bytes(paged_plan(batch, c->kv_heads, q_heads / c->kv_heads, total_q, max_q, max_kv), total_q,
+                          q_heads, c->head_dim);
+}
+
+extern "C" int qv_paged_attention(const qv_paged_cache* c, int32_t batch, int32_t q_heads, const int32_t* block_table,
+                                  int32_t max_pages, const int32_t* kv_lens, const int32_t* cu_q, int32_t total_q,
+                                  int32_t max_q, int32_t max_kv, const void* q, int64_t q_stride, float scale,
+                                  int32_t causal, void* out, void* workspace, size_t workspace_bytes,
+                                  qv_stream_t stream) {
+    const int rc = paged_cache_check(c);
+    if (rc != QV_OK) return rc;
+    if (!attn_dims_ok(c, batch, q_heads, total_q, max_q, max_kv)) return QV_EINVAL;
+    if (batch == 0 || total_q == 0 || max_q == 0) return QV_OK;
+    if (!block_table || max_pages <= 0 || !kv_lens || !cu_q || !q || !out) return QV_EINVAL;
+    if ((int64_t)max_kv > (int64_t)max_pages * c->page_size) return QV_EINVAL;
+    const int64_t per16 = 16 / (int64_t)elt_size(c->dtype);
+    if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) || q_stride % per16 ||
+        q_stride < (int64_t)q_heads * c->head_dim)
+        return QV_EINVAL;
+    const int G = q_heads / c->kv_heads;
+    const PagedPlan p = paged_plan(batch, c->kv_heads, G, total_q, max_q, max_kv);
+    const size_t need = paged_ws_bytes(p, total_q, q_heads, c->head_dim);
+    if (need > workspace_bytes) return QV_ESPACE;
+    if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return QV_EINVAL;
+    PagedArgs a = {};
+    a.k = c->k; a.v = c->v; a.k_scale = c->k_scale; a.v_scale = c->v_scale; a.err = c->err;
+    a.block_table = block_table; a.kv_lens = kv_lens; a.cu_q = cu_q; a.q = q; a.out = out;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)p.splits * total_q * q_heads * c->head_dim;
+    a.q_stride = q_stride; a.pages = c->pages; a.H = c->kv_heads; a.G = G; a.page_shift = paged_shift(c->page_size);
+    a.max_pages = max_pages; a.B = batch; a.total_q = total_q; a.max_q = max_q; a.max_kv = max_kv; a.causal = causal != 0;
+    a.splits = p.splits; a.chunk = p.chunk;
+    a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+    const bool q8 = c->bits == 8;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (c->head_dim == 128) {
+        if (c->dtype == QV_F32) return paged_launch<QV_F32, 128>(a, p, q8, s);
+        if (c->dtype == QV_BF16) return paged_launch<QV_BF16, 128>(a, p, q8, s);
+        return paged_launch<QV_F16, 128>(a, p, q8, s);
+    }
+    if (c->dtype == QV_F32) return paged_launch<QV_F32, 64>(a, p, q8, s);
+    if (c->dtype == QV_BF16) return paged_launch<QV_BF16, 64>(a, p, q8, s);
+    return paged_launch<QV_F16, 64>(a, p, q8, s);
+}

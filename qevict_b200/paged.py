@@ -1,0 +1,316 @@
+"""Paged KV cache: full-context K/V of many sequences in pages of one pool.
+
+For prompts that arrive in chunks and for full-cache decode, beside the
+Sticky layout (which keeps a selected part of one prompt).  Four operators of
+the native library, each an ordinary kernel launch on the current stream of its
+tensors' device, none of which synchronises:
+
+  qk_norm_rope     per-head norm and rotation of query and key heads
+  paged_append     the same, with the new keys and values written into pages
+  paged_gather     pages read back into contiguous rows (what
+                   model.prefill_attention and StickyLayerState.prefill take)
+  paged_attention  chunks of new tokens, from one token to whole prompts,
+                   over the pages
+
+PagedKVCache holds a pool and calls them.  Pools are [pages, kv_heads,
+page_size, head_dim] in the model's dtype or INT8 with one fp32 scale per row
+([pages, kv_heads, page_size]); token j of sequence b lives in page
+block_table[b, j // page_size] at offset j % page_size.
+"""
+
+import ctypes
+import math
+
+import torch
+
+from . import _native as N
+
+_DTYPES = {torch.float32: N.QV_F32, torch.bfloat16: N.QV_BF16, torch.float16: N.QV_F16}
+
+
+def rope_table(max_pos, rot_dim, theta=10000.0, scaling=None, device="cuda"):
+    """The fp32 rotation table [max_pos, rot_dim]: cos | sin, angles in 64 bits.
+
+    scaling (long contexts), a dict with "type" and "factor" f:
+      linear  positions divided by f
+      ntk     theta * f^(r / (r - 2)): the slowest pair turns f times slower, the fastest as before
+      llama3  frequencies divided by f where the wavelength is above
+              original_max_position / low_freq_factor, kept where below
+              original_max_position / high_freq_factor, blended between
+      yarn    divided by f below beta_slow turns over original_max_position, kept above
+              beta_fast, a linear ramp over the pairs between; cos and sin times
+              attention_factor (default 0.1 ln f + 1)"""
+    if max_pos <= 0 or rot_dim < 8 or rot_dim % 8:
+        raise N.QevictError("rope_table: max_pos > 0 and rot_dim a positive multiple of 8 are needed")
+    dev = torch.device(device)
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64, device=dev)
+    mult = 1.0
+    if scaling is None:
+        inv = theta ** (-i / rot_dim)
+    else:
+        kind, f = scaling["type"], float(scaling["factor"])
+        if kind == "ntk":
+            theta = theta * f ** (rot_dim / (rot_dim - 2))
+        inv = theta ** (-i / rot_dim)
+        if kind == "linear":
+            inv = inv / f
+        elif kind == "llama3":
+            lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+            turns = float(scaling["original_max_position"]) * inv / (2 * math.pi)
+            keep = ((turns - lo) / (hi - lo)).clamp(0, 1)
+            inv = inv / f * (1 - keep) + inv * keep
+        elif kind == "yarn":
+            orig = float(scaling["original_max_position"])
+
+            def pair(turns):   # the (fractional) pair that turns this often over the original length
+                return rot_dim * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(theta))
+            lo = max(math.floor(pair(float(scaling.get("beta_fast", 32)))), 0)
+            hi = min(math.ceil(pair(float(scaling.get("beta_slow", 1)))), rot_dim - 1)
+            ramp = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+            inv = inv * (1 - ramp) + inv / f * ramp
+            mult = float(scaling.get("attention_factor") or 0.1 * math.log(f) + 1.0)
+        elif kind != "ntk":
+            raise N.QevictError(f"rope_table: unknown scaling type {kind!r}")
+    a = torch.arange(max_pos, dtype=torch.float64, device=dev)[:, None] * inv
+    return (torch.cat([a.cos(), a.sin()], 1) * mult).float()
+
+
+def _need(ok, what):
+    if not ok:
+        raise N.QevictError(what)
+
+
+def _heads(name, x, tokens, dim, dtype, dev):
+    """A [tokens, heads, head_dim] tensor whose heads are contiguous within a token (a view of a
+    packed projection will do); returns its token stride."""
+    _need(x.dim() == 3 and x.shape[2] == dim and (tokens is None or x.shape[0] == tokens) and x.dtype == dtype
+          and x.device == dev, f"{name}: expected [tokens, heads, {dim}] {dtype} on {dev}, got "
+          f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    st = x.stride()
+    h = x.shape[1]
+    _need((st[2] == 1 or dim == 1) and (st[1] == dim or h == 1), f"{name}: a token's heads must be contiguous")
+    return st[0] if x.shape[0] > 1 else h * dim
+
+
+def _vector(name, x, shape, dtype, dev):
+    _need(x.dtype == dtype and tuple(x.shape) == shape and x.is_contiguous() and x.device == dev,
+          f"{name}: expected a contiguous {shape} {dtype} tensor on {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(dev, name, *args):
+    """Call a native entry point on the current stream of `dev`."""
+    fn = getattr(N.lib(), name)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    N.check(rc, name)
+
+
+def _pool(k_pages, v_pages, k_scale, v_scale, dtype, err):
+    """The native descriptor of a pool (checked)."""
+    _need(dtype in _DTYPES, f"dtype {dtype} is not one of fp32, bf16, fp16")
+    _need(k_pages.is_cuda, "pages must be on a CUDA device")
+    dev = k_pages.device
+    _need(k_pages.dim() == 4 and v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype
+          and v_pages.device == dev and k_pages.is_contiguous() and v_pages.is_contiguous(),
+          "pages: k and v must be contiguous [pages, kv_heads, page_size, head_dim] tensors of one type and device")
+    P, H, S, D = k_pages.shape
+    _need(S in (16, 32, 64, 128), f"page_size {S} is not 16, 32, 64 or 128")
+    _need(8 <= D <= 256 and D % 8 == 0, f"head_dim {D} is not a multiple of 8 up to 256")
+    q8 = k_pages.dtype == torch.int8
+    _need(q8 or k_pages.dtype == dtype, f"pages of {k_pages.dtype} do not go with {dtype} rows")
+    if q8:
+        _need(k_scale is not None and v_scale is not None, "INT8 pages need k_scale and v_scale")
+        _vector("k_scale", k_scale, (P, H, S), torch.float32, dev)
+        _vector("v_scale", v_scale, (P, H, S), torch.float32, dev)
+    else:
+        _need(k_scale is None and v_scale is None, "k_scale and v_scale go with INT8 pages only")
+    if err is not None:
+        _vector("err", err, (1,), torch.int32, dev)
+    return N.QvPagedCache(k_pages.data_ptr(), v_pages.data_ptr(), _p(k_scale), _p(v_scale), _p(err), P, H, S, D,
+                          _DTYPES[dtype], 8 if q8 else 0)
+
+
+def _turn(tokens, dim, dtype, dev, positions, table, q_weight, k_weight):
+    """Checked (max_pos, rot_dim) of the rotation, and the norm weights."""
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _vector(name, w, (dim,), dtype, dev)
+    if table is None:
+        return 0, 0
+    _need(table.dim() == 2 and table.dtype == torch.float32 and table.is_contiguous() and table.device == dev,
+          "table: expected a contiguous [max_pos, rot_dim] fp32 tensor (rope_table)")
+    max_pos, rot = table.shape
+    _need(8 <= rot <= dim and rot % 8 == 0, f"table: rot_dim {rot} is not a multiple of 8 up to head_dim {dim}")
+    _need(positions is not None, "a rotation needs positions")
+    _vector("positions", positions, (tokens,), torch.int32, dev)
+    return max_pos, rot
+
+
+def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
+                 out=None):
+    """RMS norm (where a weight is given) and rotation (where a table is) of each query and key head.
+
+    q [T, q_heads, D], k [T, kv_heads, D], heads contiguous within a token; positions [T] int32; table from
+    rope_table, its rot_dim the part of the head that turns, in pairs (i, i + rot_dim/2), or (2i, 2i+1) with
+    interleaved.  Returns contiguous (q, k), or fills out=(q_out, k_out), which may be q and k themselves
+    where those are contiguous.  A position outside the table gives NaN.  (qv_qk_norm_rope)"""
+    _need(q.is_cuda and q.dtype in _DTYPES and q.dim() == 3, "q: expected a [tokens, heads, head_dim] fp32, bf16 or "
+          "fp16 CUDA tensor")
+    T, Hq, D = q.shape
+    dev, dt = q.device, q.dtype
+    _need(8 <= D <= 256 and D % 8 == 0, f"head_dim {D} is not a multiple of 8 up to 256")
+    qs, ks = _heads("q", q, T, D, dt, dev), _heads("k", k, T, D, dt, dev)
+    H = k.shape[1]
+    max_pos, rot = _turn(T, D, dt, dev, positions, table, q_weight, k_weight)
+    if out is None:
+        qo = torch.empty(T, Hq, D, dtype=dt, device=dev)
+        ko = torch.empty(T, H, D, dtype=dt, device=dev)
+    else:
+        qo, ko = out
+        _vector("out[0]", qo, (T, Hq, D), dt, dev)
+        _vector("out[1]", ko, (T, H, D), dt, dev)
+    _launch(dev, "qv_qk_norm_rope", T, Hq, H, D, _DTYPES[dt], q.data_ptr(), qs, k.data_ptr(), ks, _p(q_weight),
+            _p(k_weight), eps, _p(table), max_pos, rot, int(interleaved), _p(positions), qo.data_ptr(), ko.data_ptr())
+    return qo, ko
+
+
+def paged_append(q, k, v, slots, positions, table, k_pages, v_pages, *, k_scale=None, v_scale=None, q_weight=None,
+                 k_weight=None, eps=1e-6, interleaved=False, q_out=None, err=None):
+    """qk_norm_rope with the keys and the values v [T, kv_heads, D] written into the pool: token t to slots[t]
+    (int64, page * page_size + offset; negative: not written).  Returns the queries.  INT8 pages get
+    scale = max|row| / 127 and code = rint(row / scale) of the fp32 row.  A slot must appear at most once per
+    call; err collects device errors (PagedKVCache.read_error).  (qv_paged_append)"""
+    c = _pool(k_pages, v_pages, k_scale, v_scale, q.dtype, err)
+    dev, dt, H, D = k_pages.device, q.dtype, k_pages.shape[1], k_pages.shape[3]
+    qs = _heads("q", q, None, D, dt, dev)
+    T, Hq = q.shape[0], q.shape[1]
+    ks, vs = _heads("k", k, T, D, dt, dev), _heads("v", v, T, D, dt, dev)
+    _need(k.shape[1] == H and v.shape[1] == H, f"k and v must have the pool's {H} heads")
+    _vector("slots", slots, (T,), torch.int64, dev)
+    max_pos, rot = _turn(T, D, dt, dev, positions, table, q_weight, k_weight)
+    if q_out is None:
+        q_out = torch.empty(T, Hq, D, dtype=dt, device=dev)
+    else:
+        _vector("q_out", q_out, (T, Hq, D), dt, dev)
+    _launch(dev, "qv_paged_append", ctypes.byref(c), T, Hq, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+            _p(q_weight), _p(k_weight), eps, _p(table), max_pos, rot, int(interleaved),
+            _p(positions) if table is not None else None, slots.data_ptr(), q_out.data_ptr())
+    return q_out
+
+
+def _tables(block_table, kv_lens, cu, dev):
+    _need(block_table.dim() == 2 and block_table.shape[1] > 0, "block_table: expected [batch, max_pages]")
+    B, width = block_table.shape
+    _vector("block_table", block_table, (B, width), torch.int32, dev)
+    _vector("kv_lens", kv_lens, (B,), torch.int32, dev)
+    _vector("cumulative lengths", cu, (B + 1,), torch.int32, dev)
+    return B, width
+
+
+def paged_gather(k_pages, v_pages, block_table, kv_lens, cu_kv, total, *, k_scale=None, v_scale=None, dtype=None,
+                 out=None, err=None):
+    """The cached rows as contiguous (k, v) [total, kv_heads, D] in dtype (default: the pages' own; INT8 pages
+    need it): the first kv_lens[b] tokens of sequence b from row cu_kv[b] on, cu_kv [batch + 1] ascending int32;
+    rows of no sequence are left as they were (out) or undefined.  (qv_paged_gather)"""
+    dt = k_pages.dtype if dtype is None else dtype
+    c = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
+    dev, H, D = k_pages.device, k_pages.shape[1], k_pages.shape[3]
+    B, width = _tables(block_table, kv_lens, cu_kv, dev)
+    _need(total >= 0, "total must not be negative")
+    if out is None:
+        ko = torch.empty(total, H, D, dtype=dt, device=dev)
+        vo = torch.empty(total, H, D, dtype=dt, device=dev)
+    else:
+        ko, vo = out
+        _vector("out[0]", ko, (total, H, D), dt, dev)
+        _vector("out[1]", vo, (total, H, D), dt, dev)
+    _launch(dev, "qv_paged_gather", ctypes.byref(c), B, block_table.data_ptr(), width, kv_lens.data_ptr(),
+            cu_kv.data_ptr(), total, ko.data_ptr(), vo.data_ptr())
+    return ko, vo
+
+
+def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=None, v_scale=None, causal=True,
+                    scale=None, max_q=None, max_kv=None, out=None, err=None):
+    """Attention of chunks of new tokens over the pool.
+
+    q [T, q_heads, D] (heads contiguous within a token), D 64 or 128, q_heads a multiple (up to 16 times) of
+    kv_heads; sequence b's new tokens are rows cu_q[b] .. cu_q[b+1] (int32 [batch + 1]) and the last of its
+    kv_lens[b] (int32 [batch]) cached tokens; block_table int32 [batch, max_pages].  Causal: each token sees the
+    keys up to its own.  A row that sees no key gives 0; rows of no chunk are left as they were (out) or
+    undefined.  max_q / max_kv: upper bounds of the chunk and cached lengths, which size the launch (default:
+    T, and all that the block table can hold); a captured call serves any lengths below them.  scale
+    defaults to D^-1/2.  (qv_paged_attention)"""
+    c = _pool(k_pages, v_pages, k_scale, v_scale, q.dtype, err)
+    dev, dt, H, S, D = k_pages.device, q.dtype, k_pages.shape[1], k_pages.shape[2], k_pages.shape[3]
+    _need(D in (64, 128), f"head_dim {D} is not 64 or 128")
+    qs = _heads("q", q, None, D, dt, dev)
+    T, Hq = q.shape[0], q.shape[1]
+    _need(Hq % H == 0 and Hq // H <= 16, f"{Hq} query heads are not 1 to 16 times the pool's {H}")
+    B, width = _tables(block_table, kv_lens, cu_q, dev)
+    max_q = T if max_q is None else max_q
+    max_kv = width * S if max_kv is None else max_kv
+    _need(0 <= max_q and 0 <= max_kv <= width * S, f"max_q {max_q} and max_kv {max_kv} must be lengths, max_kv at most "
+          f"the block table's {width * S}")
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=dt, device=dev)
+    else:
+        _vector("out", out, (T, Hq, D), dt, dev)
+    cp = ctypes.byref(c)
+    wsb = N.lib().qv_paged_attention_workspace_bytes(cp, B, Hq, T, max_q, max_kv)
+    # from torch's allocator at each call: a captured graph gets one of its own
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    _launch(dev, "qv_paged_attention", cp, B, Hq, block_table.data_ptr(), width, kv_lens.data_ptr(), cu_q.data_ptr(),
+            T, max_q, max_kv, q.data_ptr(), qs, 1.0 / math.sqrt(D) if scale is None else scale, int(causal),
+            out.data_ptr(), _p(ws), wsb)
+    return out
+
+
+class PagedKVCache:
+    """A pool of pages for one layer, and the operators on it.
+
+    bits = 16 keeps pages in dtype, 8 in INT8 with fp32 row scales (fp32 pools: 32 or 8).  Which pages a
+    sequence owns is the caller's: block_table [batch, max_pages] int32 on the pool's device."""
+
+    def __init__(self, pages, kv_heads, head_dim, page_size=64, dtype=torch.bfloat16, bits=None, device="cuda"):
+        _need(dtype in _DTYPES, f"dtype {dtype} is not one of fp32, bf16, fp16")
+        full = torch.finfo(dtype).bits
+        bits = full if bits is None else bits
+        _need(bits in (8, full), f"bits {bits} is not 8 or the dtype's own {full}")
+        _need(pages > 0 and kv_heads > 0, "a pool needs pages and heads")
+        self.dtype, self.page_size = dtype, page_size
+        shape = (pages, kv_heads, page_size, head_dim)
+        self.k_pages = torch.zeros(shape, dtype=torch.int8 if bits == 8 else dtype, device=device)
+        self.v_pages = torch.zeros_like(self.k_pages)
+        self.k_scale = torch.zeros(shape[:3], dtype=torch.float32, device=device) if bits == 8 else None
+        self.v_scale = torch.zeros_like(self.k_scale) if bits == 8 else None
+        self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        _pool(self.k_pages, self.v_pages, self.k_scale, self.v_scale, dtype, self.err)
+
+    def slots(self, block_table, seq, pos):
+        """Slots of tokens at index pos [T] of sequences seq [T] (int64 [T])."""
+        pos = pos.long()
+        page = torch.div(pos, self.page_size, rounding_mode="floor")
+        return block_table[seq.long(), page].long() * self.page_size + pos % self.page_size
+
+    def append(self, q, k, v, slots, positions=None, table=None, **kw):
+        return paged_append(q, k, v, slots, positions, table, self.k_pages, self.v_pages, k_scale=self.k_scale,
+                            v_scale=self.v_scale, err=self.err, **kw)
+
+    def gather(self, block_table, kv_lens, cu_kv, total, **kw):
+        return paged_gather(self.k_pages, self.v_pages, block_table, kv_lens, cu_kv, total, k_scale=self.k_scale,
+                            v_scale=self.v_scale, dtype=self.dtype, err=self.err, **kw)
+
+    def attend(self, q, block_table, kv_lens, cu_q, **kw):
+        return paged_attention(q, self.k_pages, self.v_pages, block_table, kv_lens, cu_q, k_scale=self.k_scale,
+                               v_scale=self.v_scale, err=self.err, **kw)
+
+    def read_error(self):
+        """The device error word (a synchronisation): bits QV_DERR_TABLE, QV_DERR_CAPACITY, QV_DERR_TIMEOUT."""
+        return int(self.err.item())

@@ -1,0 +1,657 @@
+"""Paged KV cache: norm + rotation, append, read-back and attention against
+their definitions in 64 bits.
+
+Bounds: a result rounded to a type t is off by eps(t)/2 of its value; what the
+kernels do in fp32 before that adds a few 2^-24 of the terms' magnitudes, which
+each bound below spells out.
+"""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from qevict_b200 import _native as N
+from qevict_b200 import paged
+
+DEV = "cuda"
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+TINY = {BF16: 2.0 ** -134, FP16: 2.0 ** -25, FP32: 2.0 ** -149}   # half a subnormal step
+
+
+def half(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def rand(g, *shape, std=1.0):
+    return torch.randn(*shape, generator=g, device=DEV) * std
+
+
+# ------------------------------------------------------------------ definitions
+def ref_heads(x, w, eps, table, pos, interleaved):
+    """Norm and rotation in 64 bits: (value, magnitude of the terms it sums)."""
+    x = x.double()
+    if w is not None:
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * w.double()
+    y, mag = x.clone(), x.abs()
+    if table is not None:
+        r = table.shape[1]
+        c, s = table[pos.long()].double()[:, None].chunk(2, -1)
+        i = torch.arange(r // 2, device=x.device)
+        a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + r // 2)
+        y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., b] * c + x[..., a] * s
+        both = x[..., a].abs() + x[..., b].abs()
+        mag = mag.clone()
+        mag[..., a], mag[..., b] = both, both
+    return y, mag
+
+
+def close_rows(got, ref, mag, dt):
+    # fp32 steps: the mean of squares (pairwise, below 16 ulp), rsqrt, two products, two of the rotation: 2^-19 of the terms
+    bound = ref.abs() * half(dt) * 1.001 + mag * 2.0 ** -19 + TINY[dt]
+    assert got.dtype == dt
+    assert bool(((got.double() - ref).abs() <= bound).all()), float(((got.double() - ref).abs() / bound).max())
+
+
+def ref_attention(q, ks, vs, causal=True, scale=None):
+    """q [n, Hq, D]; ks, vs [L, H, D] in 64 bits -> (out, sum of p |v|, largest |q||k| scale)."""
+    n, Hq, D = q.shape
+    L, H = ks.shape[:2]
+    scale = D ** -0.5 if scale is None else scale
+    q = q.double().view(n, H, Hq // H, D)
+    if L == 0:
+        z = torch.zeros(n, Hq, D, dtype=torch.float64, device=q.device)
+        return z, z, 0.0
+    x = torch.einsum("nhgd,lhd->hgnl", q, ks) * scale
+    if causal:
+        seen = torch.arange(L, device=q.device)[None] <= torch.arange(L - n, L, device=q.device)[:, None]
+        x = x.masked_fill(~seen, -math.inf)
+    p = torch.exp(x - x.amax(-1, keepdim=True).clamp(min=-1e300))
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+    out = torch.einsum("hgnl,lhd->nhgd", p, vs).reshape(n, Hq, D)
+    mag = torch.einsum("hgnl,lhd->nhgd", p, vs.abs()).reshape(n, Hq, D)
+    big = float(q.norm(dim=-1).max() * ks.norm(dim=-1).max()) * abs(scale)
+    return out, mag, big
+
+
+def attention_bound(out, mag, big, L, D, dt, vmax):
+    """The output's rounding; each probability's rounding to the type (with the value scale of an INT8 row in it);
+    fp32 logits (D terms of size up to |q||k|, an exponent's error is relative to p) and sums over L keys; and, in
+    fp16, probabilities below its smallest normal: half a step of 2^-24 each against a sum of at least 1."""
+    delta = 2.0 ** -24 * (2 * (D + 8) * big + L + 64)
+    b = out.abs() * half(dt) * 1.001 + mag * (half(dt) + delta) * 1.01 + TINY[dt]
+    return b + (L * 2.0 ** -25 * vmax if dt == FP16 else 0.0)
+
+
+class Pool:
+    """A pool with `lens` tokens per sequence in pages of random order; every slot that no sequence owns holds
+    NaN (in INT8 pools its scale), and the block table's unused entries ids outside the pool."""
+
+    def __init__(self, g, lens, H, D, page, dt, q8, extra=3, std=1.0):
+        need = [-(-n // page) for n in lens]
+        P, B = sum(need) + extra, len(lens)
+        self.cache = paged.PagedKVCache(P, H, D, page, dt, bits=8 if q8 else None, device=DEV)
+        c = self.cache
+        ids = torch.randperm(P, generator=g, device=DEV)[: sum(need)].tolist()
+        width = max(1, max(need, default=1))
+        bt = torch.full((B, width), -7, dtype=torch.int32)
+        bt[:, 1::2] = 2 ** 31 - 1
+        for b in range(B):
+            for i in range(need[b]):
+                bt[b, i] = ids.pop()
+        self.bt = bt.to(DEV)
+        self.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        self.ks, self.vs = [], []
+        for x in (c.k_pages, c.v_pages):
+            x.fill_(127 if q8 else math.nan)
+        if q8:
+            c.k_scale.fill_(math.nan)
+            c.v_scale.fill_(math.nan)
+        for b, n in enumerate(lens):
+            pos = torch.arange(n, device=DEV)
+            sl = c.slots(self.bt, torch.full_like(pos, b), pos)
+            pg, off = sl // page, sl % page
+            for x, sc, keep in ((c.k_pages, c.k_scale, self.ks), (c.v_pages, c.v_scale, self.vs)):
+                rows = rand(g, n, H, D, std=std)
+                if q8:
+                    s = rows.abs().amax(-1) / 127
+                    code = (rows / s[..., None]).round()
+                    x[pg, :, off] = code.to(torch.int8)
+                    sc[pg, :, off] = s
+                    keep.append(code.double() * s.double()[..., None])
+                else:
+                    x[pg, :, off] = rows.to(dt)
+                    keep.append(rows.to(dt).double())
+
+
+def cu(lens):
+    return torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32, device=DEV)
+
+
+def check_attention(g, q_lens, kv_lens, Hq, H, D, page, dt, q8, causal=True, scale=None, std=1.0, qstd=1.0, **kw):
+    pool = Pool(g, kv_lens, H, D, page, dt, q8, std=std)
+    T = sum(q_lens)
+    qkv = rand(g, T + 2, Hq + 2 * H, D, std=qstd).to(dt)    # two rows of padding behind the last sequence
+    q = qkv[:, :Hq]
+    out = torch.full((T + 2, Hq, D), 7.0, dtype=dt, device=DEV)
+    got = pool.cache.attend(q, pool.bt, pool.lens, cu(q_lens), causal=causal, scale=scale, out=out, **kw)
+    assert got is out and pool.cache.read_error() == 0
+    assert bool((out[T:] == 7).all())
+    at = 0
+    for b, n in enumerate(q_lens):
+        if n:
+            o, mag, big = ref_attention(q[at:at + n], pool.ks[b], pool.vs[b], causal, scale)
+            vmax = float(pool.vs[b].abs().max()) if kv_lens[b] else 0.0
+            bound = attention_bound(o, mag, big, kv_lens[b], D, dt, vmax)
+            d = (out[at:at + n].double() - o).abs()
+            assert bool((d <= bound).all()), (b, n, kv_lens[b], float((d / bound).max()))
+        at += n
+    return pool, q, out
+
+
+# ------------------------------------------------------------------ CPU: tables, refusals
+@pytest.mark.parametrize("scaling,hf", [
+    (None, None),
+    (dict(type="linear", factor=4.0), dict(rope_type="linear", factor=4.0)),
+    (dict(type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position=8192),
+     dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+          original_max_position_embeddings=8192)),
+    (dict(type="yarn", factor=16.0, original_max_position=4096),
+     dict(rope_type="yarn", factor=16.0, original_max_position_embeddings=4096)),
+])
+def test_rope_table_against_transformers(scaling, hf):
+    from transformers import LlamaConfig
+    from transformers.models.llama.modeling_llama import LlamaRotaryEmbedding
+    theta, D, n = 500000.0, 128, 4096
+    rp = dict(hf or dict(rope_type="default"), rope_theta=theta)
+    conf = LlamaConfig(hidden_size=D * 2, num_attention_heads=2, head_dim=D, rope_theta=theta, rope_scaling=rp,
+                       rope_parameters=rp, max_position_embeddings=65536)
+    cos, sin = LlamaRotaryEmbedding(conf)(torch.zeros(1), torch.arange(n)[None])
+    t = paged.rope_table(n, D, theta, scaling, device="cpu")
+    # theirs multiplies fp32 frequencies (three roundings) by the position: an angle off by 2^-22 of itself
+    bound = (2.0 ** -22 * torch.arange(n)[:, None] + 2.0 ** -22) * 1.5
+    assert bool(((t[:, : D // 2] - cos[0, :, : D // 2]).abs() <= bound).all())
+    assert bool(((t[:, D // 2:] - sin[0, :, : D // 2]).abs() <= bound).all())
+
+
+def test_rope_table_ntk_keeps_the_fastest_pair_and_stretches_the_slowest():
+    f, D, theta = 8.0, 64, 10000.0
+    a = paged.rope_table(3, D, theta, device="cpu").double()
+    b = paged.rope_table(3, D, theta, dict(type="ntk", factor=f), device="cpu").double()
+    assert torch.equal(a[:, 0], b[:, 0])
+    slow = theta ** (-(D - 2) / D)
+    assert abs(float(torch.asin(b[1, -1])) - slow / f) <= slow * 2.0 ** -23
+    with pytest.raises(N.QevictError):
+        paged.rope_table(3, D, theta, dict(type="other", factor=f), device="cpu")
+    with pytest.raises(N.QevictError):
+        paged.rope_table(3, 12, theta, device="cpu")
+
+
+def test_python_refusals_without_a_gpu():
+    x = torch.zeros(2, 4, 64)
+    with pytest.raises(N.QevictError):
+        paged.qk_norm_rope(x, x)
+    pages = torch.zeros(2, 1, 16, 64)
+    i = torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(N.QevictError):
+        paged.paged_append(x, x, x, i, None, None, pages, pages)
+    with pytest.raises(N.QevictError):
+        paged.paged_gather(pages, pages, i, i[0], i[0], 0)
+    with pytest.raises(N.QevictError):
+        paged.paged_attention(x, pages, pages, i, i[0], i[0])
+    for bad in (dict(bits=4), dict(dtype=torch.float64), dict(page_size=48), dict(pages=0), dict(head_dim=20)):
+        with pytest.raises(N.QevictError):
+            paged.PagedKVCache(**{**dict(pages=2, kv_heads=1, head_dim=64, page_size=16, device="cpu"), **bad})
+
+
+FAKE = 1 << 20   # an aligned address that no refused call touches
+
+
+def cache_desc(**kw):
+    d = dict(k=FAKE, v=FAKE, k_scale=None, v_scale=None, err=None, pages=4, kv_heads=2, page_size=16, head_dim=64,
+             dtype=N.QV_BF16, bits=0)
+    d.update(kw)
+    return N.QvPagedCache(*d.values())
+
+
+BAD_CACHES = [dict(k=None), dict(v=FAKE + 8), dict(pages=0), dict(kv_heads=0), dict(page_size=48), dict(head_dim=60),
+              dict(head_dim=264), dict(dtype=3), dict(bits=4), dict(bits=8)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES)
+def test_native_refuses_bad_caches(bad):
+    L, c = N.lib(), ctypes.byref(cache_desc(**bad))
+    assert L.qv_paged_gather(c, 1, FAKE, 1, FAKE, FAKE, 1, FAKE, FAKE, None) == N.QV_EINVAL
+    assert L.qv_paged_append(c, 1, 2, FAKE, 128, FAKE, 128, FAKE, 128, None, None, 0.0, None, 0, 0, 0, None, FAKE,
+                             FAKE, None) == N.QV_EINVAL
+    assert L.qv_paged_attention(c, 1, 2, FAKE, 1, FAKE, FAKE, 1, 1, 16, FAKE, 128, 1.0, 1, FAKE, None, 0,
+                                None) == N.QV_EINVAL
+    assert L.qv_paged_attention_workspace_bytes(c, 1, 2, 1, 1, 16) == 0
+
+
+def test_native_refuses_bad_arguments():
+    L, c = N.lib(), ctypes.byref(cache_desc())
+
+    def attn(batch=1, heads=4, bt=FAKE, width=2, lens=FAKE, cuq=FAKE, total=1, mq=1, mkv=32, q=FAKE, qs=256, out=FAKE,
+             ws=None, wsb=0, cache=c):
+        return L.qv_paged_attention(cache, batch, heads, bt, width, lens, cuq, total, mq, mkv, q, qs, 1.0, 1, out, ws,
+                                    wsb, None)
+    for bad in (dict(batch=-1), dict(heads=3), dict(heads=34), dict(heads=0), dict(bt=None), dict(width=0),
+                dict(lens=None), dict(cuq=None), dict(total=-1), dict(mq=-1), dict(mkv=-1), dict(mkv=33), dict(q=None),
+                dict(q=FAKE + 2), dict(qs=255), dict(qs=260), dict(out=None), dict(out=FAKE + 8),
+                dict(cache=ctypes.byref(cache_desc(head_dim=96)))):
+        assert attn(**bad) == N.QV_EINVAL, bad
+    assert attn(batch=0) == attn(total=0) == attn(mq=0) == N.QV_OK
+    # a call that needs a workspace and gets none, or too little
+    need = L.qv_paged_attention_workspace_bytes(c, 1, 4, 1, 1, 32768)
+    assert need > 0
+    assert attn(width=4096, mkv=32768) == N.QV_ESPACE
+    assert attn(width=4096, mkv=32768, ws=FAKE, wsb=need - 1) == N.QV_ESPACE
+    assert attn(width=4096, mkv=32768, ws=FAKE + 4, wsb=need) == N.QV_EINVAL
+
+    def rope(T=1, Hq=2, H=1, D=64, dt=N.QV_BF16, q=FAKE, qs=128, k=FAKE, ks=64, qw=None, table=FAKE, mp=8, rot=64,
+             pos=FAKE, qo=FAKE, ko=FAKE):
+        return L.qv_qk_norm_rope(T, Hq, H, D, dt, q, qs, k, ks, qw, None, 0.0, table, mp, rot, 0, pos, qo, ko, None)
+    for bad in (dict(T=-1), dict(Hq=0), dict(H=0), dict(D=4), dict(D=260), dict(D=60), dict(dt=7), dict(q=None),
+                dict(q=FAKE + 4), dict(qs=100), dict(qs=132), dict(k=None), dict(ks=32), dict(qw=FAKE + 2), dict(mp=0),
+                dict(rot=12), dict(rot=72), dict(rot=0), dict(pos=None), dict(qo=None), dict(ko=None),
+                dict(ko=FAKE + 8), dict(table=FAKE + 4)):
+        assert rope(**bad) == N.QV_EINVAL, bad
+    assert rope(T=0) == N.QV_OK
+    assert L.qv_paged_append(c, 1, 2, FAKE, 128, FAKE, 128, FAKE, 128, None, None, 0.0, None, 0, 0, 0, None, None,
+                             FAKE, None) == N.QV_EINVAL
+    assert L.qv_paged_append(c, 1, 2, FAKE, 128, FAKE, 128, None, 128, None, None, 0.0, None, 0, 0, 0, None, FAKE,
+                             FAKE, None) == N.QV_EINVAL
+    assert L.qv_paged_gather(c, 1, FAKE, 0, FAKE, FAKE, 1, FAKE, FAKE, None) == N.QV_EINVAL
+    assert L.qv_paged_gather(c, 1, FAKE, 1, FAKE, FAKE, 1, FAKE, FAKE + 8, None) == N.QV_EINVAL
+    assert L.qv_paged_gather(c, 0, None, 0, None, None, 0, None, None, None) == N.QV_OK
+
+
+# ------------------------------------------------------------------ norm + rotation
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T,Hq,H,D,rot,norm,dt", [
+    (1, 32, 8, 128, 128, False, BF16), (3, 5, 1, 64, 64, True, FP16), (7, 4, 4, 128, 64, True, BF16),
+    (2, 3, 1, 128, 8, False, FP32), (5, 20, 4, 256, 256, True, FP32), (9, 2, 2, 80, 40, True, BF16),
+    (4, 2, 2, 80, 80, False, FP16), (6, 7, 1, 96, 24, True, FP32), (257, 33, 3, 64, 32, True, BF16),
+    (2, 1, 1, 8, 8, True, FP32), (3, 70, 2, 256, 200, False, BF16), (4, 4, 2, 64, 0, True, FP16)])
+def test_qk_norm_rope(T, Hq, H, D, rot, norm, dt, interleaved):
+    g = gen(T * 1000 + D + rot)
+    qkv = rand(g, T, (Hq + 2 * H) * D).to(dt)
+    q, k, _ = (x.view(T, -1, D) for x in qkv.split([Hq * D, H * D, H * D], 1))
+    table = paged.rope_table(5000, rot, 10000.0) if rot else None
+    pos = torch.randint(0, 5000, (T,), generator=g, device=DEV, dtype=torch.int32) if rot else None
+    qw = rand(g, D).to(dt) if norm else None
+    kw = rand(g, D).to(dt) if norm and T != 7 else None      # one case with a query weight alone
+    before = qkv.clone()
+    qo, ko = paged.qk_norm_rope(q, k, pos, table, q_weight=qw, k_weight=kw, eps=1e-5, interleaved=interleaved)
+    assert torch.equal(qkv, before) and qo.is_contiguous() and ko.is_contiguous()
+    close_rows(qo, *ref_heads(q, qw, 1e-5, table, pos, interleaved), dt)
+    close_rows(ko, *ref_heads(k, kw, 1e-5, table, pos, interleaved), dt)
+    # in place, where the inputs are contiguous
+    qc, kc = q.contiguous(), k.contiguous()
+    a, b = paged.qk_norm_rope(qc, kc, pos, table, q_weight=qw, k_weight=kw, eps=1e-5, interleaved=interleaved,
+                              out=(qc, kc))
+    assert a is qc and b is kc and torch.equal(a, qo) and torch.equal(b, ko)
+
+
+@pytest.mark.gpu
+def test_qk_norm_rope_edges():
+    g = gen(3)
+    table = paged.rope_table(16, 32)
+    q, k = rand(g, 4, 2, 64).to(BF16), rand(g, 4, 1, 64).to(BF16)
+    # a position outside the table shows as NaN in what turns, and nowhere else
+    pos = torch.tensor([0, 16, -1, 15], dtype=torch.int32, device=DEV)
+    qo, ko = paged.qk_norm_rope(q, k, pos, table)
+    for x in (qo, ko):
+        assert bool(x[1:3, :, :32].isnan().all()) and not bool(x[1:3, :, 32:].isnan().any())
+        assert not bool(x[[0, 3]].isnan().any())
+    # rows do not touch one another: a NaN row and an infinite one stay where they are; a zero row gives zero
+    q[1, 0], q[2, 1], q[3] = math.nan, math.inf, 0
+    w = torch.ones(64, dtype=BF16, device=DEV)
+    qo, _ = paged.qk_norm_rope(q, k, torch.zeros(4, dtype=torch.int32, device=DEV), table, q_weight=w, k_weight=w)
+    assert bool(qo[1, 0].isnan().all()) and not bool(qo[1, 1].isnan().any()) and not bool(qo[2, 0].isnan().any())
+    assert bool((qo[3] == 0).all())
+    e = torch.empty(0, 2, 64, dtype=BF16, device=DEV)
+    qo, ko = paged.qk_norm_rope(e, e, pos[:0], table)
+    assert qo.shape == (0, 2, 64) and ko.shape == (0, 2, 64)
+    for bad in (dict(q=q.float()), dict(k=k[:3]), dict(positions=pos.long()), dict(positions=pos[:2]),
+                dict(table=table.double()), dict(q=q.transpose(1, 2)), dict(q_weight=w.float()), dict(q_weight=w[:32]),
+                dict(out=(q, q)), dict(positions=None), dict(table=paged.rope_table(16, 128))):
+        with pytest.raises(N.QevictError):
+            paged.qk_norm_rope(**{**dict(q=q, k=k, positions=pos, table=table), **bad})
+
+
+# ------------------------------------------------------------------ append and read-back
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("lens,Hq,H,D,page,rot,norm,interleaved,dt", [
+    ([1], 32, 8, 128, 64, 128, False, False, BF16), ([5, 1, 33, 0, 16], 6, 2, 64, 16, 32, True, True, FP16),
+    ([130, 7], 4, 4, 128, 128, 64, True, False, BF16), ([40, 3, 64], 20, 4, 256, 32, 256, False, True, BF16),
+    ([17, 90], 3, 1, 80, 16, 40, True, False, FP32), ([1] * 70, 5, 5, 64, 32, 0, True, False, FP32)])
+def test_append_and_gather(lens, Hq, H, D, page, rot, norm, interleaved, dt, q8):
+    g = gen(sum(lens) + D)
+    T = sum(lens)
+    pool = Pool(g, lens, H, D, page, dt, q8)
+    c = pool.cache
+    for x in (c.k_pages, c.v_pages):
+        x.fill_(5)
+    qkv = rand(g, T, (Hq + 2 * H) * D, std=3.0).to(dt)
+    q, k, v = (x.view(T, -1, D) for x in qkv.split([Hq * D, H * D, H * D], 1))
+    table = paged.rope_table(300, rot) if rot else None
+    pos = torch.randint(0, 300, (T,), generator=g, device=DEV, dtype=torch.int32) if rot else None
+    w = rand(g, D).to(dt) if norm else None
+    seq = torch.repeat_interleave(torch.arange(len(lens), device=DEV), pool.lens.long())
+    at = torch.arange(T, device=DEV) - cu(lens).long()[seq]
+    slots = c.slots(pool.bt, seq, at)
+    skipped = torch.zeros(T, dtype=torch.bool, device=DEV)
+    if T > 4:
+        skipped[2] = True
+        slots[2] = -1
+    order = torch.randperm(T, generator=g, device=DEV)      # tokens of a call come in any order
+    qo = c.append(q[order], k[order], v[order], slots[order], None if pos is None else pos[order], table, q_weight=w,
+                  k_weight=w, interleaved=interleaved)
+    assert c.read_error() == 0
+    rq, mq = ref_heads(q, w, 1e-6, table, pos, interleaved)
+    close_rows(qo, rq[order], mq[order], dt)
+    # slots that were not written keep what they held
+    used = torch.zeros(c.k_pages.shape[0] * page, dtype=torch.bool, device=DEV)
+    used[slots[~skipped]] = True
+    flat = c.k_pages.transpose(1, 2).reshape(-1, H, D), c.v_pages.transpose(1, 2).reshape(-1, H, D)
+    for x in flat:
+        assert bool((x[~used] == 5).all())
+    total = T + 3
+    out = tuple(torch.full((total, H, D), 9.0, dtype=dt, device=DEV) for _ in range(2))
+    ko, vo = c.gather(pool.bt, pool.lens, cu(lens), total, out=out)
+    assert c.read_error() == 0 and bool((ko[T:] == 9).all()) and bool((vo[T:] == 9).all())
+    rk, mk = ref_heads(k, w, 1e-6, table, pos, interleaved)
+    for got, ref, mag in ((ko, rk, mk), (vo, v.double(), v.double().abs())):
+        got, ref, mag = got[:T][~skipped], ref[~skipped], mag[~skipped]
+        if not q8:
+            close_rows(got, ref, mag, dt)
+        else:
+            # half a step of max|row| / 127 (the step and the ratio in fp32), then the type's rounding
+            step = ref.abs().amax(-1, keepdim=True) / 127
+            bound = step * (0.5 + 127 * 2.0 ** -18) + got.double().abs() * half(dt) * 1.001 + mag * 2.0 ** -18 + TINY[dt]
+            assert bool(((got.double() - ref).abs() <= bound).all())
+    if q8:   # the stored codes and scales are what the read-back returns, exactly
+        kf, vf = (x.transpose(1, 2).reshape(-1, H, D)[slots[~skipped]] for x in (c.k_pages, c.v_pages))
+        s = c.k_scale.transpose(1, 2).reshape(-1, H)[slots[~skipped]]
+        assert torch.equal((kf.float() * s[..., None]).to(dt), ko[:T][~skipped])
+        assert int(kf.abs().max()) == 127
+
+
+@pytest.mark.gpu
+def test_append_edges():
+    g = gen(8)
+    c = paged.PagedKVCache(3, 1, 64, 16, BF16, bits=8)
+    q, k, v = (rand(g, 6, 1, 64).to(BF16) for _ in range(3))
+    k[1], k[2], k[3], k[4] = 0, math.nan, math.inf, 1e-38     # a zero row, two that are not finite, a tiny one
+    k[2, 0, 1:], k[3, 0, 1:] = 1, 1
+    c.append(q, k, v, torch.arange(6, device=DEV))
+    bt = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    n = torch.tensor([6], dtype=torch.int32, device=DEV)
+    ko, vo = c.gather(bt, n, cu([6]), 6)
+    assert bool((ko[1] == 0).all()) and bool(ko[2].isnan().all()) and bool(ko[3].isnan().all())
+    assert bool(((ko[4].double() - k[4].double()).abs() <= 1e-38 * (0.5 / 127 + half(BF16)) * 1.01).all())
+    assert not bool(ko[[0, 1, 4, 5]].isnan().any()) and not bool(vo.isnan().any()) and c.read_error() == 0
+    # a slot behind the pool, a position outside the table
+    c.append(q[:1], k[:1], v[:1], torch.tensor([48], device=DEV))
+    assert c.read_error() == N.QV_DERR_CAPACITY
+    c.err.zero_()
+    c.append(q[:1], k[:1], v[:1], torch.tensor([7], device=DEV), torch.tensor([9], dtype=torch.int32, device=DEV),
+             paged.rope_table(9, 64))
+    assert c.read_error() == N.QV_DERR_TABLE
+    c.err.zero_()
+    # read-back: a page id outside the pool, a length above the block table
+    out = tuple(torch.full((20, 1, 64), 4.0, dtype=BF16, device=DEV) for _ in range(2))
+    for page in (-1, 3, 2 ** 31 - 1):
+        c.gather(torch.tensor([[page]], dtype=torch.int32, device=DEV), n, cu([6]), 20, out=out)
+        assert c.read_error() == N.QV_DERR_TABLE and bool((out[0] == 4).all())
+        c.err.zero_()
+    c.gather(bt, torch.tensor([20], dtype=torch.int32, device=DEV), cu([20]), 20, out=out)
+    assert c.read_error() == N.QV_DERR_CAPACITY and bool((out[0][16:] == 4).all()) and not bool((out[0][:2] == 4).all())
+    e = torch.empty(0, 1, 64, dtype=BF16, device=DEV)
+    assert c.append(e, e, e, torch.empty(0, dtype=torch.int64, device=DEV)).shape == (0, 1, 64)
+    with pytest.raises(N.QevictError):
+        c.append(q, k, v, torch.arange(6, device=DEV, dtype=torch.int32))
+    with pytest.raises(N.QevictError):
+        c.append(q, k[:, :, :32], v, torch.arange(6, device=DEV))
+    with pytest.raises(N.QevictError):
+        c.append(q, k.expand(6, 2, 64), v, torch.arange(6, device=DEV))
+    with pytest.raises(N.QevictError):
+        paged.paged_gather(c.k_pages, c.v_pages, bt, n, cu([6]), 6, dtype=BF16)       # INT8 pages without scales
+
+
+# ------------------------------------------------------------------ attention
+SHAPES = [   # q_lens, kv_lens, Hq, H, D, page
+    ([1], [1], 4, 1, 64, 16),
+    ([1], [2000], 32, 8, 128, 64),                                     # one decode step, keys split over blocks
+    ([1, 1, 1, 0, 1, 1], [63, 64, 65, 12, 1, 700], 8, 2, 128, 32),     # decode of a ragged batch
+    ([1, 1], [5000, 3], 16, 1, 64, 128),
+    ([2, 3, 1], [300, 3, 129], 5, 1, 128, 16),                         # a few tokens each
+    ([16, 1, 4], [1000, 1, 90], 1, 1, 64, 16),
+    ([40, 0, 7], [40, 5, 900], 12, 4, 128, 64),
+    ([130], [130], 4, 4, 64, 32),                                      # a whole prompt
+    ([257, 64, 1, 33], [1025, 64, 500, 34], 8, 2, 128, 16),            # chunks and single tokens in one batch
+    ([100], [3000], 15, 5, 64, 128),                                   # few tiles over long keys
+    ([5, 64], [0, 20], 8, 1, 64, 16),                                  # more new tokens than cached: rows that see nothing
+    ([300, 200], [300, 1999], 3, 1, 128, 64),
+    ([513], [640], 16, 8, 128, 128),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,q8", [(BF16, False), (FP16, False), (FP32, False), (BF16, True), (FP16, True), (FP32, True)])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_attention(shape, dt, q8):
+    q_lens, kv_lens, Hq, H, D, page = SHAPES[shape]
+    g = gen(100 + shape)
+    check_attention(g, q_lens, kv_lens, Hq, H, D, page, dt, q8, max_q=max(q_lens), max_kv=max(kv_lens))
+    if shape in (2, 6, 8):
+        # every key seen by every row; a scale of its own; bounds left to their defaults
+        check_attention(g, q_lens, kv_lens, Hq, H, D, page, dt, q8, causal=False, scale=0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,q8", [(BF16, False), (FP16, False), (BF16, True), (FP16, True), (FP32, False)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [900]), ([300], [900])])
+def test_attention_large_and_growing_logits(q_lens, kv_lens, dt, q8):
+    g = gen(7)
+    # logits of up to +-200: the maximum moves by far more than the exponent's range from tile to tile
+    check_attention(g, q_lens, kv_lens, 8, 2, 128, 32, dt, q8, std=4.0, qstd=6.0)
+    # values far from 1
+    check_attention(g, q_lens, kv_lens, 8, 2, 64, 32, dt, q8, std=3e-3)
+    if dt != FP16:
+        check_attention(g, q_lens, kv_lens, 8, 2, 64, 32, dt, q8, std=1e4, qstd=1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 200])
+def test_attention_bad_tables_stay_inside(n):
+    g = gen(11)
+    pool, q, out = check_attention(g, [n, n], [400, 300], 8, 2, 128, 64, BF16, False)
+    c, good = pool.cache, out.clone()
+    bt = pool.bt.clone()
+    for bad in (-1, c.k_pages.shape[0], 2 ** 31 - 1):
+        bt[1, 2] = bad
+        c.k_pages.nan_to_num_(0.0), c.v_pages.nan_to_num_(0.0)
+        got = c.attend(q[: 2 * n], bt, pool.lens, cu([n, n]))
+        assert c.read_error() == N.QV_DERR_TABLE
+        assert torch.equal(got[:n], good[:n])               # the other sequence is right
+        c.err.zero_()
+    # a length above max_kv is cut to it (and what it then reaches of the shorter sequence's table lies outside the
+    # pool); rows past max_q are left as they were
+    out = torch.full((2 * n, 8, 128), 3.0, dtype=BF16, device=DEV)
+    c.attend(q[: 2 * n], pool.bt, pool.lens + 100000, cu([n, n]), out=out)
+    assert c.read_error() == N.QV_DERR_CAPACITY | N.QV_DERR_TABLE
+    c.err.zero_()
+    if n > 1:
+        out.fill_(3.0)
+        c.attend(q[: 2 * n], pool.bt, pool.lens, cu([n, n]), out=out, max_q=n - 1)
+        assert c.read_error() == N.QV_DERR_CAPACITY and bool((out[n - 1] == 3).all()) and bool((out[-1] == 3).all())
+        assert torch.equal(out[: n - 1], good[: n - 1])
+        c.err.zero_()
+    # cumulative lengths outside the rows, negative lengths
+    c.attend(q[: 2 * n], pool.bt, pool.lens, torch.tensor([-5, n, 10 ** 6], dtype=torch.int32, device=DEV))
+    c.attend(q[: 2 * n], pool.bt, -pool.lens, cu([n, n]))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_attention_refusals():
+    g = gen(12)
+    pool = Pool(g, [20], 2, 64, 16, BF16, False)
+    q = rand(g, 3, 4, 64).to(BF16)
+    ok = dict(q=q, block_table=pool.bt, kv_lens=pool.lens, cu_q=cu([3]))
+    pool.cache.attend(**ok)
+    for bad in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q.cpu()), dict(cu_q=cu([3]).long()),
+                dict(cu_q=cu([3])[:1]), dict(kv_lens=pool.lens.repeat(2)), dict(block_table=pool.bt.long()),
+                dict(block_table=pool.bt[0]), dict(max_kv=33), dict(max_kv=-1), dict(max_q=-1),
+                dict(out=torch.empty(3, 4, 32, dtype=BF16, device=DEV)), dict(q=q.transpose(0, 1))):
+        with pytest.raises(N.QevictError):
+            pool.cache.attend(**{**ok, **bad})
+    small = paged.PagedKVCache(2, 2, 96, 16, BF16)
+    with pytest.raises(N.QevictError):
+        small.attend(rand(g, 3, 4, 96).to(BF16), pool.bt, pool.lens, cu([3]))
+    e = torch.empty(0, 4, 64, dtype=BF16, device=DEV)
+    assert pool.cache.attend(e, pool.bt, pool.lens, cu([0])).shape == (0, 4, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,q8", [(BF16, False), (BF16, True), (FP32, False)])
+def test_attention_offsets_past_32_bits(dt, q8):
+    """Pages whose elements lie behind 2^31 elements (and, in 16 bits, 2^32 bytes) of the pool."""
+    H, D, page = 8, 128, 128
+    per = H * page * D
+    P = 2 ** 31 // per + 4
+    c = paged.PagedKVCache(P, H, D, page, dt, bits=8 if q8 else None)
+    g = gen(5)
+    bt = torch.tensor([[P - 1, P - 3], [0, P - 2]], dtype=torch.int32, device=DEV)
+    lens = [200, 256]
+    T = sum(lens)
+    q, k, v = (rand(g, T, n, D).to(dt) for n in (2 * H, H, H))
+    seq = torch.repeat_interleave(torch.arange(2, device=DEV), torch.tensor(lens, device=DEV))
+    pos = torch.arange(T, device=DEV) - cu(lens).long()[seq]
+    c.append(q, k, v, c.slots(bt, seq, pos))
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ko, vo = c.gather(bt, n, cu(lens), T)
+    if not q8:
+        assert torch.equal(ko, k) and torch.equal(vo, v)
+    for ql in ([1, 1], [200, 150]):
+        rows = torch.cat([q[:ql[0]], q[200:200 + ql[1]]])
+        out = c.attend(rows, bt, n, cu(ql))
+        at = 0
+        for b in range(2):
+            lo, hi = (0, 200) if b == 0 else (200, 456)
+            kb, vb = ko[lo:hi].double(), vo[lo:hi].double()
+            o, mag, big = ref_attention(rows[at:at + ql[b]], kb, vb)
+            # INT8: the read-back used here is itself rounded to the type (K: an exponent's error of |q||k| half)
+            more = mag * half(dt) * (1 + 2 * big) if q8 else 0.0
+            bound = attention_bound(o, mag, big, lens[b], D, dt, float(vb.abs().max())) + more
+            assert bool(((out[at:at + ql[b]].double() - o).abs() <= bound).all())
+            at += ql[b]
+    assert c.read_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1], [3000, 10, 700]), ([70, 1, 200], [2500, 900, 200])])
+def test_attention_graph_streams_and_repeats(q_lens, kv_lens, q8):
+    """The same bits eagerly, twice, in two captured graphs replayed at once, and on another stream; a replay with
+    other lengths below the captured bounds."""
+    g = gen(21)
+    pool, q, out = check_attention(g, q_lens, kv_lens, 8, 2, 128, 64, BF16, q8)
+    c, cq, T = pool.cache, cu(q_lens), sum(q_lens)
+    kw = dict(max_q=max(q_lens), max_kv=max(kv_lens))
+    want = c.attend(q[:T], pool.bt, pool.lens, cq, **kw)
+    assert torch.equal(c.attend(q[:T], pool.bt, pool.lens, cq, **kw), want)
+    lens = pool.lens.clone()
+    graphs, outs = [], [torch.zeros_like(want), torch.zeros_like(want)]
+    for o in outs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            c.attend(q[:T], pool.bt, lens, cq, out=o, **kw)
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for gr, st in zip(graphs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                gr.replay()
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+    lens.copy_(torch.clamp(pool.lens // 2, min=max(0, 1)))
+    lens[0] = pool.lens[0] - 1000
+    graphs[0].replay()
+    assert torch.equal(outs[0], c.attend(q[:T], pool.bt, lens, cq, **kw)) and not torch.equal(outs[0], want)
+    with torch.cuda.stream(streams[0]):
+        streams[0].wait_stream(torch.cuda.current_stream())
+        again = c.attend(q[:T], pool.bt, pool.lens, cq, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(again, want) and c.read_error() == 0
+
+
+# ------------------------------------------------------------------ together
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 8])
+def test_chunked_prompt_then_decode(bits):
+    """Two prompts served as a program would: ragged chunks rotated, written and attended together, then single
+    tokens, from packed projections; each step against 64 bits on what the pool holds; at the end the pool is
+    read back and the framework's own prompt attention on it gives the same prompt outputs."""
+    from qevict_b200.model import prefill_attention
+    Hq, H, D, page, dt = 8, 2, 128, 32, BF16
+    g = gen(33)
+    lens, steps = [200, 131], 4
+    qkv = [rand(g, n + steps, Hq + 2 * H, D).to(dt) for n in lens]
+    w = (1 + rand(g, D, std=0.1)).to(dt)
+    table = paged.rope_table(512, D, 500000.0, dict(type="llama3", factor=8.0, low_freq_factor=1.0,
+                                                    high_freq_factor=4.0, original_max_position=128))
+    c = paged.PagedKVCache(16, H, D, page, dt, bits=bits)
+    bt = torch.randperm(16, generator=g, device=DEV).int()[:14].view(2, 7).contiguous()
+    done, outs, rot = [0, 0], [[], []], [[], []]
+    plan = [(64, 50), (100, 1), (36, 80)] + [(1, 1)] * steps
+    for take in plan:
+        rows = torch.cat([qkv[b][done[b]:done[b] + take[b]] for b in range(2)])
+        seq = torch.repeat_interleave(torch.arange(2, device=DEV), torch.tensor(take, device=DEV))
+        pos = torch.cat([torch.arange(done[b], done[b] + take[b], device=DEV) for b in range(2)])
+        q, k, v = rows[:, :Hq], rows[:, Hq:Hq + H], rows[:, Hq + H:]
+        qr = c.append(q, k, v, c.slots(bt, seq, pos), pos.int(), table, q_weight=w, k_weight=w)
+        done = [done[b] + take[b] for b in range(2)]
+        n = torch.tensor(done, dtype=torch.int32, device=DEV)
+        o = c.attend(qr, bt, n, cu(take), max_q=max(take), max_kv=max(done))
+        kk, vv = c.gather(bt, n, cu(done), sum(done))
+        at = 0
+        for b in range(2):
+            lo = 0 if b == 0 else done[0]
+            kb, vb = kk[lo:lo + done[b]].double(), vv[lo:lo + done[b]].double()
+            ref, mag, big = ref_attention(qr[at:at + take[b]], kb, vb)
+            more = mag * half(dt) * (1 + 2 * big) if bits == 8 else 0.0
+            bound = attention_bound(ref, mag, big, done[b], D, dt, float(vb.abs().max())) + more
+            assert bool(((o[at:at + take[b]].double() - ref).abs() <= bound).all())
+            outs[b].append(o[at:at + take[b]])
+            rot[b].append(qr[at:at + take[b]])
+            at += take[b]
+    assert c.read_error() == 0
+    # the rotated keys in the pool are the formula's
+    if bits == 16:
+        for b in range(2):
+            lo = 0 if b == 0 else done[0]
+            close_rows(kk[lo:lo + done[b]], *ref_heads(qkv[b][:, Hq:Hq + H], w, 1e-6, table,
+                                                       torch.arange(done[b], device=DEV), False), dt)
+    n0 = lens[0]
+    po, _ = prefill_attention(torch.cat(rot[0])[None, :n0].contiguous(), kk[None, :n0].contiguous(),
+                              vv[None, :n0].contiguous())
+    mine = torch.cat(outs[0])[:n0].double()
+    # the prompt lane rounds each logit twice to bf16 (the reference's arithmetic): an exponent's error of a logit's
+    # own size, up to |q||k| D^-1/2, and its probabilities once more
+    kb, vb = kk[:n0].double(), vv[:n0].double()
+    ref, mag, big = ref_attention(torch.cat(rot[0])[:n0], kb, vb)
+    bound = attention_bound(ref, mag, big, n0, D, dt, float(vb.abs().max())) * 2 + mag * half(dt) * (2 * 2 * big + 2)
+    assert bool(((po[0].double() - mine).abs() <= bound).all())
