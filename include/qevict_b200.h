@@ -315,7 +315,7 @@ int qv_paged_gather(const qv_paged_cache* c, int32_t batch, const int32_t* block
  * of the chunk and cached lengths (max_kv <= max_pages * page_size): they size
  * the launch, so a captured call serves any lengths below them.  Of a longer
  * chunk the rows past max_q are left as they were, a longer sequence is cut.  out [total_q][q_heads][head_dim].  head_dim 64
- * or 128, q_heads / kv_heads up to 16.  Sums run in a fixed order.  Rows of one
+ * or 128, q_heads / kv_heads up to 16, scale > 0.  Sums run in a fixed order.  Rows of one
  * tile share their P.V products, so a K or V row that is not finite can reach
  * rows of its own sequence that do not see it; what lies behind a sequence's
  * last token, in its pages or others, is never used. */

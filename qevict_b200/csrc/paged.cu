@@ -295,7 +295,7 @@ int paged_cache_check(const qv_paged_cache* c) {
     if (c->pages <= 0 || c->kv_heads <= 0 || c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8) return QV_EINVAL;
     if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return QV_EINVAL;
     if (!dtype_ok(c->dtype) || (c->bits != 0 && c->bits != 8)) return QV_EINVAL;
-    if (c->bits == 8 && (!c->k_scale || !c->v_scale)) return QV_EINVAL;
+    if (c->bits == 8 && (!c->k_scale || !c->v_scale || !al16(c->k_scale) || !al16(c->v_scale))) return QV_EINVAL;
     return QV_OK;
 }
 

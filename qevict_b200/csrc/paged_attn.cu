@@ -18,6 +18,8 @@ namespace qv {
 int paged_cache_check(const qv_paged_cache* c);
 int paged_shift(int page);
 
+int paged_tc_launch(const PagedArgs& a, int dt, int D, bool q8, int64_t tiles, cudaStream_t s);
+
 constexpr int PC_THREADS = 128;
 
 // One block per (token, query head): its four warps take the splits in turn,
@@ -70,25 +72,33 @@ __global__ void __launch_bounds__(PC_THREADS) paged_combine_kernel(const PagedAr
 }
 
 // ---------------------------------------------------------------- plan
+enum PagedKernel { PK_SIMT, PK_TC };
+
 struct PagedPlan {
-    int bm;        // query rows per tile
+    PagedKernel kernel;
+    int rows;      // query rows per tile (PK_SIMT)
     int64_t tiles; // upper bound of the query tiles of a KV head
     int splits, chunk;
 };
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-static PagedPlan paged_plan(int B, int H, int G, int total_q, int max_q, int max_kv) {
+static PagedPlan paged_plan(int dt, int B, int H, int G, int total_q, int max_q, int max_kv) {
     PagedPlan p;
-    p.bm = (int64_t)max_q * G <= 16 ? 16 : 64;
-    // every sequence ends in at most one partial tile, and none is longer than max_q
-    p.tiles = (int64_t)total_q * G / p.bm + (B < total_q ? B : total_q);
-    const int64_t by_len = (int64_t)B * ceil_div((int64_t)max_q * G, p.bm);
+    const bool few = (int64_t)max_q * G <= 16;
+    p.kernel = dt == QV_F32 || few ? PK_SIMT : PK_TC;
+    p.rows = few ? 16 : 64;
+    // tokens (times G: rows) per tile; every sequence ends in at most one partial
+    // tile, and none is longer than max_q
+    const int64_t unit = p.kernel == PK_TC ? 1 : G, per = p.kernel == PK_TC ? 2 * (128 / G) : p.rows;
+    p.tiles = total_q * unit / per + (B < total_q ? B : total_q);
+    const int64_t by_len = (int64_t)B * ceil_div(max_q * unit, per);
     if (p.tiles > by_len) p.tiles = by_len;
-    // splits: enough blocks for two per SM, of at least 256 keys
-    const int64_t blocks = p.tiles * H;
-    int64_t n = blocks > 0 ? ceil_div(2 * 148, blocks) : 1;
-    const int64_t most = ceil_div(max_kv, 256);
+    // splits of the keys: enough blocks for two per SM (one where a block fills
+    // it, in four rounds that even out), each of at least 256 (512) keys
+    const int64_t blocks = p.tiles * H, want = p.kernel == PK_TC ? 4 * 148 : 2 * 148;
+    int64_t n = blocks > 0 ? ceil_div(want, blocks) : 1;
+    const int64_t most = ceil_div(max_kv, p.kernel == PK_TC ? 512 : 256);
     if (n > most) n = most;
     if (n < 1) n = 1;
     p.chunk = (int)(ceil_div(ceil_div(max_kv, n), 128) * 128);
@@ -116,11 +126,13 @@ static int simt_launch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
 }
 
 template <int DT, int D, bool Q8> static int simt_dispatch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
-    return p.bm == 16 ? simt_launch<DT, D, Q8, 16>(a, p, s) : simt_launch<DT, D, Q8, 64>(a, p, s);
+    return p.rows == 16 ? simt_launch<DT, D, Q8, 16>(a, p, s) : simt_launch<DT, D, Q8, 64>(a, p, s);
 }
 
 template <int DT, int D> static int paged_launch(const PagedArgs& a, const PagedPlan& p, bool q8, cudaStream_t s) {
-    const int rc = q8 ? simt_dispatch<DT, D, true>(a, p, s) : simt_dispatch<DT, D, false>(a, p, s);
+    int rc;
+    if (p.kernel == PK_TC) rc = paged_tc_launch(a, DT, D, q8, p.tiles, s);
+    else rc = q8 ? simt_dispatch<DT, D, true>(a, p, s) : simt_dispatch<DT, D, false>(a, p, s);
     if (rc != QV_OK || p.splits == 1) return rc;
     paged_combine_kernel<DT, D><<<(unsigned)((int64_t)a.total_q * a.H * a.G), PC_THREADS, 0, s>>>(a);
     return check_launch();
@@ -142,7 +154,7 @@ extern "C" size_t qv_paged_attention_workspace_bytes(const qv_paged_cache* c, in
                                                      int32_t total_q, int32_t max_q, int32_t max_kv) {
     if (paged_cache_check(c) != QV_OK || !attn_dims_ok(c, batch, q_heads, total_q, max_q, max_kv)) return 0;
     if (batch == 0 || total_q == 0 || max_q == 0) return 0;
-    return paged_ws_bytes(paged_plan(batch, c->kv_heads, q_heads / c->kv_heads, total_q, max_q, max_kv), total_q,
+    return paged_ws_bytes(paged_plan(c->dtype, batch, c->kv_heads, q_heads / c->kv_heads, total_q, max_q, max_kv), total_q,
                           q_heads, c->head_dim);
 }
 
@@ -157,12 +169,14 @@ extern "C" int qv_paged_attention(const qv_paged_cache* c, int32_t batch, int32_
     if (batch == 0 || total_q == 0 || max_q == 0) return QV_OK;
     if (!block_table || max_pages <= 0 || !kv_lens || !cu_q || !q || !out) return QV_EINVAL;
     if ((int64_t)max_kv > (int64_t)max_pages * c->page_size) return QV_EINVAL;
+    if (!(scale > 0.f && scale < INFINITY)) return QV_EINVAL;
     const int64_t per16 = 16 / (int64_t)elt_size(c->dtype);
     if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) || q_stride % per16 ||
         q_stride < (int64_t)q_heads * c->head_dim)
         return QV_EINVAL;
     const int G = q_heads / c->kv_heads;
-    const PagedPlan p = paged_plan(batch, c->kv_heads, G, total_q, max_q, max_kv);
+    const PagedPlan p = paged_plan(c->dtype, batch, c->kv_heads, G, total_q, max_q, max_kv);
+    if (p.tiles * c->kv_heads > 0x7fffffff) return QV_EINVAL;
     const size_t need = paged_ws_bytes(p, total_q, q_heads, c->head_dim);
     if (need > workspace_bytes) return QV_ESPACE;
     if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return QV_EINVAL;

@@ -1,0 +1,613 @@
+// Paged attention of many query rows on the 5th-generation tensor cores
+// (tcgen05 + TMEM), bf16 and fp16, pages in the same type or INT8.
+//
+// A block takes two tiles of up to 128 query rows of one KV head (row r is token
+// r / G of the tile, head r % G of the group) and a range of keys, 128 at a
+// time.  Per key tile j and row tile x:  S_x = Q_x K_j^T (fp32, TMEM);  P_x =
+// exp2(S_x c - m_x) rounded to 16 bits, written over S_x in TMEM;  O_x += P_x V_j
+// with P_x as the TMEM operand.  The two row tiles alternate: while one's 128
+// softmax threads work (one row each), the tensor cores run the other's two
+// products, so a key tile costs the larger of 2 x 2 products and the
+// exponentials (16 per clock and SM) instead of their sum.
+//
+// m_x is a reference, not always the maximum: it moves (and O_x, l_x are
+// rescaled) only when a tile's maximum exceeds it by more than 2^8.  P is then
+// at most 2^8, which neither 16-bit type's relative rounding nor the fp32 sums
+// notice, and O stays in TMEM untouched for almost every tile.
+//
+// INT8 pages: codes become exact 16-bit integers in shared memory (four extra
+// warps); the row scales stay in fp32.  With ks, vs the scales of key j,
+//   u_j = S_j c ks_j + log2(vs_j),  P_j = exp2(u_j - m),  O = sum P_j code_j,
+//   l = sum P_j / vs_j,
+// so the value scale sits inside the exponent that P is rounded from: one
+// rounding, as without INT8, and the row's reference m keeps P in the type's
+// range whatever the scales are.
+//
+// Warps 0-3 and 4-7: the softmax of the two tiles; 8: TMA; 9: MMA (one elected
+// thread each); with INT8 12-15 convert.  Every wait is bounded.
+#include <cudaTypedefs.h>
+#include <math.h>
+
+#include "paged.cuh"
+#include "ptx.cuh"
+#include "tcgen05.cuh"
+
+namespace qv {
+
+constexpr int PT_KEYS = 128;
+constexpr int PT_SLAB = 16384;            // 128 rows x 64 16-bit elements, 128-byte swizzle
+constexpr float PT_LAZY = 8.f;            // the reference moves past 2^8
+constexpr int PT_SC = 4;                  // tiles of row scales held (INT8)
+constexpr float PT_MIN_SCALE = 7.8886090522101181e-31f;   // 2^-100: a smaller value scale counts as this
+
+template <int D, bool Q8> struct PtCfg {
+    static constexpr int NS = D / 64;                       // slabs per operand tile
+    static constexpr int SLOT = NS * PT_SLAB;
+    static constexpr int SLOTS = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8);   // K and V tiles in turn
+    static constexpr int RAW = PT_KEYS * D;                 // one tile of codes
+    static constexpr int RAWS = Q8 ? 2 : 0;
+    static constexpr int THREADS = Q8 ? 512 : 384;
+    // registers per thread after the split (the launch holds 128 x 512 or 168 x 384 of them)
+    static constexpr int REGS_SOFTMAX = Q8 ? 192 : 208, REGS_OTHER = Q8 ? 64 : 88;
+    // Q, slots, codes, and the row scales as loaded (2) and prepared (PT_SC x 3)
+    static_assert(!Q8 || 2 * PT_SC - SLOTS >= 2, "scale ring");
+    static constexpr size_t SMEM = 1024 + 2 * SLOT + SLOTS * SLOT + RAWS * RAW +
+                                   (Q8 ? (2 + PT_SC * 3) * PT_KEYS * 4 : 0);
+    static_assert(SMEM <= 232448 - 512, "shared memory");
+};
+
+__device__ __forceinline__ float pt_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t pt_pack(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void pt_unpack(uint64_t r, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(r));
+}
+__device__ __forceinline__ uint64_t pt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float pt_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+template <int DT> __device__ __forceinline__ uint32_t pt_cvt2(float lo, float hi) {
+    uint32_t p;
+    if (DT == QV_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+    return p;
+}
+
+// Two signed codes (bytes b0, b1 of w, chosen by sel) as exact 16-bit floats.
+// fp16: 0x6400 | u is 1024 + u for a byte u; with u = code + 128, minus 1152.
+// bf16 has 7 fraction bits: 0x4300 | (code & 127) is 128 + the low seven bits,
+// 0x4300 | (code & 128) is 128 or, by the exponent's last bit, 256: their
+// difference is the code.
+template <int DT> __device__ __forceinline__ uint32_t pt_codes2(uint32_t w, uint32_t sel) {
+    uint32_t r;
+    if (DT == QV_F16) {
+        const uint32_t p = __byte_perm(w ^ 0x80808080u, 0x64646464u, sel);
+        asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(0x64806480u));
+    } else {
+        const uint32_t p = __byte_perm(w, 0, sel);
+        const uint32_t lo = (p & 0x007F007Fu) | 0x43004300u, hi = (p & 0x00800080u) | 0x43004300u;
+        asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(lo), "r"(hi));
+    }
+    return r;
+}
+
+// Bounded wait: false after about a second (raising the error word), or at once
+// when another warp of the block has given up.
+__device__ __forceinline__ bool pt_wait_slow(uint64_t* bar, uint32_t parity, volatile int* quit, int32_t* err) {
+    const uint64_t t0 = global_ns();
+    while (true) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*quit) return false;
+        if (global_ns() - t0 > 1000000000ull) {
+            *quit = 1;
+            if (err) set_err(err, QV_DERR_TIMEOUT);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile int* quit, int32_t* err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    return pt_wait_slow(bar, parity, quit, err);
+}
+
+template <int DT, int D, bool Q8>
+__global__ void __launch_bounds__(PtCfg<D, Q8>::THREADS, 1)
+paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
+                const __grid_constant__ CUtensorMap mV, const PagedArgs a) {
+    using C = PtCfg<D, Q8>;
+    constexpr int NS = C::NS, SLOT = C::SLOT, SLOTS = C::SLOTS;
+    extern __shared__ unsigned char pt_raw[];
+    unsigned char* sm = pt_raw + ((1024u - (smem_u32(pt_raw) & 1023u)) & 1023u);
+    unsigned char* sQ = sm;                              // [2][NS] slabs
+    unsigned char* sKV = sQ + 2 * SLOT;                  // [SLOTS]: K0, V0, K1, V1, ...
+    unsigned char* sRaw = sKV + SLOTS * SLOT;            // [RAWS] tiles of codes
+    float* sRawSc = reinterpret_cast<float*>(sRaw + C::RAWS * C::RAW);   // [2][128] as loaded: ks, vs
+    float* sSc = sRawSc + 2 * PT_KEYS;                   // [PT_SC][3][128]: c ks, log2 vs, 1 / vs
+    __shared__ __align__(8) uint64_t q_full, kv_full[SLOTS], kv_empty[SLOTS], raw_full[2], raw_empty[2], sc_full[PT_SC];
+    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], tail, done;
+    __shared__ uint32_t s_taddr;
+    __shared__ int2 s_tile;
+    __shared__ int s_quit;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x % a.H, sp = blockIdx.y;
+    const int QT = PT_KEYS / a.G;                        // tokens per row tile
+
+    if (warp == 0) {
+        // tiles from the end: the longest rows of a causal prompt first
+        const int2 t = paged_find_tile(a, (int)(gridDim.x / a.H) - 1 - (int)(blockIdx.x / a.H), 1, 2 * QT);
+        if (lane == 0) s_tile = t;
+    }
+    __syncthreads();
+    const int b = s_tile.x;
+    if (b < 0) return;
+    const PagedSeq s = paged_seq(a, b);
+    const int Hq = a.H * a.G;
+    const bool split = a.splits > 1 && s.kv > a.chunk;
+    if (!split && sp > 0) return;
+    const int k_begin = split ? sp * a.chunk : 0;
+    // per row tile: first token, tokens, key tiles of this block's range
+    int tok[2], cnt[2], nt[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        tok[x] = (2 * s_tile.y + x) * QT;
+        cnt[x] = min(max(s.live - tok[x], 0), QT);
+        int end = cnt[x] > 0 ? paged_limit(a, s, tok[x] + cnt[x] - 1) : 0;
+        if (split) end = min(end, k_begin + a.chunk);
+        nt[x] = end > k_begin ? (end - k_begin + PT_KEYS - 1) / PT_KEYS : 0;
+    }
+    const int n = max(nt[0], nt[1]);
+    if (split && n == 0) return;
+    // keys of the last tile that exist: what lies behind them is never multiplied
+    const int live_last = n > 0 ? s.kv - k_begin - (n - 1) * PT_KEYS : PT_KEYS;
+    const bool cut = live_last < PT_KEYS;
+
+    if (warp == 9) { tmem_alloc(&s_taddr, 512); tmem_relinquish(); }
+    if (threadIdx.x == 0) {
+        mbar_init(&q_full, 1);
+        for (int i = 0; i < SLOTS; ++i) { mbar_init(&kv_full[i], Q8 ? 4 : 1); mbar_init(&kv_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4);
+            mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
+        }
+        for (int i = 0; i < PT_SC; ++i) mbar_init(&sc_full[i], 4);
+        mbar_init(&tail, 1);
+        mbar_init(&done, 1);
+        s_quit = 0;
+        fence_barrier_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t taddr = s_taddr;      // S (P over it): [0, 128), [128, 256); O: [256, 256 + D), [384, 384 + D)
+    volatile int* quit = &s_quit;
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
+        // ------------------------------------------------------------ softmax of row tile x
+        const int x = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t ts = taddr + lane_off + 128 * x, to = taddr + lane_off + 256 + 128 * x;
+        const int i = r / a.G;
+        const int tok_x = x ? tok[1] : tok[0], tn = x ? nt[1] : nt[0];
+        const bool live = i < (x ? cnt[1] : cnt[0]);
+        int lim = live ? paged_limit(a, s, tok_x + i) - k_begin : 0x7fffffff;   // relative to the block's range
+        int lim_min = lim;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
+        float m = -INFINITY;
+        uint64_t l2 = pt_pack(0.f, 0.f);
+        const float cl = a.scale_log2;
+        const uint64_t c2 = pt_pack(cl, cl);
+        bool ok = true;
+        for (int j = 0; j < tn; ++j) {
+            ok = pt_wait(&s_full[x], j & 1, quit, a.err);
+            // (an entry is refilled once K of tile j + 1 has been released, which follows
+            // this tile's P: 2 PT_SC - SLOTS >= 2 steps of the ring lie between)
+            if (Q8 && ok) ok = pt_wait(&sc_full[j % PT_SC], (j / PT_SC) & 1, quit, a.err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            float v[128];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) tmem_ld32(ts + 32 * w, v + 32 * w);
+            tmem_wait_ld();
+            const float* sc = sSc + (j % PT_SC) * 3 * PT_KEYS;
+            if constexpr (Q8) {
+                // base-2 logits with the value scale in them
+#pragma unroll
+                for (int e = 0; e < 128; e += 4) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(sc + e);
+                    const float4 l4 = *reinterpret_cast<const float4*>(sc + PT_KEYS + e);
+                    pt_unpack(pt_fma2(pt_pack(v[e], v[e + 1]), pt_pack(k4.x, k4.y), pt_pack(l4.x, l4.y)), v[e], v[e + 1]);
+                    pt_unpack(pt_fma2(pt_pack(v[e + 2], v[e + 3]), pt_pack(k4.z, k4.w), pt_pack(l4.z, l4.w)), v[e + 2], v[e + 3]);
+                }
+            }
+            const int seen = lim - j * PT_KEYS;
+            if (lim_min < (j + 1) * PT_KEYS) {
+#pragma unroll
+                for (int e = 0; e < 128; ++e) v[e] = e < seen ? v[e] : -INFINITY;
+            }
+            float mx0 = v[0], mx1 = v[1];
+#pragma unroll
+            for (int e = 2; e < 126; e += 4) {
+                mx0 = pt_max3(mx0, v[e], v[e + 1]);
+                mx1 = pt_max3(mx1, v[e + 2], v[e + 3]);
+            }
+            float mx = fmaxf(pt_max3(mx0, v[126], v[127]), mx1);
+            if (!Q8) mx *= cl;
+            const bool move = mx > m + PT_LAZY;
+            if (__any_sync(0xffffffffu, move)) {
+                const float mn = move ? mx : m;
+                const float f = move && m != -INFINITY ? pt_ex2(m - mn) : 1.f;
+                m = mn;
+                l2 = pt_fma2(l2, pt_pack(f, f), pt_pack(0.f, 0.f));
+                if (j > 0) {
+                    // S(j) is complete, so P.V of every earlier tile is
+#pragma unroll
+                    for (int w = 0; w < D / 16; ++w) {
+                        float o[16];
+                        uint32_t u[16];
+                        tmem_ld16(to + 16 * w, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
+                        tmem_st16(to + 16 * w, u);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.f : m;     // nothing seen yet: every term is 0
+            const uint64_t nm2 = pt_pack(-base, -base);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int k = 32 * w + 2 * e;
+                    float d0, d1;
+                    if (Q8) pt_unpack(pt_add2(pt_pack(v[k], v[k + 1]), nm2), d0, d1);
+                    else pt_unpack(pt_fma2(pt_pack(v[k], v[k + 1]), c2, nm2), d0, d1);
+                    d0 = pt_ex2(d0);
+                    d1 = pt_ex2(d1);
+                    if (Q8) {
+                        const float2 iv = *reinterpret_cast<const float2*>(sc + 2 * PT_KEYS + k);
+                        l2 = pt_fma2(pt_pack(d0, d1), pt_pack(iv.x, iv.y), l2);
+                    } else {
+                        l2 = pt_add2(l2, pt_pack(d0, d1));
+                    }
+                    p[e] = pt_cvt2<DT>(d0, d1);
+                }
+                tmem_st16(ts + 16 * w, p);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[x]);
+        }
+        float l0, l1;
+        pt_unpack(l2, l0, l1);
+        const float l = l0 + l1;
+        if (tn > 0) ok = ok && pt_wait(&o_full[x], 0, quit, a.err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+            tc_fence_after();
+            const size_t orow = (size_t)(s.q0 + tok_x + i) * Hq + h * a.G + (r - i * a.G);
+            const size_t prow = (size_t)sp * a.total_q * Hq + orow;
+            const float inv = split ? 1.f : l > 0.f ? 1.f / l : l;   // no key seen: 0 (a NaN sum stays NaN)
+            if (split && live && tn > 0) {
+                a.part_ml[2 * prow] = m;
+                a.part_ml[2 * prow + 1] = l;
+            }
+#pragma unroll
+            for (int w = 0; w < D / 32; ++w) {
+                float o[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                if (tn > 0) {
+                    tmem_ld32(to + 32 * w, o);
+                    tmem_wait_ld();
+                }
+                if (!live) continue;
+                if (split) {
+                    if (tn > 0)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4*>(a.part_o + prow * D + 32 * w + e) =
+                                make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                } else {
+                    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + orow * D + 32 * w);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        dst[e / 8] = make_uint4(pt_cvt2<DT>(o[e] * inv, o[e + 1] * inv),
+                                                pt_cvt2<DT>(o[e + 2] * inv, o[e + 3] * inv),
+                                                pt_cvt2<DT>(o[e + 4] * inv, o[e + 5] * inv),
+                                                pt_cvt2<DT>(o[e + 6] * inv, o[e + 7] * inv));
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_OTHER));
+        if (warp == 8) {
+            // -------------------------------------------------------- loads
+            if (n > 0 && lane == 0) {
+                prefetch_tensormap(&mQ);
+                prefetch_tensormap(&mK);
+                prefetch_tensormap(&mV);
+                int bytes = 0;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    if (nt[x] > 0) bytes += NS * QT * a.G * 128;
+                mbar_arrive_expect_tx(&q_full, bytes);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    for (int w = 0; nt[x] > 0 && w < NS; ++w)
+                        tma_load_3d(sQ + x * SLOT + w * PT_SLAB, &mQ, 64 * w, h * a.G, s.q0 + tok[x], &q_full);
+            }
+            const int page = 1 << a.page_shift, per_tile = PT_KEYS >> a.page_shift;
+            // lane i keeps the id of the tile's page i
+            int id = 0, next = 0;
+            bool ok = true;
+            if (n > 0 && lane < per_tile && lane * page < s.kv - k_begin) next = paged_page(a, b, k_begin + lane * page);
+            int issued = 0;
+            for (int j = 0; j < n && ok; ++j) {
+                id = next;
+                const int k0 = k_begin + j * PT_KEYS, left = s.kv - k0;
+                const int np = min(per_tile, (left + page - 1) >> a.page_shift);   // pages of the tile that hold keys
+                if (j + 1 < n && lane < per_tile && lane * page < left - PT_KEYS)
+                    next = paged_page(a, b, k0 + PT_KEYS + lane * page);
+                for (int kv = 0; kv < 2 && ok; ++kv) {
+                    const int it = 2 * j + kv;
+                    const CUtensorMap* map = kv ? &mV : &mK;
+                    if constexpr (Q8) {
+                        const int st = it & 1;
+                        if (it >= 2) ok = pt_wait(&raw_empty[st], ((it >> 1) - 1) & 1, quit, a.err);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(&raw_full[st], np * page * (D + (kv ? 0 : 8)));
+                        __syncwarp();
+                        if (lane < np) {
+                            tma_load_4d(sRaw + st * C::RAW + lane * page * D, map, 0, 0, h, id, &raw_full[st]);
+                            if (kv == 0) {
+                                const size_t row = ((size_t)id * a.H + h) << a.page_shift;
+                                float* dst = sRawSc + lane * page;
+                                bulk_load(dst, a.k_scale + row, page * 4, &raw_full[st]);
+                                bulk_load(dst + PT_KEYS, a.v_scale + row, page * 4, &raw_full[st]);
+                            }
+                        }
+                    } else {
+                        const int st = it % SLOTS;
+                        if (it >= SLOTS) ok = pt_wait(&kv_empty[st], (it / SLOTS - 1) & 1, quit, a.err);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], np * page * D * 2);
+                        __syncwarp();
+                        if (lane < np)
+                            for (int w = 0; w < NS; ++w)
+                                tma_load_4d(sKV + st * SLOT + w * PT_SLAB + lane * page * 128, map, 64 * w, 0, h, id,
+                                            &kv_full[st]);
+                    }
+                    issued = it + 1;
+                }
+            }
+            if (!Q8 && cut && ok && n > 0) {
+                // the last V tile's rows behind the sequence: zero, whatever the pages hold there
+                const int it = 2 * n - 1, st = it % SLOTS;
+                ok = pt_wait(&kv_full[st], (it / SLOTS) & 1, quit, a.err);
+                if (__all_sync(0xffffffffu, ok)) {
+                    for (int w = 0; w < NS; ++w)
+                        for (int c = live_last * 8 + lane; c < PT_KEYS * 8; c += 32)
+                            *reinterpret_cast<uint4*>(sKV + st * SLOT + w * PT_SLAB + c * 16) = make_uint4(0, 0, 0, 0);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tail);
+                }
+            }
+            // the copies this warp issued have landed before the block exits
+            if (n > 0) mbar_wait_bounded(&q_full, 0);
+            constexpr int RING = Q8 ? 2 : SLOTS;
+            uint64_t* full = Q8 ? raw_full : kv_full;
+            for (int it = max(issued - RING, 0); it < issued; ++it) mbar_wait_bounded(&full[it % RING], (it / RING) & 1);
+        } else if (warp == 9) {
+            // -------------------------------------------------------- products
+            if (lane == 0 && n > 0) {
+                const uint32_t id_s = umma_idesc_f16(DT == QV_BF16, 128, 128, 0, 0);
+                const uint32_t id_o = umma_idesc_f16(DT == QV_BF16, 128, D, 0, 1);
+                bool ok = pt_wait(&q_full, 0, quit, a.err);
+                tc_fence_after();
+                auto scores = [&](int x, int j) {
+                    const uint32_t qa = smem_u32(sQ + x * SLOT), ka = smem_u32(sKV + ((2 * j) % SLOTS) * SLOT);
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * PT_SLAB + (kk & 3) * 32;
+                        umma_f16(taddr + 128 * x, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024),
+                                 id_s, kk > 0);
+                    }
+                    umma_commit(&s_full[x]);
+                };
+                auto wait_tile = [&](int it) {
+                    bool o = pt_wait(&kv_full[it % SLOTS], (it / SLOTS) & 1, quit, a.err);
+                    if (!Q8 && o && cut && it == 2 * n - 1) o = pt_wait(&tail, 0, quit, a.err);
+                    tc_fence_after();
+                    return o;
+                };
+                if (ok) ok = wait_tile(0);
+                if (ok) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        if (nt[x] > 0) scores(x, 0);
+                    umma_commit(&kv_empty[0]);
+                }
+                for (int j = 0; j < n && ok; ++j) {
+                    bool v_in = false, k_in = false;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (!ok || j >= nt[x]) continue;
+                        const bool last_user = x == 1 || j >= nt[1];
+                        if (!v_in) { ok = wait_tile(2 * j + 1); v_in = true; }
+                        if (ok) ok = pt_wait(&p_full[x], j & 1, quit, a.err);
+                        if (!ok) continue;
+                        tc_fence_after();
+                        const uint32_t va = smem_u32(sKV + ((2 * j + 1) % SLOTS) * SLOT);
+#pragma unroll
+                        for (int kk = 0; kk < PT_KEYS / 16; ++kk)
+                            umma_f16_ta(taddr + 256 + 128 * x, taddr + 128 * x + 8 * kk,
+                                        umma_desc_sw128(va + kk * 2048, PT_SLAB, 1024), id_o, (j > 0 || kk > 0) ? 1 : 0);
+                        if (j + 1 == nt[x]) umma_commit(&o_full[x]);
+                        if (last_user) umma_commit(&kv_empty[(2 * j + 1) % SLOTS]);
+                        if (j + 1 < nt[x]) {
+                            if (!k_in) { ok = wait_tile(2 * j + 2); k_in = true; }
+                            if (!ok) continue;
+                            scores(x, j + 1);
+                            if (x == 1 || j + 1 >= nt[1]) umma_commit(&kv_empty[(2 * j + 2) % SLOTS]);
+                        }
+                    }
+                }
+                // no MMA is in flight when the TMEM is released
+                umma_commit(&done);
+                mbar_wait_bounded(&done, 0);
+            }
+        } else if (Q8 && warp >= 12) {
+            // -------------------------------------------------------- codes -> 16-bit operands
+            const int t = threadIdx.x - 384;
+            constexpr int CPR = D / 16;              // 16-code chunks per row
+            bool ok = true;
+            for (int it = 0; it < 2 * n && ok; ++it) {
+                const int st = it & 1, slot = it % SLOTS, j = it >> 1;
+                ok = pt_wait(&raw_full[st], (it >> 1) & 1, quit, a.err);
+                if (ok && it >= SLOTS) ok = pt_wait(&kv_empty[slot], (it / SLOTS - 1) & 1, quit, a.err);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const int rows = j + 1 == n ? min(live_last, PT_KEYS) : PT_KEYS;
+                if ((it & 1) == 0) {
+                    // scales of this tile's keys; one behind the sequence contributes nothing
+                    float* sc = sSc + (j % PT_SC) * 3 * PT_KEYS;
+                    const float ks = sRawSc[t];
+                    float vs = sRawSc[PT_KEYS + t];
+                    if (vs < PT_MIN_SCALE) vs = PT_MIN_SCALE;    // also a zero row, whose codes are 0
+                    const bool in = t < rows;
+                    sc[t] = in ? ks * a.scale_log2 : 0.f;
+                    sc[PT_KEYS + t] = in ? log2f(vs) : 0.f;
+                    sc[2 * PT_KEYS + t] = in ? 1.f / vs : 0.f;
+                }
+                const unsigned char* raw = sRaw + st * C::RAW;
+                unsigned char* dst = sKV + slot * SLOT;
+#pragma unroll 4
+                for (int c = t; c < PT_KEYS * CPR; c += 128) {
+                    const int r = c / CPR, cc = c % CPR;
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (r < rows) u = *reinterpret_cast<const uint4*>(raw + r * D + cc * 16);
+                    constexpr uint32_t S0 = 0x4140, S1 = 0x4342;
+                    uint4 lo = make_uint4(pt_codes2<DT>(u.x, S0), pt_codes2<DT>(u.x, S1), pt_codes2<DT>(u.y, S0),
+                                          pt_codes2<DT>(u.y, S1));
+                    uint4 hi = make_uint4(pt_codes2<DT>(u.z, S0), pt_codes2<DT>(u.z, S1), pt_codes2<DT>(u.w, S0),
+                                          pt_codes2<DT>(u.w, S1));
+                    unsigned char* row = dst + (cc >> 2) * PT_SLAB + r * 128;
+                    const int ch = (2 * cc) & 7;
+                    *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = lo;
+                    *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = hi;
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&kv_full[slot]);
+                    mbar_arrive(&raw_empty[st]);
+                    if ((it & 1) == 0) mbar_arrive(&sc_full[j % PT_SC]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(taddr, 512);
+    }
+}
+
+// ---------------------------------------------------------------- host
+static PFN_cuTensorMapEncodeTiled_v12000 pt_encode() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }
+    return fn;
+}
+
+static CUtensorMapDataType pt_type(int dt) {
+    return dt == QV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// Pages as (D, page, heads, pages); a box is one page's rows, 64 elements wide
+// with the 128-byte swizzle, or a whole row of codes.
+static bool pt_map_pages(CUtensorMap* m, const void* base, int dt, bool q8, int D, int page, int H, int pages) {
+    auto fn = pt_encode();
+    if (!fn) return false;
+    const cuuint64_t e = q8 ? 1 : 2;
+    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)H, (cuuint64_t)pages};
+    cuuint64_t strides[3] = {D * e, D * e * page, D * e * page * H};
+    cuuint32_t box[4] = {(cuuint32_t)(q8 ? D : 64), (cuuint32_t)page, 1, 1};
+    cuuint32_t es[4] = {1, 1, 1, 1};
+    return fn(m, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : pt_type(dt), 4, const_cast<void*>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, q8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Queries as (D, heads, tokens); a box is one row tile: 64 elements x G heads x 128 / G tokens.
+static bool pt_map_q(CUtensorMap* m, const PagedArgs& a, int dt, int D) {
+    auto fn = pt_encode();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.H * a.G, (cuuint64_t)a.total_q};
+    cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)a.q_stride * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)(PT_KEYS / a.G)};
+    cuuint32_t es[3] = {1, 1, 1};
+    return fn(m, pt_type(dt), 3, const_cast<void*>(a.q), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+           CUDA_SUCCESS;
+}
+
+template <int DT, int D, bool Q8> static int pt_launch(const PagedArgs& a, int64_t tiles, cudaStream_t s) {
+    using C = PtCfg<D, Q8>;
+    CUtensorMap mQ, mK, mV;
+    const int page = 1 << a.page_shift;
+    if (!pt_map_q(&mQ, a, DT, D) || !pt_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages) ||
+        !pt_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages))
+        return QV_EINVAL;
+    const cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<DT, D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)C::SMEM);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    paged_tc_kernel<DT, D, Q8><<<dim3((unsigned)(tiles * a.H), a.splits), C::THREADS, C::SMEM, s>>>(mQ, mK, mV, a);
+    return check_launch();
+}
+
+template <int DT> static int pt_dispatch(const PagedArgs& a, int D, bool q8, int64_t tiles, cudaStream_t s) {
+    if (D == 128) return q8 ? pt_launch<DT, 128, true>(a, tiles, s) : pt_launch<DT, 128, false>(a, tiles, s);
+    return q8 ? pt_launch<DT, 64, true>(a, tiles, s) : pt_launch<DT, 64, false>(a, tiles, s);
+}
+
+int paged_tc_launch(const PagedArgs& a, int dt, int D, bool q8, int64_t tiles, cudaStream_t s) {
+    return dt == QV_BF16 ? pt_dispatch<QV_BF16>(a, D, q8, tiles, s) : pt_dispatch<QV_F16>(a, D, q8, tiles, s);
+}
+
+}  // namespace qv

@@ -246,7 +246,7 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
     keys up to its own.  A row that sees no key gives 0; rows of no chunk are left as they were (out) or
     undefined.  max_q / max_kv: upper bounds of the chunk and cached lengths, which size the launch (default:
     T, and all that the block table can hold); a captured call serves any lengths below them.  scale
-    defaults to D^-1/2.  (qv_paged_attention)"""
+    (positive) defaults to D^-1/2.  (qv_paged_attention)"""
     c = _pool(k_pages, v_pages, k_scale, v_scale, q.dtype, err)
     dev, dt, H, S, D = k_pages.device, q.dtype, k_pages.shape[1], k_pages.shape[2], k_pages.shape[3]
     _need(D in (64, 128), f"head_dim {D} is not 64 or 128")
