@@ -19,6 +19,7 @@ int paged_cache_check(const qv_paged_cache* c);
 int paged_shift(int page);
 
 int paged_tc_launch(const PagedArgs& a, int dt, int D, bool q8, int64_t tiles, cudaStream_t s);
+int paged_few_launch(const PagedArgs& a, int dt, int D, bool q8, cudaStream_t s);
 
 constexpr int PC_THREADS = 128;
 
@@ -28,6 +29,7 @@ template <int DT, int D>
 __global__ void __launch_bounds__(PC_THREADS) paged_combine_kernel(const PagedArgs a) {
     constexpr int E = D / 32;
     __shared__ float s_o[4][D], s_l[4], s_m[4];
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the splits still run
     const int Hq = a.H * a.G;
     const int t = blockIdx.x / Hq, hq = blockIdx.x % Hq;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -72,7 +74,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_combine_kernel(const PagedAr
 }
 
 // ---------------------------------------------------------------- plan
-enum PagedKernel { PK_SIMT, PK_TC };
+enum PagedKernel { PK_SIMT, PK_TC, PK_FEW };
 
 struct PagedPlan {
     PagedKernel kernel;
@@ -86,7 +88,7 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static PagedPlan paged_plan(int dt, int B, int H, int G, int total_q, int max_q, int max_kv) {
     PagedPlan p;
     const bool few = (int64_t)max_q * G <= 16;
-    p.kernel = dt == QV_F32 || few ? PK_SIMT : PK_TC;
+    p.kernel = dt == QV_F32 ? PK_SIMT : few ? PK_FEW : PK_TC;
     p.rows = few ? 16 : 64;
     // tokens (times G: rows) per tile; every sequence ends in at most one partial
     // tile, and none is longer than max_q
@@ -131,11 +133,13 @@ template <int DT, int D, bool Q8> static int simt_dispatch(const PagedArgs& a, c
 
 template <int DT, int D> static int paged_launch(const PagedArgs& a, const PagedPlan& p, bool q8, cudaStream_t s) {
     int rc;
-    if (p.kernel == PK_TC) rc = paged_tc_launch(a, DT, D, q8, p.tiles, s);
-    else rc = q8 ? simt_dispatch<DT, D, true>(a, p, s) : simt_dispatch<DT, D, false>(a, p, s);
+    if constexpr (DT == QV_F32) rc = q8 ? simt_dispatch<DT, D, true>(a, p, s) : simt_dispatch<DT, D, false>(a, p, s);
+    else if (p.kernel == PK_FEW) rc = paged_few_launch(a, DT, D, q8, s);
+    else rc = paged_tc_launch(a, DT, D, q8, p.tiles, s);
     if (rc != QV_OK || p.splits == 1) return rc;
-    paged_combine_kernel<DT, D><<<(unsigned)((int64_t)a.total_q * a.H * a.G), PC_THREADS, 0, s>>>(a);
-    return check_launch();
+    const cudaError_t e = launch_pdl(paged_combine_kernel<DT, D>, dim3((unsigned)((int64_t)a.total_q * a.H * a.G)),
+                                     dim3(PC_THREADS), 0, s, a);
+    return e == cudaSuccess ? check_launch() : set_cuda_error(e);
 }
 
 }  // namespace qv

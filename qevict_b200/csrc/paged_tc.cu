@@ -559,18 +559,19 @@ static CUtensorMapDataType pt_type(int dt) {
     return dt == QV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
 
-// Pages as (D, page, heads, pages); a box is one page's rows, 64 elements wide
-// with the 128-byte swizzle, or a whole row of codes.
-static bool pt_map_pages(CUtensorMap* m, const void* base, int dt, bool q8, int D, int page, int H, int pages) {
+// Pages as (D, page, heads, pages); a box is box_rows rows of one page, 64
+// elements wide with the 128-byte swizzle, or whole rows of codes.
+bool paged_map_pages(CUtensorMap* m, const void* base, int dt, bool q8, int D, int page, int H, int pages, int box_rows,
+                     CUtensorMapSwizzle codes) {
     auto fn = pt_encode();
     if (!fn) return false;
     const cuuint64_t e = q8 ? 1 : 2;
     cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)H, (cuuint64_t)pages};
     cuuint64_t strides[3] = {D * e, D * e * page, D * e * page * H};
-    cuuint32_t box[4] = {(cuuint32_t)(q8 ? D : 64), (cuuint32_t)page, 1, 1};
+    cuuint32_t box[4] = {(cuuint32_t)(q8 ? D : 64), (cuuint32_t)box_rows, 1, 1};
     cuuint32_t es[4] = {1, 1, 1, 1};
     return fn(m, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : pt_type(dt), 4, const_cast<void*>(base), dims, strides, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, q8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, q8 ? codes : CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -591,8 +592,8 @@ template <int DT, int D, bool Q8> static int pt_launch(const PagedArgs& a, int64
     using C = PtCfg<D, Q8>;
     CUtensorMap mQ, mK, mV;
     const int page = 1 << a.page_shift;
-    if (!pt_map_q(&mQ, a, DT, D) || !pt_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages) ||
-        !pt_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages))
+    if (!pt_map_q(&mQ, a, DT, D) || !paged_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages, page, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, page, CU_TENSOR_MAP_SWIZZLE_NONE))
         return QV_EINVAL;
     const cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<DT, D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)C::SMEM);
