@@ -75,26 +75,32 @@ def rope_table(max_pos, rot_dim, theta=10000.0, scaling=None, device="cuda"):
     return (torch.cat([a.cos(), a.sin()], 1) * mult).float()
 
 
-def _need(ok, what):
-    if not ok:
-        raise N.QevictError(what)
+# Checks format their message only when they fail: a decode step's calls are
+# short enough for the host's time per call to count.
+_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(dev).cuda_stream without building the object
+
+
+def _bad(name, expected, x):
+    return N.QevictError(f"{name}: expected {expected}, got {tuple(x.shape)} {x.dtype} on {x.device}")
 
 
 def _heads(name, x, tokens, dim, dtype, dev):
     """A [tokens, heads, head_dim] tensor whose heads are contiguous within a token (a view of a
-    packed projection will do); returns its token stride."""
-    _need(x.dim() == 3 and x.shape[2] == dim and (tokens is None or x.shape[0] == tokens) and x.dtype == dtype
-          and x.device == dev, f"{name}: expected [tokens, heads, {dim}] {dtype} on {dev}, got "
-          f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    packed projection will do); returns (tokens, heads, token stride)."""
+    shape = x.shape
+    if (len(shape) != 3 or shape[2] != dim or (tokens is not None and shape[0] != tokens) or x.dtype is not dtype
+            or x.device != dev):
+        raise _bad(name, f"[{'tokens' if tokens is None else tokens}, heads, {dim}] {dtype} on {dev}", x)
     st = x.stride()
-    h = x.shape[1]
-    _need((st[2] == 1 or dim == 1) and (st[1] == dim or h == 1), f"{name}: a token's heads must be contiguous")
-    return st[0] if x.shape[0] > 1 else h * dim
+    n, h, _ = shape
+    if st[2] != 1 or (st[1] != dim and h != 1):
+        raise N.QevictError(f"{name}: a token's heads must be contiguous, got strides {st}")
+    return n, h, st[0] if n > 1 else h * dim
 
 
 def _vector(name, x, shape, dtype, dev):
-    _need(x.dtype == dtype and tuple(x.shape) == shape and x.is_contiguous() and x.device == dev,
-          f"{name}: expected a contiguous {shape} {dtype} tensor on {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    if x.dtype is not dtype or x.shape != shape or x.device != dev or not x.is_contiguous():
+        raise _bad(name, f"a contiguous {shape} {dtype} tensor on {dev}", x)
 
 
 def _p(t):
@@ -105,50 +111,70 @@ def _launch(dev, name, *args):
     """Call a native entry point on the current stream of `dev`."""
     fn = getattr(N.lib(), name)
     if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = fn(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    N.check(rc, name)
+            rc = fn(*args, _raw_stream(dev.index))
+    if rc:
+        N.check(rc, name)
 
 
 def _pool(k_pages, v_pages, k_scale, v_scale, dtype, err):
-    """The native descriptor of a pool (checked)."""
-    _need(dtype in _DTYPES, f"dtype {dtype} is not one of fp32, bf16, fp16")
-    _need(k_pages.is_cuda, "pages must be on a CUDA device")
-    dev = k_pages.device
-    _need(k_pages.dim() == 4 and v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype
-          and v_pages.device == dev and k_pages.is_contiguous() and v_pages.is_contiguous(),
-          "pages: k and v must be contiguous [pages, kv_heads, page_size, head_dim] tensors of one type and device")
-    P, H, S, D = k_pages.shape
-    _need(S in (16, 32, 64, 128), f"page_size {S} is not 16, 32, 64 or 128")
-    _need(8 <= D <= 256 and D % 8 == 0, f"head_dim {D} is not a multiple of 8 up to 256")
-    q8 = k_pages.dtype == torch.int8
-    _need(q8 or k_pages.dtype == dtype, f"pages of {k_pages.dtype} do not go with {dtype} rows")
+    """The native descriptor of a pool (checked), with its device, heads, page size and head_dim."""
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise N.QevictError(f"dtype {dtype} is not one of fp32, bf16, fp16")
+    if not k_pages.is_cuda:
+        raise N.QevictError("pages must be on a CUDA device")
+    dev, shape, pt = k_pages.device, k_pages.shape, k_pages.dtype
+    if (len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not pt or v_pages.device != dev
+            or not k_pages.is_contiguous() or not v_pages.is_contiguous()):
+        raise _bad("pages", "k and v contiguous [pages, kv_heads, page_size, head_dim] of one type and device; v", v_pages)
+    P, H, S, D = shape
+    _pool_sizes(S, D)
+    q8 = pt is torch.int8
     if q8:
-        _need(k_scale is not None and v_scale is not None, "INT8 pages need k_scale and v_scale")
+        if k_scale is None or v_scale is None:
+            raise N.QevictError("INT8 pages need k_scale and v_scale")
         _vector("k_scale", k_scale, (P, H, S), torch.float32, dev)
         _vector("v_scale", v_scale, (P, H, S), torch.float32, dev)
-    else:
-        _need(k_scale is None and v_scale is None, "k_scale and v_scale go with INT8 pages only")
+    elif pt is not dtype:
+        raise N.QevictError(f"pages of {pt} do not go with {dtype} rows")
+    elif k_scale is not None or v_scale is not None:
+        raise N.QevictError("k_scale and v_scale go with INT8 pages only")
     if err is not None:
         _vector("err", err, (1,), torch.int32, dev)
-    return N.QvPagedCache(k_pages.data_ptr(), v_pages.data_ptr(), _p(k_scale), _p(v_scale), _p(err), P, H, S, D,
-                          _DTYPES[dtype], 8 if q8 else 0)
+    c = N.QvPagedCache(k_pages.data_ptr(), v_pages.data_ptr(), _p(k_scale), _p(v_scale), _p(err), P, H, S, D, code,
+                       8 if q8 else 0)
+    return c, dev, H, S, D
+
+
+def _pool_sizes(page_size, head_dim):
+    if page_size not in (16, 32, 64, 128):
+        raise N.QevictError(f"page_size {page_size} is not 16, 32, 64 or 128")
+    _head_dim(head_dim)
+
+
+def _head_dim(D):
+    if not 8 <= D <= 256 or D % 8:
+        raise N.QevictError(f"head_dim {D} is not a multiple of 8 up to 256")
 
 
 def _turn(tokens, dim, dtype, dev, positions, table, q_weight, k_weight):
     """Checked (max_pos, rot_dim) of the rotation, and the norm weights."""
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            _vector(name, w, (dim,), dtype, dev)
+    if q_weight is not None:
+        _vector("q_weight", q_weight, (dim,), dtype, dev)
+    if k_weight is not None:
+        _vector("k_weight", k_weight, (dim,), dtype, dev)
     if table is None:
         return 0, 0
-    _need(table.dim() == 2 and table.dtype == torch.float32 and table.is_contiguous() and table.device == dev,
-          "table: expected a contiguous [max_pos, rot_dim] fp32 tensor (rope_table)")
+    if table.dim() != 2 or table.dtype is not torch.float32 or not table.is_contiguous() or table.device != dev:
+        raise _bad("table", f"a contiguous [max_pos, rot_dim] fp32 tensor on {dev} (rope_table)", table)
     max_pos, rot = table.shape
-    _need(8 <= rot <= dim and rot % 8 == 0, f"table: rot_dim {rot} is not a multiple of 8 up to head_dim {dim}")
-    _need(positions is not None, "a rotation needs positions")
+    if not 8 <= rot <= dim or rot % 8:
+        raise N.QevictError(f"table: rot_dim {rot} is not a multiple of 8 up to head_dim {dim}")
+    if positions is None:
+        raise N.QevictError("a rotation needs positions")
     _vector("positions", positions, (tokens,), torch.int32, dev)
     return max_pos, rot
 
@@ -161,13 +187,13 @@ def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=No
     rope_table, its rot_dim the part of the head that turns, in pairs (i, i + rot_dim/2), or (2i, 2i+1) with
     interleaved.  Returns contiguous (q, k), or fills out=(q_out, k_out), which may be q and k themselves
     where those are contiguous.  A position outside the table gives NaN.  (qv_qk_norm_rope)"""
-    _need(q.is_cuda and q.dtype in _DTYPES and q.dim() == 3, "q: expected a [tokens, heads, head_dim] fp32, bf16 or "
-          "fp16 CUDA tensor")
-    T, Hq, D = q.shape
-    dev, dt = q.device, q.dtype
-    _need(8 <= D <= 256 and D % 8 == 0, f"head_dim {D} is not a multiple of 8 up to 256")
-    qs, ks = _heads("q", q, T, D, dt, dev), _heads("k", k, T, D, dt, dev)
-    H = k.shape[1]
+    dt, dev = q.dtype, q.device
+    if not q.is_cuda or dt not in _DTYPES or q.dim() != 3:
+        raise _bad("q", "a [tokens, heads, head_dim] fp32, bf16 or fp16 CUDA tensor", q)
+    D = q.shape[2]
+    _head_dim(D)
+    T, Hq, qs = _heads("q", q, None, D, dt, dev)
+    _, H, ks = _heads("k", k, T, D, dt, dev)
     max_pos, rot = _turn(T, D, dt, dev, positions, table, q_weight, k_weight)
     if out is None:
         qo = torch.empty(T, Hq, D, dtype=dt, device=dev)
@@ -187,12 +213,13 @@ def paged_append(q, k, v, slots, positions, table, k_pages, v_pages, *, k_scale=
     (int64, page * page_size + offset; negative: not written).  Returns the queries.  INT8 pages get
     scale = max|row| / 127 and code = rint(row / scale) of the fp32 row.  A slot must appear at most once per
     call; err collects device errors (PagedKVCache.read_error).  (qv_paged_append)"""
-    c = _pool(k_pages, v_pages, k_scale, v_scale, q.dtype, err)
-    dev, dt, H, D = k_pages.device, q.dtype, k_pages.shape[1], k_pages.shape[3]
-    qs = _heads("q", q, None, D, dt, dev)
-    T, Hq = q.shape[0], q.shape[1]
-    ks, vs = _heads("k", k, T, D, dt, dev), _heads("v", v, T, D, dt, dev)
-    _need(k.shape[1] == H and v.shape[1] == H, f"k and v must have the pool's {H} heads")
+    dt = q.dtype
+    c, dev, H, _, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
+    T, Hq, qs = _heads("q", q, None, D, dt, dev)
+    _, kh, ks = _heads("k", k, T, D, dt, dev)
+    _, vh, vs = _heads("v", v, T, D, dt, dev)
+    if kh != H or vh != H:
+        raise N.QevictError(f"k and v must have the pool's {H} heads, got {kh} and {vh}")
     _vector("slots", slots, (T,), torch.int64, dev)
     max_pos, rot = _turn(T, D, dt, dev, positions, table, q_weight, k_weight)
     if q_out is None:
@@ -206,7 +233,8 @@ def paged_append(q, k, v, slots, positions, table, k_pages, v_pages, *, k_scale=
 
 
 def _tables(block_table, kv_lens, cu, dev):
-    _need(block_table.dim() == 2 and block_table.shape[1] > 0, "block_table: expected [batch, max_pages]")
+    if block_table.dim() != 2 or not block_table.shape[1]:
+        raise _bad("block_table", "[batch, max_pages]", block_table)
     B, width = block_table.shape
     _vector("block_table", block_table, (B, width), torch.int32, dev)
     _vector("kv_lens", kv_lens, (B,), torch.int32, dev)
@@ -220,10 +248,10 @@ def paged_gather(k_pages, v_pages, block_table, kv_lens, cu_kv, total, *, k_scal
     need it): the first kv_lens[b] tokens of sequence b from row cu_kv[b] on, cu_kv [batch + 1] ascending int32;
     rows of no sequence are left as they were (out) or undefined.  (qv_paged_gather)"""
     dt = k_pages.dtype if dtype is None else dtype
-    c = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
-    dev, H, D = k_pages.device, k_pages.shape[1], k_pages.shape[3]
+    c, dev, H, _, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
     B, width = _tables(block_table, kv_lens, cu_kv, dev)
-    _need(total >= 0, "total must not be negative")
+    if total < 0:
+        raise N.QevictError("total must not be negative")
     if out is None:
         ko = torch.empty(total, H, D, dtype=dt, device=dev)
         vo = torch.empty(total, H, D, dtype=dt, device=dev)
@@ -247,17 +275,18 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
     undefined.  max_q / max_kv: upper bounds of the chunk and cached lengths, which size the launch (default:
     T, and all that the block table can hold); a captured call serves any lengths below them.  scale
     (positive) defaults to D^-1/2.  (qv_paged_attention)"""
-    c = _pool(k_pages, v_pages, k_scale, v_scale, q.dtype, err)
-    dev, dt, H, S, D = k_pages.device, q.dtype, k_pages.shape[1], k_pages.shape[2], k_pages.shape[3]
-    _need(D in (64, 128), f"head_dim {D} is not 64 or 128")
-    qs = _heads("q", q, None, D, dt, dev)
-    T, Hq = q.shape[0], q.shape[1]
-    _need(Hq % H == 0 and Hq // H <= 16, f"{Hq} query heads are not 1 to 16 times the pool's {H}")
+    dt = q.dtype
+    c, dev, H, S, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
+    if D != 64 and D != 128:
+        raise N.QevictError(f"head_dim {D} is not 64 or 128")
+    T, Hq, qs = _heads("q", q, None, D, dt, dev)
+    if Hq % H or Hq // H > 16:
+        raise N.QevictError(f"{Hq} query heads are not 1 to 16 times the pool's {H}")
     B, width = _tables(block_table, kv_lens, cu_q, dev)
     max_q = T if max_q is None else max_q
     max_kv = width * S if max_kv is None else max_kv
-    _need(0 <= max_q and 0 <= max_kv <= width * S, f"max_q {max_q} and max_kv {max_kv} must be lengths, max_kv at most "
-          f"the block table's {width * S}")
+    if max_q < 0 or not 0 <= max_kv <= width * S:
+        raise N.QevictError(f"max_q {max_q} and max_kv {max_kv} must be lengths, max_kv at most the block table's {width * S}")
     if out is None:
         out = torch.empty(T, Hq, D, dtype=dt, device=dev)
     else:
@@ -279,11 +308,15 @@ class PagedKVCache:
     sequence owns is the caller's: block_table [batch, max_pages] int32 on the pool's device."""
 
     def __init__(self, pages, kv_heads, head_dim, page_size=64, dtype=torch.bfloat16, bits=None, device="cuda"):
-        _need(dtype in _DTYPES, f"dtype {dtype} is not one of fp32, bf16, fp16")
+        if dtype not in _DTYPES:
+            raise N.QevictError(f"dtype {dtype} is not one of fp32, bf16, fp16")
         full = torch.finfo(dtype).bits
         bits = full if bits is None else bits
-        _need(bits in (8, full), f"bits {bits} is not 8 or the dtype's own {full}")
-        _need(pages > 0 and kv_heads > 0, "a pool needs pages and heads")
+        if bits not in (8, full):
+            raise N.QevictError(f"bits {bits} is not 8 or the dtype's own {full}")
+        if pages <= 0 or kv_heads <= 0:
+            raise N.QevictError("a pool needs pages and heads")
+        _pool_sizes(page_size, head_dim)
         self.dtype, self.page_size = dtype, page_size
         shape = (pages, kv_heads, page_size, head_dim)
         self.k_pages = torch.zeros(shape, dtype=torch.int8 if bits == 8 else dtype, device=device)
@@ -291,7 +324,6 @@ class PagedKVCache:
         self.k_scale = torch.zeros(shape[:3], dtype=torch.float32, device=device) if bits == 8 else None
         self.v_scale = torch.zeros_like(self.k_scale) if bits == 8 else None
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
-        _pool(self.k_pages, self.v_pages, self.k_scale, self.v_scale, dtype, self.err)
 
     def slots(self, block_table, seq, pos):
         """Slots of tokens at index pos [T] of sequences seq [T] (int64 [T])."""
