@@ -96,11 +96,14 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int total_q, int max_q,
     p.tiles = total_q * unit / per + (B < total_q ? B : total_q);
     const int64_t by_len = (int64_t)B * ceil_div(max_q * unit, per);
     if (p.tiles > by_len) p.tiles = by_len;
-    // splits of the keys: enough blocks for two per SM (one where a block fills
-    // it, in four rounds that even out), each of at least 256 (512) keys
-    const int64_t blocks = p.tiles * H, want = p.kernel == PK_TC ? 4 * 148 : 2 * 148;
+    // splits of the keys: enough blocks for the SMs.  One sequence: one round of
+    // equal blocks; several, whose lengths differ: rounds enough to even out
+    int64_t blocks = p.tiles * H, want, least;
+    if (p.kernel == PK_FEW) { blocks = (int64_t)B * H; want = (B > 1 ? 8 : 1) * 2 * 148; least = B > 1 ? 1024 : 512; }
+    else if (p.kernel == PK_TC) { want = 4 * 148; least = 512; }
+    else { want = 2 * 148; least = 256; }
     int64_t n = blocks > 0 ? ceil_div(want, blocks) : 1;
-    const int64_t most = ceil_div(max_kv, p.kernel == PK_TC ? 512 : 256);
+    const int64_t most = ceil_div(max_kv, least);
     if (n > most) n = most;
     if (n < 1) n = 1;
     p.chunk = (int)(ceil_div(ceil_div(max_kv, n), 128) * 128);

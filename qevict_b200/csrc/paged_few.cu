@@ -11,16 +11,23 @@
 // end.  Two blocks share an SM: one's start and end hide behind the other's
 // loads.
 //
-// Per tile: S = Q K^T and O += P V with warp-level MMA (m16n8k16, rows = query
-// rows; P goes from accumulator to operand registers as it is), and in base 2
-//   P = exp2(S c - m),  l += P,
-// where the reference m moves only when a logit exceeds it by 2^8, so that a
-// tile needs no row maximum across lanes.  INT8 rows: the codes become exact
-// 16-bit integers in registers and the scales stay in fp32,
-//   u = S c ks + log2(vs),  P = exp2(u - m),  O += P code,  l += P / vs.
+// Per tile, with warp-level MMA (m16n8k16) and the cached rows as the M side, so
+// that up to 8 query rows cost one n-tile and no padding of the conversions:
+//   S^T = K Q^T,  P = exp2(S c - m),  l += P,  O^T += V^T P^T
+// P^T's operand registers are the accumulators' 8x8 blocks transposed
+// (movmatrix).  The reference m is set 2^7 below a maximum and moves only when a
+// logit exceeds it by 2^15, so that a tile needs no row maximum across lanes and
+// P spans fp16 down to 2^-31 of the largest.  With bf16 pages P is split into two
+// bf16 parts (P V is then exact to 2^-17; the tensor pipe is idle anyway).
+//
+// INT8 rows: the codes become exact fp16 integers in registers and the scales
+// stay in fp32,
+//   u = S c ks + log2(vs),  P = exp2(u - m),  O += P code,  l += P / vs,
+// with P in fp16 whatever the type; bf16 queries become fp16 scaled by a power
+// of two of their row's own (off by at most 2^-25 of the row's largest element).
 // The contraction over the head's elements may run in any order, and so may the
-// columns of O: with INT8 each lane takes 16-byte chunks of a row as the
-// elements of its own fragments.
+// rows of O^T: each lane takes 16-byte chunks of codes as the elements of its
+// own fragments.
 #include <cudaTypedefs.h>
 #include <math.h>
 
@@ -32,7 +39,7 @@ namespace qv {
 constexpr int PF_WARPS = 4;
 constexpr int PF_THREADS = 32 * PF_WARPS;
 constexpr int PF_PIECE = 16;              // keys per TMA box: never across a page
-constexpr float PF_LAZY = 8.f;
+constexpr float PF_BELOW = 7.f, PF_LAZY = 15.f;
 constexpr float PF_MIN_SCALE = 7.8886090522101181e-31f;   // 2^-100: a smaller value scale counts as this
 
 template <int D, bool Q8> struct PfCfg {
@@ -60,27 +67,24 @@ template <int DT> __device__ __forceinline__ void pf_mma(float* c, const uint32_
     const uint32_t b[2] = {b0, b1};
     if (DT == QV_BF16) mma_bf16(c, a, b); else mma_f16(c, a, b);
 }
-// Codes in bytes 0 and 2 of w as exact 16-bit floats.  fp16: 0x6400 | u is
-// 1024 + u, u = code + 128.  bf16: 0x4300 | (code & 127) is 128 + the low seven
-// bits and 0x4300 | (code & 128) is 128, or 256 by the exponent's last bit.
-template <int DT> __device__ __forceinline__ uint32_t pf_codes(uint32_t w) {
+// Two biased codes (bytes of u and v chosen by sel; the other bytes become 0x64)
+// as exact fp16 integers: 0x6400 | b is 1024 + b, b = code + 128.
+__device__ __forceinline__ uint32_t pf_codes(uint32_t u, uint32_t v, uint32_t sel) {
+    const uint32_t p = __byte_perm(u, v, sel);
     uint32_t r;
-    if (DT == QV_F16) {
-        const uint32_t p = ((w ^ 0x00800080u) & 0x00FF00FFu) | 0x64006400u;
-        asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(0x64806480u));
-    } else {
-        const uint32_t lo = (w & 0x007F007Fu) | 0x43004300u, hi = (w & 0x00800080u) | 0x43004300u;
-        asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(lo), "r"(hi));
-    }
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(0x64806480u));
     return r;
 }
 
-template <int DT, int D, bool Q8>
+// NQ: n-tiles of 8 query rows.
+template <int DT, int D, bool Q8, int NQ>
 __global__ void __launch_bounds__(PF_THREADS, 2)
 paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const PagedArgs a) {
     using C = PfCfg<D, Q8>;
     using T = typename Elt<DT>::T;
-    constexpr int KT = C::KT, NT = KT / 8, KS = D / 16, ND = D / 8;
+    constexpr int MT = Q8 ? QV_F16 : DT;                 // type of the products
+    constexpr bool HILO = MT == QV_BF16;
+    constexpr int KT = C::KT, NM = KT / 16, KS = D / 16, ND = D / 16;
     extern __shared__ unsigned char pf_raw[];
     unsigned char* sm = pf_raw + ((1024u - (smem_u32(pf_raw) & 1023u)) & 1023u);
     __shared__ __align__(8) uint64_t full[PF_WARPS][C::STAGES];
@@ -112,12 +116,11 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
 
     // lane 0 loads: tile i of this warp holds the keys from k_begin + (warp + 4 i) KT on
     const int mine = tiles > warp ? (tiles - warp + PF_WARPS - 1) / PF_WARPS : 0;
-    constexpr int PP = KT / PF_PIECE;
-    int ids[PP];
+    int ids[NM];
     auto find_pages = [&](int i) {
         const int k0 = k_begin + (warp + PF_WARPS * i) * KT;
 #pragma unroll
-        for (int p = 0; p < PP; ++p) ids[p] = i < mine && k0 + p * PF_PIECE < s.kv ? paged_page(a, b, k0 + p * PF_PIECE) : -1;
+        for (int p = 0; p < NM; ++p) ids[p] = i < mine && k0 + p * PF_PIECE < s.kv ? paged_page(a, b, k0 + p * PF_PIECE) : -1;
     };
     auto issue = [&](int i) {
         const int st = i % C::STAGES, k0 = k_begin + (warp + PF_WARPS * i) * KT;
@@ -125,10 +128,10 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
         unsigned char* dst = ring + st * C::STAGE;
         int n = 0;
 #pragma unroll
-        for (int p = 0; p < PP; ++p) n += ids[p] >= 0;
+        for (int p = 0; p < NM; ++p) n += ids[p] >= 0;
         mbar_arrive_expect_tx(bar, n * PF_PIECE * (2 * C::ROWB + (Q8 ? 8 : 0)));
 #pragma unroll
-        for (int p = 0; p < PP; ++p) {
+        for (int p = 0; p < NM; ++p) {
             if (ids[p] < 0) continue;
             const int off = (k0 + p * PF_PIECE) & ((1 << a.page_shift) - 1);
             if (Q8) {
@@ -152,33 +155,60 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
         find_pages(C::STAGES);
     }
 
-    // query fragments: row g (and g + 8) of the group's rows
-    uint32_t qa[KS][4];
-    {
-        const T* q0 = nullptr;
-        const T* q1 = nullptr;
-        if (g < rows) q0 = reinterpret_cast<const T*>(a.q) + (size_t)(s.q0 + g / a.G) * a.q_stride + (size_t)(h * a.G + g % a.G) * D;
-        if (g + 8 < rows)
-            q1 = reinterpret_cast<const T*>(a.q) + (size_t)(s.q0 + (g + 8) / a.G) * a.q_stride + (size_t)(h * a.G + (g + 8) % a.G) * D;
+    // query fragments: lane (g, t) holds row 8 q + g; its four slots of a k-step are elements 2t, 2t + 1,
+    // 2t + 8, 2t + 9, or with INT8 the four consecutive codes of the chunk it reads
+    uint32_t qb[NQ][KS][2];
+    float cq[NQ][2];                     // c of the rows 8 q + 2t, 8 q + 2t + 1
+    int lim[NQ][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const int r = 8 * q + g;
+        const T* src = r < rows ? reinterpret_cast<const T*>(a.q) + (size_t)(s.q0 + r / a.G) * a.q_stride + (size_t)(h * a.G + r % a.G) * D : nullptr;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            // elements of the lane's four slots of a k-step: 2t, 2t + 1, 2t + 8, 2t + 9, or with
-            // INT8 four consecutive codes of the chunks the lane reads
             const int d0 = Q8 ? 64 * (k >> 2) + 16 * t + 4 * (k & 3) : 16 * k + 2 * t;
-            const int d1 = Q8 ? d0 + 2 : d0 + 8;
-            qa[k][0] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d0) : 0u;
-            qa[k][1] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d0) : 0u;
-            qa[k][2] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d1) : 0u;
-            qa[k][3] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d1) : 0u;
+            qb[q][k][0] = src ? *reinterpret_cast<const uint32_t*>(src + d0) : 0u;
+            qb[q][k][1] = src ? *reinterpret_cast<const uint32_t*>(src + d0 + (Q8 ? 2 : 8)) : 0u;
+        }
+        float back = 1.f;
+        if constexpr (Q8 && DT == QV_BF16) {
+            float mx = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    mx = fmaxf(mx, fabsf(__uint_as_float(qb[q][k][e] << 16)));
+                    mx = fmaxf(mx, fabsf(__uint_as_float(qb[q][k][e] & 0xFFFF0000u)));
+                }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // 2^-e with 2^e <= mx < 2^(e+1), from the exponent's bits (kept where both powers are normal)
+            const int e = min(max((int)(__float_as_uint(mx) >> 23), 2), 252);
+            const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+            back = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+                    qb[q][k][w] = pf_cvt2<QV_F16>(__uint_as_float(qb[q][k][w] << 16) * down,
+                                                  __uint_as_float(qb[q][k][w] & 0xFFFF0000u) * down);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int rr = 8 * q + 2 * t + e;
+            cq[q][e] = a.scale_log2 * __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
+            lim[q][e] = min(rr < rows ? paged_limit(a, s, rr / a.G) : s.kv, k_end);
         }
     }
-    const int lim0 = g < rows ? paged_limit(a, s, g / a.G) : s.kv;
-    const int lim1 = g + 8 < rows ? paged_limit(a, s, (g + 8) / a.G) : s.kv;
-    const int lim_min = paged_limit(a, s, 0);
-    float o[ND][4];
+    const int lim_min = min(paged_limit(a, s, 0), k_end);
+    float o[NQ][ND][4], m[NQ][2], l[NQ][2];
 #pragma unroll
-    for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    for (int q = 0; q < NQ; ++q) {
+        m[q][0] = m[q][1] = -INFINITY;
+        l[q][0] = l[q][1] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[q][d][0] = o[q][d][1] = o[q][d][2] = o[q][d][3] = 0.f;
+    }
 
     for (int i = 0; i < mine; ++i) {
         const int st = i % C::STAGES, k0 = k_begin + (warp + PF_WARPS * i) * KT;
@@ -191,109 +221,112 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
         unsigned char* kt = ring + st * C::STAGE;
         unsigned char* vt = kt + C::HALF;
         const uint32_t ka = smem_u32(kt), va = smem_u32(vt);
-        float x[NT][4];
+        float x[NM][NQ][4];              // keys 16 i + g (, + 8) x rows 2t, 2t + 1
 #pragma unroll
-        for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
+        for (int i2 = 0; i2 < NM; ++i2)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) x[i2][q][0] = x[i2][q][1] = x[i2][q][2] = x[i2][q][3] = 0.f;
         if constexpr (!Q8) {
-            const int r = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
+            const int r = lane & 15, hi = lane >> 4;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 const uint32_t ch = (((2 * k) & 7) + hi) ^ (r & 7);
 #pragma unroll
-                for (int n = 0; n < NT; n += 2) {
-                    uint32_t b0, b1, b2, b3;
-                    ldsm_x4(ka + (k >> 2) * KT * 128 + (8 * n + r) * 128 + (ch << 4), b0, b1, b2, b3);
-                    pf_mma<DT>(x[n], qa[k], b0, b1);
-                    pf_mma<DT>(x[n + 1], qa[k], b2, b3);
+                for (int i2 = 0; i2 < NM; ++i2) {
+                    uint32_t w[4];
+                    ldsm_x4(ka + (k >> 2) * KT * 128 + (16 * i2 + r) * 128 + (ch << 4), w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) pf_mma<MT>(x[i2][q], w, qb[q][k][0], qb[q][k][1]);
                 }
             }
         } else {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int key = 8 * n + g;
+            for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
+                for (int i2 = 0; i2 < NM; ++i2) {
+                    const int key = 16 * i2 + g;                 // and key + 8: the same place in the swizzle
                     const int ch = (t + 4 * c) ^ (D == 128 ? key & 7 : (key >> 1) & 3);
-                    const uint4 u = *reinterpret_cast<const uint4*>(kt + key * D + (ch << 4));
-                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+                    uint4 u = *reinterpret_cast<const uint4*>(kt + key * D + (ch << 4));
+                    uint4 v = *reinterpret_cast<const uint4*>(kt + (key + 8) * D + (ch << 4));
+                    const uint32_t* wu = reinterpret_cast<const uint32_t*>(&u);
+                    const uint32_t* wv = reinterpret_cast<const uint32_t*>(&v);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        pf_mma<DT>(x[n], qa[4 * c + k], pf_codes<DT>(__byte_perm(w[k], 0, 0x4140)),
-                                   pf_codes<DT>(__byte_perm(w[k], 0, 0x4342)));
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t cu = wu[k] ^ 0x80808080u, cv = wv[k] ^ 0x80808080u;
+                        const uint32_t w[4] = {pf_codes(cu, 0x64646464u, 0x4140), pf_codes(cv, 0x64646464u, 0x4140),
+                                               pf_codes(cu, 0x64646464u, 0x4342), pf_codes(cv, 0x64646464u, 0x4342)};
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) pf_mma<MT>(x[i2][q], w, qb[q][4 * c + k][0], qb[q][4 * c + k][1]);
+                    }
                 }
-            }
         }
         // base-2 logits; keys behind a row's limit leave
-        const bool edge = k0 + KT > min(lim_min, k_end);
-        float iv[Q8 ? NT : 1][2];
+        const bool edge = k0 + KT > lim_min;
+        float iv[NM][2];
+        float top[NQ][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int key = k0 + 8 * n + 2 * t;
-            if constexpr (Q8) {
-                const float* sc = ring_sc + st * 2 * KT + 8 * n + 2 * t;
-                float2 ks = *reinterpret_cast<const float2*>(sc);
-                float2 vs = *reinterpret_cast<const float2*>(sc + KT);
-                vs.x = vs.x < PF_MIN_SCALE ? PF_MIN_SCALE : vs.x;      // also a zero row, whose codes are 0
-                vs.y = vs.y < PF_MIN_SCALE ? PF_MIN_SCALE : vs.y;
-                if (edge) {
-                    if (key >= s.kv) { ks.x = 0.f; vs.x = 1.f; }       // what lies there is not a row
-                    if (key + 1 >= s.kv) { ks.y = 0.f; vs.y = 1.f; }
+        for (int q = 0; q < NQ; ++q) top[q][0] = top[q][1] = -INFINITY;
+#pragma unroll
+        for (int i2 = 0; i2 < NM; ++i2)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int key = k0 + 16 * i2 + g + 8 * e;
+                float ks = 1.f, lv = 0.f;
+                if constexpr (Q8) {
+                    const float* sc = ring_sc + st * 2 * KT + 16 * i2 + g + 8 * e;
+                    ks = sc[0];
+                    float vs = sc[KT];
+                    vs = vs < PF_MIN_SCALE ? PF_MIN_SCALE : vs;          // also a zero row, whose codes are 0
+                    if (edge && key >= s.kv) { ks = 0.f; vs = 1.f; }     // what lies there is not a row
+                    lv = __log2f(vs);
+                    iv[i2][e] = pf_ex2(-lv);
                 }
-                const float lx = __log2f(vs.x), ly = __log2f(vs.y);
-                iv[n][0] = pf_ex2(-lx);
-                iv[n][1] = pf_ex2(-ly);
-                ks.x *= a.scale_log2;
-                ks.y *= a.scale_log2;
-                x[n][0] = fmaf(x[n][0], ks.x, lx);
-                x[n][1] = fmaf(x[n][1], ks.y, ly);
-                x[n][2] = fmaf(x[n][2], ks.x, lx);
-                x[n][3] = fmaf(x[n][3], ks.y, ly);
-            } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[n][j] *= a.scale_log2;
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float& y = x[i2][q][2 * e + j];
+                        y = Q8 ? fmaf(y * cq[q][j], ks, lv) : y * cq[q][j];
+                        if (edge && key >= lim[q][j]) y = -INFINITY;
+                        top[q][j] = fmaxf(top[q][j], y);
+                    }
             }
-            if (edge) {
-                if (key >= min(lim0, k_end)) x[n][0] = -INFINITY;
-                if (key + 1 >= min(lim0, k_end)) x[n][1] = -INFINITY;
-                if (key >= min(lim1, k_end)) x[n][2] = -INFINITY;
-                if (key + 1 >= min(lim1, k_end)) x[n][3] = -INFINITY;
-            }
-        }
-        float a0 = x[0][0], a1 = x[0][2];
+        bool move = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            a0 = fmaxf(a0, fmaxf(x[n][0], x[n][1]));
-            a1 = fmaxf(a1, fmaxf(x[n][2], x[n][3]));
-        }
-        if (__any_sync(0xffffffffu, a0 > m0 + PF_LAZY || a1 > m1 + PF_LAZY)) {
-            a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, 1));
-            a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, 1));
-            a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, 2));
-            a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, 2));
-            const float n0 = a0 > m0 + PF_LAZY ? a0 : m0, n1 = a1 > m1 + PF_LAZY ? a1 : m1;
-            const float f0 = m0 == -INFINITY ? 1.f : pf_ex2(m0 - n0), f1 = m1 == -INFINITY ? 1.f : pf_ex2(m1 - n1);
-            m0 = n0;
-            m1 = n1;
-            l0 *= f0;
-            l1 *= f1;
+        for (int q = 0; q < NQ; ++q) move = move || top[q][0] > m[q][0] + PF_LAZY || top[q][1] > m[q][1] + PF_LAZY;
+        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-            for (int d = 0; d < ND; ++d) { o[d][0] *= f0; o[d][1] *= f0; o[d][2] *= f1; o[d][3] *= f1; }
-        }
-        const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
-        uint32_t p[NT][2];
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float p0 = pf_ex2(x[n][0] - b0), p1 = pf_ex2(x[n][1] - b0);
-            const float p2 = pf_ex2(x[n][2] - b1), p3 = pf_ex2(x[n][3] - b1);
-            if constexpr (Q8) {
-                l0 = fmaf(p0, iv[n][0], fmaf(p1, iv[n][1], l0));
-                l1 = fmaf(p2, iv[n][0], fmaf(p3, iv[n][1], l1));
-            } else {
-                l0 += p0 + p1;
-                l1 += p2 + p3;
-            }
-            p[n][0] = pf_cvt2<DT>(p0, p1);
-            p[n][1] = pf_cvt2<DT>(p2, p3);
+                for (int j = 0; j < 2; ++j) {
+                    float mx = top[q][j];
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+                    const bool mv = mx > m[q][j] + PF_LAZY;
+                    const float mn = mv ? mx - PF_BELOW : m[q][j];
+                    const float f = mv && m[q][j] != -INFINITY ? pf_ex2(m[q][j] - mn) : 1.f;
+                    m[q][j] = mn;
+                    l[q][j] *= f;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) { o[q][d][j] *= f; o[q][d][2 + j] *= f; }
+                }
+        }
+        uint32_t p[NM][NQ][2], plo[NM][NQ][2];       // P^T as operand; the low parts
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const float b0 = m[q][0] == -INFINITY ? 0.f : m[q][0], b1 = m[q][1] == -INFINITY ? 0.f : m[q][1];
+#pragma unroll
+            for (int i2 = 0; i2 < NM; ++i2)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float p0 = pf_ex2(x[i2][q][2 * e] - b0), p1 = pf_ex2(x[i2][q][2 * e + 1] - b1);
+                    l[q][0] = Q8 ? fmaf(p0, iv[i2][e], l[q][0]) : l[q][0] + p0;
+                    l[q][1] = Q8 ? fmaf(p1, iv[i2][e], l[q][1]) : l[q][1] + p1;
+                    const uint32_t w = pf_cvt2<MT>(p0, p1);
+                    p[i2][q][e] = movm_t(w);
+                    if constexpr (HILO)
+                        plo[i2][q][e] = movm_t(pf_cvt2<MT>(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xFFFF0000u)));
+                }
         }
         if (!Q8 && k0 + KT > s.kv) {
             // rows behind the sequence may hold anything: 0 times that must be 0
@@ -302,23 +335,26 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
             __syncwarp();
         }
 #pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk) {
-            const uint32_t pa[4] = {p[2 * kk][0], p[2 * kk][1], p[2 * kk + 1][0], p[2 * kk + 1][1]};
+        for (int i2 = 0; i2 < NM; ++i2) {
             if constexpr (!Q8) {
-                const int r = 16 * kk + (lane & 7) + (((lane >> 3) & 1) << 3), hi = lane >> 4;
+                const int r = 16 * i2 + (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
 #pragma unroll
-                for (int d = 0; d < ND; d += 2) {
-                    uint32_t v0, v1, v2, v3;
-                    ldsm_x4_t(va + (d >> 3) * KT * 128 + r * 128 + ((((d & 7) + hi) ^ (r & 7)) << 4), v0, v1, v2, v3);
-                    pf_mma<DT>(o[d], pa, v0, v1);
-                    pf_mma<DT>(o[d + 1], pa, v2, v3);
+                for (int d = 0; d < ND; ++d) {
+                    uint32_t w[4];
+                    ldsm_x4_t(va + (d >> 2) * KT * 128 + r * 128 + (((((2 * d) & 7) + hi) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+                        pf_mma<MT>(o[q][d], w, p[i2][q][0], p[i2][q][1]);
+                        if constexpr (HILO) pf_mma<MT>(o[q][d], w, plo[i2][q][0], plo[i2][q][1]);
+                    }
                 }
             } else {
-                // lane (g, t): bytes ND g .. of key rows 2t, 2t + 1, 2t + 8, 2t + 9; column n of tile d is element n ND + d
-                uint32_t w[4][ND / 4];
+                // lane (g, t): chunk g (D / 8 codes) of key rows 2t, 2t + 1, 2t + 8, 2t + 9; rows g and g + 8 of tile d
+                // are its elements 2d and 2d + 1
+                uint32_t w[4][D / 32];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int key = 16 * kk + 2 * t + (e & 1) + 8 * (e >> 1);
+                    const int key = 16 * i2 + 2 * t + (e & 1) + 8 * (e >> 1);
                     if constexpr (D == 128) {
                         const uint4 u = *reinterpret_cast<const uint4*>(vt + key * D + ((g ^ (key & 7)) << 4));
                         w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
@@ -328,10 +364,18 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
                     }
                 }
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const uint32_t sel = (d & 3) | ((d & 3) << 4) | ((4 + (d & 3)) << 8) | ((4 + (d & 3)) << 12);
-                    pf_mma<DT>(o[d], pa, pf_codes<DT>(__byte_perm(w[0][d >> 2], w[1][d >> 2], sel)),
-                               pf_codes<DT>(__byte_perm(w[2][d >> 2], w[3][d >> 2], sel)));
+                for (int c = 0; c < D / 32; ++c) {
+                    // byte i of both keys of a pair, then 0x64 above each code
+                    const uint32_t a0 = __byte_perm(w[0][c], w[1][c], 0x5140) ^ 0x80808080u, a1 = __byte_perm(w[0][c], w[1][c], 0x7362) ^ 0x80808080u;
+                    const uint32_t b0 = __byte_perm(w[2][c], w[3][c], 0x5140) ^ 0x80808080u, b1 = __byte_perm(w[2][c], w[3][c], 0x7362) ^ 0x80808080u;
+                    const uint32_t f[2][4] = {{pf_codes(a0, 0x64646464u, 0x4140), pf_codes(a0, 0x64646464u, 0x4342),
+                                               pf_codes(b0, 0x64646464u, 0x4140), pf_codes(b0, 0x64646464u, 0x4342)},
+                                              {pf_codes(a1, 0x64646464u, 0x4140), pf_codes(a1, 0x64646464u, 0x4342),
+                                               pf_codes(b1, 0x64646464u, 0x4140), pf_codes(b1, 0x64646464u, 0x4342)}};
+#pragma unroll
+                    for (int d = 0; d < 2; ++d)
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) pf_mma<MT>(o[q][2 * c + d], f[d], p[i2][q][0], p[i2][q][1]);
                 }
             }
         }
@@ -342,10 +386,12 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
         }
     }
     // the warps' states join
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) l[q][j] += __shfl_xor_sync(0xffffffffu, l[q][j], w);
     __syncthreads();
     if (s_bad) {
         // a load never arrived: wait (bounded) for those in flight before the block's memory goes
@@ -356,14 +402,22 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
     float* so = reinterpret_cast<float*>(ring);          // [16][D + 4]
     constexpr int LD = D + 4;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-        const int c0 = Q8 ? 2 * t * ND + d : 8 * d + 2 * t, c1 = Q8 ? c0 + ND : c0 + 1;
-        so[g * LD + c0] = o[d][0];
-        so[g * LD + c1] = o[d][1];
-        so[(g + 8) * LD + c0] = o[d][2];
-        so[(g + 8) * LD + c1] = o[d][3];
+    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const int c0 = Q8 ? D / 8 * g + 2 * d : 16 * d + g, c1 = Q8 ? c0 + 1 : c0 + 8;
+            so[(8 * q + 2 * t) * LD + c0] = o[q][d][0];
+            so[(8 * q + 2 * t + 1) * LD + c0] = o[q][d][1];
+            so[(8 * q + 2 * t) * LD + c1] = o[q][d][2];
+            so[(8 * q + 2 * t + 1) * LD + c1] = o[q][d][3];
+        }
+        if (g == 0)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                s_m[warp][8 * q + 2 * t + j] = m[q][j];
+                s_l[warp][8 * q + 2 * t + j] = l[q][j];
+            }
     }
-    if (t == 0) { s_m[warp][g] = m0; s_m[warp][g + 8] = m1; s_l[warp][g] = l0; s_l[warp][g + 8] = l1; }
     __syncthreads();
     const int Hq = a.H * a.G;
     const float* all = reinterpret_cast<const float*>(sm);
@@ -400,14 +454,15 @@ template <int DT, int D, bool Q8> static int pf_launch(const PagedArgs& a, cudaS
     using C = PfCfg<D, Q8>;
     CUtensorMap mK, mV;
     const int page = 1 << a.page_shift;
+    const bool few8 = a.max_q * a.G <= 8;
     const CUtensorMapSwizzle sw = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     if (!paged_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages, PF_PIECE, sw) ||
         !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, PF_PIECE, sw))
         return QV_EINVAL;
-    const cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<DT, D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)C::SMEM);
+    auto kernel = few8 ? paged_few_kernel<DT, D, Q8, 1> : paged_few_kernel<DT, D, Q8, 2>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
     if (e != cudaSuccess) return set_cuda_error(e);
-    paged_few_kernel<DT, D, Q8><<<dim3((unsigned)(a.B * a.H), a.splits), PF_THREADS, C::SMEM, s>>>(mK, mV, a);
+    kernel<<<dim3((unsigned)(a.B * a.H), a.splits), PF_THREADS, C::SMEM, s>>>(mK, mV, a);
     return check_launch();
 }
 
