@@ -21,56 +21,87 @@ int paged_shift(int page);
 int paged_tc_launch(const PagedArgs& a, int dt, int D, bool q8, int64_t tiles, cudaStream_t s);
 int paged_few_launch(const PagedArgs& a, int dt, int D, bool q8, cudaStream_t s);
 
-constexpr int PC_THREADS = 128;
+constexpr int PC_THREADS = 256;
 
-// One block per (token, query head): its four warps take the splits in turn,
-// lane i holds columns of the row, and the warps' sums join in shared memory.
-template <int DT, int D>
+// W warps per (token, query head) row, 8 / W rows per block: one where there are
+// rows enough to fill the GPU, otherwise eight, which take a row's splits in
+// turn and join in shared memory.  Lane i holds D / 32 columns of the row.
+template <int DT, int D, int W>
 __global__ void __launch_bounds__(PC_THREADS) paged_combine_kernel(const PagedArgs a) {
     constexpr int E = D / 32;
-    __shared__ float s_o[4][D], s_l[4], s_m[4];
+    __shared__ float s_o[W > 1 ? W : 1][W > 1 ? D : 1], s_l[8], s_m[8];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the splits still run
     const int Hq = a.H * a.G;
-    const int t = blockIdx.x / Hq, hq = blockIdx.x % Hq;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * (8 / W) + (W == 1 ? warp : 0);
+    if (row >= (int64_t)a.total_q * Hq) return;
+    const int t = (int)(row / Hq);
     const int b = paged_find_token(a.cu_q, a.B, t);
     const PagedSeq s = paged_seq(a, b);
     const int i = t - s.q0;
     if (i < 0 || i >= s.live || s.kv <= a.chunk) return;   // behind the last sequence, or written by its only split
     const int limit = paged_limit(a, s, i);
     const int n = limit > 0 ? (limit + a.chunk - 1) / a.chunk : 0;
-    const size_t row = (size_t)t * Hq + hq, step = (size_t)a.total_q * Hq;
+    const size_t step = (size_t)a.total_q * Hq;
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int sp = warp; sp < n; sp += 4) {
-        const size_t p = sp * step + row;
-        const float ms = a.part_ml[2 * p], ls = a.part_ml[2 * p + 1];
-        float v[E];
+    for (int s0 = W == 1 ? 0 : warp; s0 < n; s0 += 4 * W) {
+        // four splits' loads at once
+        float ms[4], ls[4], v[4][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = a.part_o[p * D + E * lane + e];
-        const float mn = fmaxf(m, ms), base = mn == -INFINITY ? 0.f : mn;
-        const float f = exp2f(m - base), g = exp2f(ms - base);
-        l = l * f + ls * g;
+        for (int u = 0; u < 4; ++u) {
+            const int sp = s0 + u * W;
+            ms[u] = -INFINITY;
+            ls[u] = 0.f;
+            if (sp < n) {
+                const size_t p = sp * step + row;
+                ms[u] = a.part_ml[2 * p];
+                ls[u] = a.part_ml[2 * p + 1];
+            }
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + v[e] * g;
+            for (int e = 0; e < E; ++e) v[u][e] = sp < n ? a.part_o[(sp * step + row) * D + E * lane + e] : 0.f;
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mn = fmaxf(mn, ms[u]);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float f = exp2f(m - base);
         m = mn;
-    }
+        l *= f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s_o[warp][E * lane + e] = o[e];
-    if (lane == 0) { s_l[warp] = l; s_m[warp] = m; }
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    const float mm = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    const float base = mm == -INFINITY ? 0.f : mm;
-    float sum = 0.f, x = 0.f;
+        for (int e = 0; e < E; ++e) o[e] *= f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float f = exp2f(s_m[w] - base);
-        sum += s_l[w] * f;
-        x += s_o[w][threadIdx.x] * f;
+        for (int u = 0; u < 4; ++u) {
+            const float g = exp2f(ms[u] - base);
+            l = fmaf(ls[u], g, l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(v[u][e], g, o[e]);
+        }
     }
-    st<DT>(a.out, row * D + threadIdx.x, sum > 0.f ? x / sum : sum);
+    if constexpr (W == 1) {
+        const float inv = l > 0.f ? 1.f / l : l;
+#pragma unroll
+        for (int e = 0; e < E; ++e) st<DT>(a.out, row * D + E * lane + e, o[e] * inv);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_o[warp][E * lane + e] = o[e];
+        if (lane == 0) { s_l[warp] = l; s_m[warp] = m; }
+        __syncthreads();
+        if (threadIdx.x >= D) return;
+        float mm = s_m[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) mm = fmaxf(mm, s_m[w]);
+        const float base = mm == -INFINITY ? 0.f : mm;
+        float sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = exp2f(s_m[w] - base);
+            sum = fmaf(s_l[w], f, sum);
+            x = fmaf(s_o[w][threadIdx.x], f, x);
+        }
+        st<DT>(a.out, row * D + threadIdx.x, sum > 0.f ? x / sum : sum);
+    }
 }
 
 // ---------------------------------------------------------------- plan
@@ -105,6 +136,8 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int total_q, int max_q,
     int64_t n = blocks > 0 ? ceil_div(want, blocks) : 1;
     const int64_t most = ceil_div(max_kv, least);
     if (n > most) n = most;
+    // what does not fill its last round fills one round fewer
+    if (B == 1 && n > 1 && blocks * n > want) --n;
     if (n < 1) n = 1;
     p.chunk = (int)(ceil_div(ceil_div(max_kv, n), 128) * 128);
     if (p.chunk < 128) p.chunk = 128;
@@ -140,8 +173,10 @@ template <int DT, int D> static int paged_launch(const PagedArgs& a, const Paged
     else if (p.kernel == PK_FEW) rc = paged_few_launch(a, DT, D, q8, s);
     else rc = paged_tc_launch(a, DT, D, q8, p.tiles, s);
     if (rc != QV_OK || p.splits == 1) return rc;
-    const cudaError_t e = launch_pdl(paged_combine_kernel<DT, D>, dim3((unsigned)((int64_t)a.total_q * a.H * a.G)),
-                                     dim3(PC_THREADS), 0, s, a);
+    const int64_t rows = (int64_t)a.total_q * a.H * a.G;
+    const bool many = rows >= 16 * 148;
+    const cudaError_t e = launch_pdl(many ? paged_combine_kernel<DT, D, 1> : paged_combine_kernel<DT, D, 8>,
+                                     dim3((unsigned)(many ? ceil_div(rows, 8) : rows)), dim3(PC_THREADS), 0, s, a);
     return e == cudaSuccess ? check_launch() : set_cuda_error(e);
 }
 

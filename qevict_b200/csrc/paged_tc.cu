@@ -10,21 +10,27 @@
 // products, so a key tile costs the larger of 2 x 2 products and the
 // exponentials (16 per clock and SM) instead of their sum.
 //
-// m_x is a reference, not always the maximum: it moves (and O_x, l_x are
-// rescaled) only when a tile's maximum exceeds it by more than 2^8.  P is then
-// at most 2^8, which neither 16-bit type's relative rounding nor the fp32 sums
-// notice, and O stays in TMEM untouched for almost every tile.
+// m_x is a reference, not the running maximum: softmax is the same for any m, and
+// P only has to stay in its type's range.  The first tile sets m to its maximum
+// (fp16: 2^7 below, so that P spans 2^-31 .. 2^8 relative to it); later tiles use
+// it at once and move it only where P would pass 2^60 (fp16: 2^15), rescaling
+// O_x and l_x.  So almost no tile waits for a maximum or touches O in TMEM.
 //
-// INT8 pages: codes become exact 16-bit integers in shared memory (four extra
-// warps); the row scales stay in fp32.  With ks, vs the scales of key j,
-//   u_j = S_j c ks_j + log2(vs_j),  P_j = exp2(u_j - m),  O = sum P_j code_j,
-//   l = sum P_j / vs_j,
-// so the value scale sits inside the exponent that P is rounded from: one
-// rounding, as without INT8, and the row's reference m keeps P in the type's
-// range whatever the scales are.
+// (Measured and left out, 8192-token prompt at D = 128, 443 us: a quarter of the
+// exponentials as a polynomial on the FMA pipe, 462 us; the two tiles' softmax
+// warps taking turns at the exponentials, 456 us.  Without any exponentials it
+// takes 443 us too: the tensor pipe at the clock that its power allows bounds it.)
+//
+// INT8 pages: codes become exact 16-bit integers in shared memory (six extra
+// warps); the row scales ks, vs of a key stay in fp32: the logit is S c ks, and the
+// value scale goes into P before its one rounding.  bf16 has the range for that:
+//   p = exp2(S c ks - m),  l += p,  P = p vs,  O += P code.
+// In fp16 it goes into the exponent, so that the row's reference keeps P in range
+// whatever the scales are:
+//   P = exp2(S c ks + log2(vs) - m),  l += P / vs,  O += P code.
 //
 // Warps 0-3 and 4-7: the softmax of the two tiles; 8: TMA; 9: MMA (one elected
-// thread each); with INT8 12-15 convert.  Every wait is bounded.
+// thread each); with INT8 10-15 convert.  Every wait is bounded.
 #include <cudaTypedefs.h>
 #include <math.h>
 
@@ -36,16 +42,17 @@ namespace qv {
 
 constexpr int PT_KEYS = 128;
 constexpr int PT_SLAB = 16384;            // 128 rows x 64 16-bit elements, 128-byte swizzle
-constexpr float PT_LAZY = 8.f;            // the reference moves past 2^8
 constexpr int PT_SC = 4;                  // tiles of row scales held (INT8)
 constexpr float PT_MIN_SCALE = 7.8886090522101181e-31f;   // 2^-100: a smaller value scale counts as this
 
-template <int D, bool Q8> struct PtCfg {
+template <int DT, int D, bool Q8> struct PtCfg {
     static constexpr int NS = D / 64;                       // slabs per operand tile
     static constexpr int SLOT = NS * PT_SLAB;
     static constexpr int SLOTS = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8);   // K and V tiles in turn
     static constexpr int RAW = PT_KEYS * D;                 // one tile of codes
     static constexpr int RAWS = Q8 ? 2 : 0;
+    // a row's reference is set this far (base 2) below a maximum, and moves when a logit exceeds it by FAR
+    static constexpr float BELOW = DT == QV_F16 ? 7.f : 0.f, FAR = DT == QV_F16 ? 15.f : 60.f;
     static constexpr int THREADS = Q8 ? 512 : 384;
     // registers per thread after the split (the launch holds 128 x 512 or 168 x 384 of them)
     static constexpr int REGS_SOFTMAX = Q8 ? 192 : 208, REGS_OTHER = Q8 ? 64 : 88;
@@ -79,6 +86,12 @@ __device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ uint64_t pt_mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pt_both(float x) { return pt_pack(x, x); }
 __device__ __forceinline__ float pt_max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -129,10 +142,10 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile
 }
 
 template <int DT, int D, bool Q8>
-__global__ void __launch_bounds__(PtCfg<D, Q8>::THREADS, 1)
+__global__ void __launch_bounds__(PtCfg<DT, D, Q8>::THREADS, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
                 const __grid_constant__ CUtensorMap mV, const PagedArgs a) {
-    using C = PtCfg<D, Q8>;
+    using C = PtCfg<DT, D, Q8>;
     constexpr int NS = C::NS, SLOT = C::SLOT, SLOTS = C::SLOTS;
     extern __shared__ unsigned char pt_raw[];
     unsigned char* sm = pt_raw + ((1024u - (smem_u32(pt_raw) & 1023u)) & 1023u);
@@ -140,13 +153,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
     unsigned char* sKV = sQ + 2 * SLOT;                  // [SLOTS]: K0, V0, K1, V1, ...
     unsigned char* sRaw = sKV + SLOTS * SLOT;            // [RAWS] tiles of codes
     float* sRawSc = reinterpret_cast<float*>(sRaw + C::RAWS * C::RAW);   // [2][128] as loaded: ks, vs
-    float* sSc = sRawSc + 2 * PT_KEYS;                   // [PT_SC][3][128]: c ks, log2 vs, 1 / vs
+    float* sSc = sRawSc + 2 * PT_KEYS;                   // [PT_SC][3][128]: c ks and vs, or (fp16) c ks, log2 vs, 1 / vs
     __shared__ __align__(8) uint64_t q_full, kv_full[SLOTS], kv_empty[SLOTS], raw_full[2], raw_empty[2], sc_full[PT_SC];
-    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], tail, done;
+    __shared__ __align__(8) uint64_t s_full[2], p_full[2][2], o_full[2], tail, done;
     __shared__ uint32_t s_taddr;
     __shared__ int2 s_tile;
     __shared__ int s_quit;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
     const int h = blockIdx.x % a.H, sp = blockIdx.y;
     const int QT = PT_KEYS / a.G;                        // tokens per row tile
 
@@ -182,10 +195,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
     if (warp == 9) { tmem_alloc(&s_taddr, 512); tmem_relinquish(); }
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
-        for (int i = 0; i < SLOTS; ++i) { mbar_init(&kv_full[i], Q8 ? 4 : 1); mbar_init(&kv_empty[i], 1); }
+        for (int i = 0; i < SLOTS; ++i) { mbar_init(&kv_full[i], Q8 ? 6 : 1); mbar_init(&kv_empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4);
-            mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
+            mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 6);
+            mbar_init(&s_full[i], 1); mbar_init(&o_full[i], 1);
+            mbar_init(&p_full[i][0], 4); mbar_init(&p_full[i][1], 4);
         }
         for (int i = 0; i < PT_SC; ++i) mbar_init(&sc_full[i], 4);
         mbar_init(&tail, 1);
@@ -209,6 +223,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
         const int tok_x = x ? tok[1] : tok[0], tn = x ? nt[1] : nt[0];
         const bool live = i < (x ? cnt[1] : cnt[0]);
         int lim = live ? paged_limit(a, s, tok_x + i) - k_begin : 0x7fffffff;   // relative to the block's range
+        const bool idle = 32 * (warp & 3) >= (x ? cnt[1] : cnt[0]) * a.G;
         int lim_min = lim;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
@@ -225,19 +240,33 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
+            if (idle) {                      // no live row in this warp: P may hold anything there
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&p_full[x][0]); mbar_arrive(&p_full[x][1]); }
+                continue;
+            }
             float v[128];
 #pragma unroll
             for (int w = 0; w < 4; ++w) tmem_ld32(ts + 32 * w, v + 32 * w);
             tmem_wait_ld();
             const float* sc = sSc + (j % PT_SC) * 3 * PT_KEYS;
             if constexpr (Q8) {
-                // base-2 logits with the value scale in them
+                // base-2 logits (fp16: with the value scale in them)
 #pragma unroll
                 for (int e = 0; e < 128; e += 4) {
                     const float4 k4 = *reinterpret_cast<const float4*>(sc + e);
-                    const float4 l4 = *reinterpret_cast<const float4*>(sc + PT_KEYS + e);
-                    pt_unpack(pt_fma2(pt_pack(v[e], v[e + 1]), pt_pack(k4.x, k4.y), pt_pack(l4.x, l4.y)), v[e], v[e + 1]);
-                    pt_unpack(pt_fma2(pt_pack(v[e + 2], v[e + 3]), pt_pack(k4.z, k4.w), pt_pack(l4.z, l4.w)), v[e + 2], v[e + 3]);
+                    uint64_t u0, u1;
+                    if constexpr (DT == QV_F16) {
+                        const float4 l4 = *reinterpret_cast<const float4*>(sc + PT_KEYS + e);
+                        u0 = pt_fma2(pt_pack(v[e], v[e + 1]), pt_pack(k4.x, k4.y), pt_pack(l4.x, l4.y));
+                        u1 = pt_fma2(pt_pack(v[e + 2], v[e + 3]), pt_pack(k4.z, k4.w), pt_pack(l4.z, l4.w));
+                    } else {
+                        u0 = pt_mul2(pt_pack(v[e], v[e + 1]), pt_pack(k4.x, k4.y));
+                        u1 = pt_mul2(pt_pack(v[e + 2], v[e + 3]), pt_pack(k4.z, k4.w));
+                    }
+                    pt_unpack(u0, v[e], v[e + 1]);
+                    pt_unpack(u1, v[e + 2], v[e + 3]);
                 }
             }
             const int seen = lim - j * PT_KEYS;
@@ -245,20 +274,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
 #pragma unroll
                 for (int e = 0; e < 128; ++e) v[e] = e < seen ? v[e] : -INFINITY;
             }
-            float mx0 = v[0], mx1 = v[1];
+            float hi[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-            for (int e = 2; e < 126; e += 4) {
-                mx0 = pt_max3(mx0, v[e], v[e + 1]);
-                mx1 = pt_max3(mx1, v[e + 2], v[e + 3]);
-            }
-            float mx = fmaxf(pt_max3(mx0, v[126], v[127]), mx1);
+            for (int e = 4; e < 124; e += 8)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) hi[w] = pt_max3(hi[w], v[e + 2 * w], v[e + 2 * w + 1]);
+            float mx = pt_max3(pt_max3(hi[0], hi[1], hi[2]), pt_max3(hi[3], v[124], v[125]), fmaxf(v[126], v[127]));
             if (!Q8) mx *= cl;
-            const bool move = mx > m + PT_LAZY;
-            if (__any_sync(0xffffffffu, move)) {
-                const float mn = move ? mx : m;
+            if (__any_sync(0xffffffffu, mx > m + C::FAR)) {
+                // the reference moves, and what was summed before follows
+                const bool move = mx > m + C::FAR;
+                const float mn = move ? mx - C::BELOW : m;
                 const float f = move && m != -INFINITY ? pt_ex2(m - mn) : 1.f;
                 m = mn;
-                l2 = pt_fma2(l2, pt_pack(f, f), pt_pack(0.f, 0.f));
+                l2 = pt_mul2(l2, pt_both(f));
                 if (j > 0) {
                     // S(j) is complete, so P.V of every earlier tile is
 #pragma unroll
@@ -273,33 +302,51 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
                     }
                 }
             }
-            const float base = m == -INFINITY ? 0.f : m;     // nothing seen yet: every term is 0
-            const uint64_t nm2 = pt_pack(-base, -base);
+            const uint64_t nm2 = pt_both(m == -INFINITY ? 0.f : -m);     // nothing seen yet: every term is 0
+            uint64_t acc[2] = {l2, pt_both(0.f)};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 uint32_t p[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                for (int e = 0; e < 16; e += 2) {
                     const int k = 32 * w + 2 * e;
-                    float d0, d1;
-                    if (Q8) pt_unpack(pt_add2(pt_pack(v[k], v[k + 1]), nm2), d0, d1);
-                    else pt_unpack(pt_fma2(pt_pack(v[k], v[k + 1]), c2, nm2), d0, d1);
-                    d0 = pt_ex2(d0);
-                    d1 = pt_ex2(d1);
-                    if (Q8) {
-                        const float2 iv = *reinterpret_cast<const float2*>(sc + 2 * PT_KEYS + k);
-                        l2 = pt_fma2(pt_pack(d0, d1), pt_pack(iv.x, iv.y), l2);
-                    } else {
-                        l2 = pt_add2(l2, pt_pack(d0, d1));
+                    float d[4];
+#pragma unroll
+                    for (int h2 = 0; h2 < 2; ++h2) {
+                        const uint64_t v2 = pt_pack(v[k + 2 * h2], v[k + 2 * h2 + 1]);
+                        pt_unpack(Q8 ? pt_add2(v2, nm2) : pt_fma2(v2, c2, nm2), d[2 * h2], d[2 * h2 + 1]);
                     }
-                    p[e] = pt_cvt2<DT>(d0, d1);
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) d[i4] = pt_ex2(d[i4]);
+                    if constexpr (Q8) {
+                        // 1 / vs (fp16), or vs
+                        const float4 f4 = *reinterpret_cast<const float4*>(sc + (DT == QV_F16 ? 2 : 1) * PT_KEYS + k);
+                        const uint64_t f0 = pt_pack(f4.x, f4.y), f1 = pt_pack(f4.z, f4.w);
+                        if constexpr (DT == QV_F16) {
+                            acc[0] = pt_fma2(pt_pack(d[0], d[1]), f0, acc[0]);
+                            acc[1] = pt_fma2(pt_pack(d[2], d[3]), f1, acc[1]);
+                        } else {
+                            acc[0] = pt_add2(acc[0], pt_pack(d[0], d[1]));
+                            acc[1] = pt_add2(acc[1], pt_pack(d[2], d[3]));
+                            pt_unpack(pt_mul2(pt_pack(d[0], d[1]), f0), d[0], d[1]);
+                            pt_unpack(pt_mul2(pt_pack(d[2], d[3]), f1), d[2], d[3]);
+                        }
+                    } else {
+                        acc[0] = pt_add2(acc[0], pt_pack(d[0], d[1]));
+                        acc[1] = pt_add2(acc[1], pt_pack(d[2], d[3]));
+                    }
+                    p[e] = pt_cvt2<DT>(d[0], d[1]);
+                    p[e + 1] = pt_cvt2<DT>(d[2], d[3]);
                 }
                 tmem_st16(ts + 16 * w, p);
+                if (w & 1) {                 // 64 keys of P: the product may start on them
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[x][w >> 1]);
+                }
             }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[x]);
+            l2 = pt_add2(acc[0], acc[1]);
         }
         float l0, l1;
         pt_unpack(l2, l0, l1);
@@ -426,24 +473,33 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
             for (int it = max(issued - RING, 0); it < issued; ++it) mbar_wait_bounded(&full[it % RING], (it / RING) & 1);
         } else if (warp == 9) {
             // -------------------------------------------------------- products
-            if (lane == 0 && n > 0) {
+            // the whole warp walks the loop (operands in uniform registers), one elected lane issues
+            if (n > 0) {
                 const uint32_t id_s = umma_idesc_f16(DT == QV_BF16, 128, 128, 0, 0);
                 const uint32_t id_o = umma_idesc_f16(DT == QV_BF16, 128, D, 0, 1);
-                bool ok = pt_wait(&q_full, 0, quit, a.err);
+                const uint64_t dq = umma_desc_sw128(smem_u32(sQ), 16, 1024);
+                const uint64_t dk = umma_desc_sw128(smem_u32(sKV), 16, 1024);
+                const uint64_t dv = umma_desc_sw128(smem_u32(sKV), PT_SLAB, 1024);
+                const bool one = elect_one();
+                auto wait = [&](uint64_t* bar, uint32_t parity) {
+                    return __all_sync(0xffffffffu, pt_wait(bar, parity, quit, a.err)) != 0;
+                };
+                bool ok = wait(&q_full, 0);
                 tc_fence_after();
                 auto scores = [&](int x, int j) {
-                    const uint32_t qa = smem_u32(sQ + x * SLOT), ka = smem_u32(sKV + ((2 * j) % SLOTS) * SLOT);
+                    const uint64_t q = dq + x * (SLOT >> 4), k = dk + ((2 * j) % SLOTS) * (SLOT >> 4);
+                    if (one) {
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * PT_SLAB + (kk & 3) * 32;
-                        umma_f16(taddr + 128 * x, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024),
-                                 id_s, kk > 0);
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            constexpr int S4 = PT_SLAB >> 4;
+                            umma_ss(taddr + 128 * x, q + (kk >> 2) * S4 + (kk & 3) * 2, k + (kk >> 2) * S4 + (kk & 3) * 2, id_s, kk > 0);
+                        }
+                        umma_commit(&s_full[x]);
                     }
-                    umma_commit(&s_full[x]);
                 };
                 auto wait_tile = [&](int it) {
-                    bool o = pt_wait(&kv_full[it % SLOTS], (it / SLOTS) & 1, quit, a.err);
-                    if (!Q8 && o && cut && it == 2 * n - 1) o = pt_wait(&tail, 0, quit, a.err);
+                    bool o = wait(&kv_full[it % SLOTS], (it / SLOTS) & 1);
+                    if (!Q8 && o && cut && it == 2 * n - 1) o = wait(&tail, 0);
                     tc_fence_after();
                     return o;
                 };
@@ -452,7 +508,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
                         if (nt[x] > 0) scores(x, 0);
-                    umma_commit(&kv_empty[0]);
+                    if (one) umma_commit(&kv_empty[0]);
                 }
                 for (int j = 0; j < n && ok; ++j) {
                     bool v_in = false, k_in = false;
@@ -461,32 +517,75 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
                         if (!ok || j >= nt[x]) continue;
                         const bool last_user = x == 1 || j >= nt[1];
                         if (!v_in) { ok = wait_tile(2 * j + 1); v_in = true; }
-                        if (ok) ok = pt_wait(&p_full[x], j & 1, quit, a.err);
-                        if (!ok) continue;
-                        tc_fence_after();
-                        const uint32_t va = smem_u32(sKV + ((2 * j + 1) % SLOTS) * SLOT);
+                        const uint64_t v = dv + ((2 * j + 1) % SLOTS) * (SLOT >> 4);
 #pragma unroll
-                        for (int kk = 0; kk < PT_KEYS / 16; ++kk)
-                            umma_f16_ta(taddr + 256 + 128 * x, taddr + 128 * x + 8 * kk,
-                                        umma_desc_sw128(va + kk * 2048, PT_SLAB, 1024), id_o, (j > 0 || kk > 0) ? 1 : 0);
-                        if (j + 1 == nt[x]) umma_commit(&o_full[x]);
-                        if (last_user) umma_commit(&kv_empty[(2 * j + 1) % SLOTS]);
+                        for (int hf = 0; hf < 2; ++hf) {
+                            if (ok) ok = wait(&p_full[x][hf], j & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            if (one) {
+#pragma unroll
+                                for (int kk = 4 * hf; kk < 4 * hf + 4; ++kk)
+                                    umma_ts(taddr + 256 + 128 * x, taddr + 128 * x + 8 * kk, v + kk * 128, id_o, j > 0 || kk > 0);
+                            }
+                        }
+                        if (!ok) continue;
+                        if (one) {
+                            if (j + 1 == nt[x]) umma_commit(&o_full[x]);
+                            if (last_user) umma_commit(&kv_empty[(2 * j + 1) % SLOTS]);
+                        }
                         if (j + 1 < nt[x]) {
                             if (!k_in) { ok = wait_tile(2 * j + 2); k_in = true; }
                             if (!ok) continue;
                             scores(x, j + 1);
-                            if (x == 1 || j + 1 >= nt[1]) umma_commit(&kv_empty[(2 * j + 2) % SLOTS]);
+                            if (one && (x == 1 || j + 1 >= nt[1])) umma_commit(&kv_empty[(2 * j + 2) % SLOTS]);
                         }
                     }
                 }
                 // no MMA is in flight when the TMEM is released
-                umma_commit(&done);
+                if (one) umma_commit(&done);
                 mbar_wait_bounded(&done, 0);
             }
-        } else if (Q8 && warp >= 12) {
+        } else if (Q8 && warp >= 10) {
             // -------------------------------------------------------- codes -> 16-bit operands
-            const int t = threadIdx.x - 384;
-            constexpr int CPR = D / 16;              // 16-code chunks per row
+            // A tile is PARTS x 128 chunks of 16 codes.  Warps 12-15 (t = 0..127) take the first five eighths of
+            // the parts, warps 10 and 11 the rest, each lane two chunks of a part.  Eight lanes hold four chunks
+            // of two rows, so that neither their reads (128-byte swizzle at D = 128) nor their writes share
+            // banks: rows r and r ^ 5, or (D = 64) r and r + 1; parts differ by constants.
+            constexpr int PARTS = PT_KEYS * D / 16 / 128, FIRST = PARTS * 5 / 8;
+            const bool extra = warp < 12;
+            const int t = extra ? threadIdx.x - 320 : threadIdx.x - 384;
+            auto place = [&](int i, int& from, int& to0, int& to1) {     // chunk i of part 0
+                int r, cc;
+                if constexpr (D == 128) {
+                    r = (i >> 5) * 8 + ((i >> 3) & 3);
+                    if (i & 4) r ^= 5;
+                    cc = i & 3;
+                    from = r * 128 + ((cc ^ (r & 7)) << 4);
+                } else {
+                    r = i >> 2;
+                    cc = i & 3;
+                    from = r * 64 + cc * 16;
+                }
+                to0 = r * 128 + (((2 * cc) ^ (r & 7)) << 4);
+                to1 = r * 128 + (((2 * cc + 1) ^ (r & 7)) << 4);
+            };
+            // D = 128: parts 0-3 are rows +32 each of the low four chunks, 4-7 of the high four (the other slab)
+            auto convert = [&](const unsigned char* raw, unsigned char* dst, int part, int from, int to0, int to1, int rows) {
+                const int r = (to0 >> 7) + 32 * (part & 3);
+                const unsigned char* src = raw + (D == 128 ? (from ^ ((part >> 2) << 6)) + (part & 3) * 32 * 128 : from + part * 32 * 64);
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (r < rows) u = *reinterpret_cast<const uint4*>(src);
+                constexpr uint32_t S0 = 0x4140, S1 = 0x4342;
+                unsigned char* out = dst + (D == 128 ? part >> 2 : 0) * PT_SLAB + (part & 3) * 32 * 128;
+                *reinterpret_cast<uint4*>(out + to0) = make_uint4(pt_codes2<DT>(u.x, S0), pt_codes2<DT>(u.x, S1),
+                                                                  pt_codes2<DT>(u.y, S0), pt_codes2<DT>(u.y, S1));
+                *reinterpret_cast<uint4*>(out + to1) = make_uint4(pt_codes2<DT>(u.z, S0), pt_codes2<DT>(u.z, S1),
+                                                                  pt_codes2<DT>(u.w, S0), pt_codes2<DT>(u.w, S1));
+            };
+            int from[2], to0[2], to1[2];
+            place(t, from[0], to0[0], to1[0]);
+            place(extra ? t + 64 : t, from[1], to0[1], to1[1]);
             bool ok = true;
             for (int it = 0; it < 2 * n && ok; ++it) {
                 const int st = it & 1, slot = it % SLOTS, j = it >> 1;
@@ -495,40 +594,39 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const int rows = j + 1 == n ? min(live_last, PT_KEYS) : PT_KEYS;
-                if ((it & 1) == 0) {
+                if ((it & 1) == 0 && !extra) {
                     // scales of this tile's keys; one behind the sequence contributes nothing
                     float* sc = sSc + (j % PT_SC) * 3 * PT_KEYS;
                     const float ks = sRawSc[t];
                     float vs = sRawSc[PT_KEYS + t];
-                    if (vs < PT_MIN_SCALE) vs = PT_MIN_SCALE;    // also a zero row, whose codes are 0
                     const bool in = t < rows;
                     sc[t] = in ? ks * a.scale_log2 : 0.f;
-                    sc[PT_KEYS + t] = in ? log2f(vs) : 0.f;
-                    sc[2 * PT_KEYS + t] = in ? 1.f / vs : 0.f;
+                    if constexpr (DT == QV_F16) {
+                        if (vs < PT_MIN_SCALE) vs = PT_MIN_SCALE;    // also a zero row, whose codes are 0
+                        sc[PT_KEYS + t] = in ? log2f(vs) : 0.f;
+                        sc[2 * PT_KEYS + t] = in ? 1.f / vs : 0.f;
+                    } else {
+                        sc[PT_KEYS + t] = in ? vs : 0.f;
+                    }
                 }
                 const unsigned char* raw = sRaw + st * C::RAW;
                 unsigned char* dst = sKV + slot * SLOT;
-#pragma unroll 4
-                for (int c = t; c < PT_KEYS * CPR; c += 128) {
-                    const int r = c / CPR, cc = c % CPR;
-                    uint4 u = make_uint4(0, 0, 0, 0);
-                    if (r < rows) u = *reinterpret_cast<const uint4*>(raw + r * D + cc * 16);
-                    constexpr uint32_t S0 = 0x4140, S1 = 0x4342;
-                    uint4 lo = make_uint4(pt_codes2<DT>(u.x, S0), pt_codes2<DT>(u.x, S1), pt_codes2<DT>(u.y, S0),
-                                          pt_codes2<DT>(u.y, S1));
-                    uint4 hi = make_uint4(pt_codes2<DT>(u.z, S0), pt_codes2<DT>(u.z, S1), pt_codes2<DT>(u.w, S0),
-                                          pt_codes2<DT>(u.w, S1));
-                    unsigned char* row = dst + (cc >> 2) * PT_SLAB + r * 128;
-                    const int ch = (2 * cc) & 7;
-                    *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = lo;
-                    *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = hi;
+                if (!extra) {
+#pragma unroll
+                    for (int part = 0; part < FIRST; ++part) convert(raw, dst, part, from[0], to0[0], to1[0], rows);
+                } else {
+#pragma unroll
+                    for (int part = FIRST; part < PARTS; ++part) {
+                        convert(raw, dst, part, from[0], to0[0], to1[0], rows);
+                        convert(raw, dst, part, from[1], to0[1], to1[1], rows);
+                    }
                 }
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&kv_full[slot]);
                     mbar_arrive(&raw_empty[st]);
-                    if ((it & 1) == 0) mbar_arrive(&sc_full[j % PT_SC]);
+                    if ((it & 1) == 0 && !extra) mbar_arrive(&sc_full[j % PT_SC]);
                 }
             }
         }
@@ -589,11 +687,12 @@ static bool pt_map_q(CUtensorMap* m, const PagedArgs& a, int dt, int D) {
 }
 
 template <int DT, int D, bool Q8> static int pt_launch(const PagedArgs& a, int64_t tiles, cudaStream_t s) {
-    using C = PtCfg<D, Q8>;
+    using C = PtCfg<DT, D, Q8>;
     CUtensorMap mQ, mK, mV;
     const int page = 1 << a.page_shift;
-    if (!pt_map_q(&mQ, a, DT, D) || !paged_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages, page, CU_TENSOR_MAP_SWIZZLE_NONE) ||
-        !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, page, CU_TENSOR_MAP_SWIZZLE_NONE))
+    const CUtensorMapSwizzle sw = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE;
+    if (!pt_map_q(&mQ, a, DT, D) || !paged_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages, page, sw) ||
+        !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, page, sw))
         return QV_EINVAL;
     const cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<DT, D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)C::SMEM);
