@@ -55,15 +55,54 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 enum { PH_ROWS_ONLY = 0, PH_PAGES = 1, PH_PAGES8 = 2 };
 
+// Packed fp32 pairs.
+__device__ __forceinline__ uint64_t ph_pack(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void ph_unpack(uint64_t r, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(r));
+}
+__device__ __forceinline__ uint64_t ph_mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t ph_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 // TPR threads share a head row (8 elements each, TPR a power of two >= D/8).
 template <int DT, int TPR, int MODE>
-__global__ void __launch_bounds__(PH_THREADS) heads_kernel(const HeadArgs a) {
+__global__ void __launch_bounds__(PH_THREADS, DT == QV_F32 ? 3 : 4) heads_kernel(const __grid_constant__ HeadArgs a) {
+    using T = typename Elt<DT>::T;
     constexpr int HPB = PH_THREADS / TPR;
+    __shared__ __align__(16) float s_w[2][256];          // norm weights of q and k (1 where there is none)
     const size_t t = blockIdx.x;
     const int c = threadIdx.x & (TPR - 1), hl = threadIdx.x / TPR;
     const int lane = threadIdx.x & 31;
     const bool on = 8 * c < a.D;
     const int rows = MODE == PH_ROWS_ONLY ? a.Hq + a.H : a.Hq + 2 * a.H;
+    const T* qt = reinterpret_cast<const T*>(a.q) + t * a.qs + 8 * c;
+    const T* kt = reinterpret_cast<const T*>(a.k) + t * a.ks + 8 * c - (size_t)a.Hq * a.D;
+    const T* vt = MODE == PH_ROWS_ONLY ? nullptr : reinterpret_cast<const T*>(a.v) + t * a.vs + 8 * c - (size_t)(a.Hq + a.H) * a.D;
+    auto fetch = [&](int r0, Chunk8<DT>* raw) {
+#pragma unroll
+        for (int i = 0; i < PH_ROWS; ++i) {
+            const int r = r0 + i * HPB + hl;
+#pragma unroll
+            for (int w = 0; w < (DT == QV_F32 ? 2 : 1); ++w) raw[i].u[w] = make_uint4(0, 0, 0, 0);
+            if (r < rows && on) {
+                const T* src = r < a.Hq ? qt : MODE == PH_ROWS_ONLY || r < a.Hq + a.H ? kt : vt;
+                raw[i] = load8<DT>(src, (size_t)(r * a.D));
+            }
+        }
+    };
+    Chunk8<DT> raw[PH_ROWS];
+    fetch(0, raw);                                       // before anything waits for the position's table row
 
     int64_t slot = -1;
     if (MODE != PH_ROWS_ONLY) {
@@ -73,15 +112,18 @@ __global__ void __launch_bounds__(PH_THREADS) heads_kernel(const HeadArgs a) {
             slot = -1;
         }
     }
-    float qw[8], kw[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) qw[i] = kw[i] = 1.f;
-    if (a.qw && on) widen8<DT>(load8<DT>(a.qw, 8 * c), qw);
-    if (a.kw && on) widen8<DT>(load8<DT>(a.kw, 8 * c), kw);
-
+    const bool norm = a.qw || a.kw;
+    if (norm) {
+        for (int i = threadIdx.x; i < 2 * a.D; i += PH_THREADS) {
+            const int k = i >= a.D, d = k ? i - a.D : i;
+            const void* w = k ? a.kw : a.qw;
+            s_w[k][d] = w ? ld<DT>(w, d) : 1.f;
+        }
+        __syncthreads();
+    }
     // the thread's rotation factors and where its partner elements sit: 4-element
     // sub-chunk u = 2c + s of a half-layout head pairs with u +- rot/8
-    float cs[8], sn[8];
+    uint64_t cs[4], sn[4];
     bool turn[2] = {false, false};
     int src[2] = {lane, lane};
     const int r8 = a.rot >> 3;
@@ -106,28 +148,19 @@ __global__ void __launch_bounds__(PH_THREADS) heads_kernel(const HeadArgs a) {
             const float* ce = reinterpret_cast<const float*>(&cv);
             const float* se = reinterpret_cast<const float*>(&sv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = a.interleaved ? 2 * s + (i >> 1) : i;
-                const bool first = a.interleaved ? (i & 1) == 0 : u < r8;
-                cs[4 * s + i] = ce[j] + bad;
-                sn[4 * s + i] = (first ? -se[j] : se[j]) + bad;
+            for (int i = 0; i < 4; i += 2) {
+                const int j0 = a.interleaved ? 2 * s + (i >> 1) : i, j1 = a.interleaved ? j0 : i + 1;
+                const float s0 = se[j0] + bad, s1 = se[j1] + bad;
+                cs[2 * s + i / 2] = ph_pack(ce[j0] + bad, ce[j1] + bad);
+                sn[2 * s + i / 2] = a.interleaved ? ph_pack(-s0, s0) : u < r8 ? ph_pack(-s0, -s1) : ph_pack(s0, s1);
             }
         }
     }
+    const float inv_d = 1.f / (float)a.D;
+    const bool swap = r8 & 1;                            // half layout: partners sit in the other sub-chunk
 
     for (int r0 = 0; r0 < rows; r0 += HPB * PH_ROWS) {
-        Chunk8<DT> raw[PH_ROWS];
-#pragma unroll
-        for (int i = 0; i < PH_ROWS; ++i) {
-            const int r = r0 + i * HPB + hl;
-#pragma unroll
-            for (int w = 0; w < (DT == QV_F32 ? 2 : 1); ++w) raw[i].u[w] = make_uint4(0, 0, 0, 0);
-            if (r < rows && on) {
-                if (r < a.Hq) raw[i] = load8<DT>(a.q, t * a.qs + (size_t)r * a.D + 8 * c);
-                else if (r < a.Hq + a.H) raw[i] = load8<DT>(a.k, t * a.ks + (size_t)(r - a.Hq) * a.D + 8 * c);
-                else raw[i] = load8<DT>(a.v, t * a.vs + (size_t)(r - a.Hq - a.H) * a.D + 8 * c);
-            }
-        }
+        if (r0 > 0) fetch(r0, raw);
 #pragma unroll
         for (int i = 0; i < PH_ROWS; ++i) {
             if (r0 + i * HPB >= rows) break;   // the same for the whole block
@@ -135,16 +168,25 @@ __global__ void __launch_bounds__(PH_THREADS) heads_kernel(const HeadArgs a) {
             const bool is_q = r < a.Hq, is_v = r >= a.Hq + a.H;
             float x[8];
             widen8<DT>(raw[i], x);
-            if (a.qw || a.kw) {
-                float ss = 0.f;
+            if (norm) {
+                uint64_t s2 = ph_mul2(ph_pack(x[0], x[1]), ph_pack(x[0], x[1]));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+                for (int j = 2; j < 8; j += 2) s2 = ph_fma2(ph_pack(x[j], x[j + 1]), ph_pack(x[j], x[j + 1]), s2);
+                float ss, s1;
+                ph_unpack(s2, ss, s1);
+                ss += s1;
 #pragma unroll
                 for (int o = TPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 if (!is_v && (is_q ? a.qw : a.kw)) {
-                    const float inv = rsqrtf(ss / (float)a.D + a.eps);
+                    const float inv = rsqrtf(fmaf(ss, inv_d, a.eps));
+                    const uint64_t inv2 = ph_pack(inv, inv);
+                    const float* w = s_w[!is_q] + 8 * c;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * (is_q ? qw[j] : kw[j]);
+                    for (int j = 0; j < 8; j += 4) {
+                        const float4 w4 = *reinterpret_cast<const float4*>(w + j);
+                        ph_unpack(ph_mul2(ph_mul2(ph_pack(x[j], x[j + 1]), inv2), ph_pack(w4.x, w4.y)), x[j], x[j + 1]);
+                        ph_unpack(ph_mul2(ph_mul2(ph_pack(x[j + 2], x[j + 3]), inv2), ph_pack(w4.z, w4.w)), x[j + 2], x[j + 3]);
+                    }
                 }
             }
             if (a.table) {
@@ -153,27 +195,27 @@ __global__ void __launch_bounds__(PH_THREADS) heads_kernel(const HeadArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
                 } else {
-                    const bool swap = r8 & 1;   // partners sit in the other sub-chunk
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         y[j] = __shfl_sync(0xffffffffu, swap ? x[4 + j] : x[j], src[0]);
                         y[4 + j] = __shfl_sync(0xffffffffu, swap ? x[j] : x[4 + j], src[1]);
                     }
                 }
-                if (!is_v) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (turn[j >> 2]) x[j] = fmaf(x[j], cs[j], y[j] * sn[j]);
-                }
+                for (int s = 0; s < 2; ++s)
+                    if (turn[s] && !is_v) {
+#pragma unroll
+                        for (int j = 4 * s; j < 4 * s + 4; j += 2)
+                            ph_unpack(ph_fma2(ph_pack(x[j], x[j + 1]), cs[j / 2], ph_mul2(ph_pack(y[j], y[j + 1]), sn[j / 2])),
+                                      x[j], x[j + 1]);
+                    }
             }
-            float scale = 0.f;
+            float m = 0.f;
             if (MODE == PH_PAGES8) {
-                float m = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(x[j]));
 #pragma unroll
                 for (int o = TPR / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                scale = __fdiv_rn(m, 127.f);
             }
             if (r >= rows || !on) continue;    // no shuffle follows in this row
             if (is_q) {
@@ -190,15 +232,28 @@ __global__ void __launch_bounds__(PH_THREADS) heads_kernel(const HeadArgs a) {
                 if (MODE == PH_PAGES) {
                     store8<DT>(pages, row * a.D + 8 * c, x);
                 } else {
-                    uint2 u;
-                    int8_t* e = reinterpret_cast<int8_t*>(&u);
+                    const float scale = __fdiv_rn(m, 127.f);
+                    // x / scale as a product (a code differs from the quotient's only where that is within 2^-16 of a
+                    // tie); a scale whose reciprocal leaves fp32's range divides; a row that is not finite: codes
+                    // of 0 and a scale that is not finite read back as NaN
+                    const bool plain = scale > 1e-37f && scale < INFINITY;
+                    const float back = plain ? __fdiv_rn(1.f, scale) : 0.f;
+                    uint32_t u[2];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        // a row that is not finite: codes of 0 and a scale that is not finite read back as NaN
-                        const float f = scale > 0.f && scale < INFINITY ? __fdiv_rn(x[j], scale) : 0.f;
-                        e[j] = (int8_t)__float2int_rn(fminf(fmaxf(f, -127.f), 127.f));
+                    for (int j = 0; j < 8; j += 4) {
+                        int e[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float f = x[j + k] * back;
+                            if (!plain)   // (a subnormal scale is itself rounded: the quotient may pass 127)
+                                f = scale > 0.f && scale < INFINITY ? fminf(fmaxf(__fdiv_rn(x[j + k], scale), -127.f), 127.f) : 0.f;
+                            // |f| <= 127 but for the rounding of back, so the nearest integer is in range; with 1.5 2^23
+                            // added it stands in the low bits
+                            e[k] = __float_as_int(__fadd_rn(f, 12582912.f));
+                        }
+                        u[j / 4] = __byte_perm(__byte_perm(e[0], e[1], 0x0040), __byte_perm(e[2], e[3], 0x0040), 0x5410);
                     }
-                    *reinterpret_cast<uint2*>(reinterpret_cast<int8_t*>(pages) + row * a.D + 8 * c) = u;
+                    *reinterpret_cast<uint2*>(reinterpret_cast<int8_t*>(pages) + row * a.D + 8 * c) = make_uint2(u[0], u[1]);
                     if (c == 0) (is_v ? a.v_scale : a.k_scale)[row] = scale;
                 }
             }
