@@ -116,7 +116,31 @@ struct PagedPlan {
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-static PagedPlan paged_plan(int dt, int B, int H, int G, int total_q, int max_q, int max_kv) {
+// Splits of the key axis that a simple model of the time finds best: a block
+// costs `start` us and `key_us` per 128 keys; the lengths are equal (one
+// sequence, hardly changed by causality: whole rounds of blocks count) or
+// uneven (half of the longest on average, dealt out longest first: the sum over
+// the slots, or the longest block); the merge writes and reads every split's
+// fp32 rows once.  Measured for the tcgen05 kernel: four 512-token chunks over
+// up to 16384 INT8 keys 264 / 289 / 275 us with 2 / 3 / 4 splits, 17 sequences of up
+// to 4000 keys 119 / 161 us with 1 / 2, a 2048-token prompt 43 / 86 us with 1 / 3.
+static int choose_splits(int64_t blocks, int slots, int max_kv, bool equal, double start, double key_us, double merge_bytes,
+                         int least_keys) {
+    const double steps = (double)ceil_div(max_kv, 128);
+    const int64_t most = ceil_div(max_kv, least_keys);
+    int best = 1;
+    double best_t = 1e30;
+    for (int n = 1; n <= most && n <= 1024; ++n) {
+        const double one = start + key_us * steps / n;
+        double t = equal ? (double)ceil_div(blocks * n, slots) * one
+                         : fmax(one, (double)blocks * (start * n + key_us * steps / 2) / slots);
+        if (n > 1) t += 3.0 + 2.0 * n * merge_bytes / 4e6;
+        if (t < best_t * 0.98) { best_t = t; best = n; }   // more splits only for a clear gain
+    }
+    return best;
+}
+
+static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int max_q, int max_kv) {
     PagedPlan p;
     const bool few = (int64_t)max_q * G <= 16;
     p.kernel = dt == QV_F32 ? PK_SIMT : few ? PK_FEW : PK_TC;
@@ -127,17 +151,19 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int total_q, int max_q,
     p.tiles = total_q * unit / per + (B < total_q ? B : total_q);
     const int64_t by_len = (int64_t)B * ceil_div(max_q * unit, per);
     if (p.tiles > by_len) p.tiles = by_len;
-    // splits of the keys: enough blocks for the SMs.  One sequence: one round of
-    // equal blocks; several, whose lengths differ: rounds enough to even out
-    int64_t blocks = p.tiles * H, want, least;
-    if (p.kernel == PK_FEW) { blocks = (int64_t)B * H; want = (B > 1 ? 8 : 1) * 2 * 148; least = B > 1 ? 1024 : 512; }
-    else if (p.kernel == PK_TC) { want = 4 * 148; least = 512; }
-    else { want = 2 * 148; least = 256; }
-    int64_t n = blocks > 0 ? ceil_div(want, blocks) : 1;
-    const int64_t most = ceil_div(max_kv, least);
-    if (n > most) n = most;
-    // what does not fill its last round fills one round fewer
-    if (B == 1 && n > 1 && blocks * n > want) --n;
+    const bool equal = B == 1 && max_kv >= 2 * max_q;
+    const double merge = 4.0 * total_q * G * H * D;
+    int n;
+    if (p.kernel == PK_FEW) {
+        // one sequence: one round of two blocks per SM; several, whose lengths
+        // differ: rounds enough to even out
+        const int64_t blocks = (int64_t)B * H, want = (B > 1 ? 8 : 1) * 2 * 148, most = ceil_div(max_kv, B > 1 ? 1024 : 512);
+        n = (int)(ceil_div(want, blocks) < most ? ceil_div(want, blocks) : most);
+    } else if (p.kernel == PK_TC) {
+        n = choose_splits(p.tiles * H, 148, max_kv, equal, 5.0, 2.0 * D / 128, merge, 512);
+    } else {
+        n = choose_splits(p.tiles * H, 2 * 148, max_kv, equal, 5.0, p.rows == 64 ? 13.0 * D / 128 : 4.0, merge, 256);
+    }
     if (n < 1) n = 1;
     p.chunk = (int)(ceil_div(ceil_div(max_kv, n), 128) * 128);
     if (p.chunk < 128) p.chunk = 128;
@@ -196,7 +222,7 @@ extern "C" size_t qv_paged_attention_workspace_bytes(const qv_paged_cache* c, in
                                                      int32_t total_q, int32_t max_q, int32_t max_kv) {
     if (paged_cache_check(c) != QV_OK || !attn_dims_ok(c, batch, q_heads, total_q, max_q, max_kv)) return 0;
     if (batch == 0 || total_q == 0 || max_q == 0) return 0;
-    return paged_ws_bytes(paged_plan(c->dtype, batch, c->kv_heads, q_heads / c->kv_heads, total_q, max_q, max_kv), total_q,
+    return paged_ws_bytes(paged_plan(c->dtype, batch, c->kv_heads, q_heads / c->kv_heads, c->head_dim, total_q, max_q, max_kv), total_q,
                           q_heads, c->head_dim);
 }
 
@@ -217,7 +243,7 @@ extern "C" int qv_paged_attention(const qv_paged_cache* c, int32_t batch, int32_
         q_stride < (int64_t)q_heads * c->head_dim)
         return QV_EINVAL;
     const int G = q_heads / c->kv_heads;
-    const PagedPlan p = paged_plan(c->dtype, batch, c->kv_heads, G, total_q, max_q, max_kv);
+    const PagedPlan p = paged_plan(c->dtype, batch, c->kv_heads, G, c->head_dim, total_q, max_q, max_kv);
     if (p.tiles * c->kv_heads > 0x7fffffff) return QV_EINVAL;
     const size_t need = paged_ws_bytes(p, total_q, q_heads, c->head_dim);
     if (need > workspace_bytes) return QV_ESPACE;
