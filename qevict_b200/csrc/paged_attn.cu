@@ -155,10 +155,14 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int
     const double merge = 4.0 * total_q * G * H * D;
     int n;
     if (p.kernel == PK_FEW) {
-        // one sequence: one round of two blocks per SM; several, whose lengths
-        // differ: rounds enough to even out
-        const int64_t blocks = (int64_t)B * H, want = (B > 1 ? 8 : 1) * 2 * 148, most = ceil_div(max_kv, B > 1 ? 1024 : 512);
-        n = (int)(ceil_div(want, blocks) < most ? ceil_div(want, blocks) : most);
+        // blocks that fit at once: three per SM (two with more than eight rows).  Few
+        // sequences: one round of blocks (a quarter more where lengths differ), of at
+        // least 128 keys; many: rounds enough to even out, of at least 1024
+        const int64_t per_round = ((int64_t)max_q * G <= 8 ? 3 : 2) * 148, blocks = (int64_t)B * H;
+        int64_t most;
+        if (2 * blocks <= per_round) { n = (int)((B > 1 ? per_round * 5 / 4 : per_round) / blocks); most = ceil_div(max_kv, 128); }
+        else { n = (int)ceil_div(6 * per_round, blocks); most = ceil_div(max_kv, 1024); }
+        if (n > most) n = (int)most;
     } else if (p.kernel == PK_TC) {
         n = choose_splits(p.tiles * H, 148, max_kv, equal, 5.0, 2.0 * D / 128, merge, 512);
     } else {

@@ -8,8 +8,9 @@
 // keys; each of its four warps walks its own tiles of 16 or 32 keys through a
 // ring of its own in shared memory (TMA, one elected lane, one mbarrier per
 // stage), so that no barrier couples the warps until their states join at the
-// end.  Two blocks share an SM: one's start and end hide behind the other's
-// loads.
+// end.  Three blocks share an SM (two with more than eight rows): one's start and
+// end hide behind the others' loads.  64 sequences over up to 8192 INT8 tokens:
+// 108 us, 122 us with two blocks and rings of three stages instead of two.
 //
 // Per tile, with warp-level MMA (m16n8k16) and the cached rows as the M side, so
 // that up to 8 query rows cost one n-tile and no padding of the conversions:
@@ -38,7 +39,6 @@ namespace qv {
 
 constexpr int PF_WARPS = 4;
 constexpr int PF_THREADS = 32 * PF_WARPS;
-constexpr int PF_PIECE = 16;              // keys per TMA box: never across a page
 constexpr float PF_BELOW = 7.f, PF_LAZY = 15.f;
 constexpr float PF_MIN_SCALE = 7.8886090522101181e-31f;   // 2^-100: a smaller value scale counts as this
 
@@ -46,7 +46,7 @@ template <int D, bool Q8> struct PfCfg {
     static constexpr int KT = D == 128 && !Q8 ? 16 : 32;            // keys per tile
     static constexpr int ROWB = Q8 ? D : 2 * D;                     // bytes of a cached row
     static constexpr int HALF = KT * ROWB, STAGE = 2 * HALF;        // K, V
-    static constexpr int STAGES = 24 * 1024 / STAGE;                // 96 KB per block in all
+    static constexpr int STAGES = 16 * 1024 / STAGE;                // 64 KB per block in all
     static constexpr int STATE = 16 * (D + 4) * 4;                  // a warp's output at the end, in its ring's place
     static constexpr size_t SMEM = 1024 + (size_t)PF_WARPS * STAGES * (STAGE + (Q8 ? 2 * KT * 4 : 0));
     static_assert(STATE <= STAGES * STAGE, "state");
@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t pf_codes(uint32_t u, uint32_t v, uint32_t se
 
 // NQ: n-tiles of 8 query rows.
 template <int DT, int D, bool Q8, int NQ>
-__global__ void __launch_bounds__(PF_THREADS, 2)
+__global__ void __launch_bounds__(PF_THREADS, NQ == 1 ? 3 : 2)
 paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const PagedArgs a) {
     using C = PfCfg<D, Q8>;
     using T = typename Elt<DT>::T;
@@ -115,44 +115,57 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
     __syncthreads();
 
     // lane 0 loads: tile i of this warp holds the keys from k_begin + (warp + 4 i) KT on
+    // (a TMA box is a whole tile, or at 16-token pages 16 of its keys)
     const int mine = tiles > warp ? (tiles - warp + PF_WARPS - 1) / PF_WARPS : 0;
-    int ids[NM];
-    auto find_pages = [&](int i) {
-        const int k0 = k_begin + (warp + PF_WARPS * i) * KT;
-#pragma unroll
-        for (int p = 0; p < NM; ++p) ids[p] = i < mine && k0 + p * PF_PIECE < s.kv ? paged_page(a, b, k0 + p * PF_PIECE) : -1;
-    };
-    auto issue = [&](int i) {
-        const int st = i % C::STAGES, k0 = k_begin + (warp + PF_WARPS * i) * KT;
-        uint64_t* bar = &full[warp][st];
-        unsigned char* dst = ring + st * C::STAGE;
-        int n = 0;
-#pragma unroll
-        for (int p = 0; p < NM; ++p) n += ids[p] >= 0;
-        mbar_arrive_expect_tx(bar, n * PF_PIECE * (2 * C::ROWB + (Q8 ? 8 : 0)));
+    const int first = k_begin + warp * KT, past = first + mine * PF_WARPS * KT;
+    const int piece = min(KT, 1 << a.page_shift), page_mask = (1 << a.page_shift) - 1;
+    const int32_t* table = a.block_table + (size_t)b * a.max_pages;
+    int ids[NM], next_key = first;       // the tile to load next, its stage, and its pages
+    int next_st = 0;
+    auto find_pages = [&]() {
 #pragma unroll
         for (int p = 0; p < NM; ++p) {
-            if (ids[p] < 0) continue;
-            const int off = (k0 + p * PF_PIECE) & ((1 << a.page_shift) - 1);
-            if (Q8) {
-                tma_load_4d(dst + p * PF_PIECE * D, &mK, 0, off, h, ids[p], bar);
-                tma_load_4d(dst + C::HALF + p * PF_PIECE * D, &mV, 0, off, h, ids[p], bar);
-                const size_t row = (((size_t)ids[p] * a.H + h) << a.page_shift) + off;
-                float* sc = ring_sc + st * 2 * KT + p * PF_PIECE;
-                bulk_load(sc, a.k_scale + row, PF_PIECE * 4, bar);
-                bulk_load(sc + KT, a.v_scale + row, PF_PIECE * 4, bar);
-            } else {
-#pragma unroll
-                for (int w = 0; w < D / 64; ++w) {
-                    tma_load_4d(dst + w * KT * 128 + p * PF_PIECE * 128, &mK, 64 * w, off, h, ids[p], bar);
-                    tma_load_4d(dst + C::HALF + w * KT * 128 + p * PF_PIECE * 128, &mV, 64 * w, off, h, ids[p], bar);
+            const int key = next_key + p * piece;
+            ids[p] = -1;
+            if (next_key < past && p * piece < KT && key < s.kv) {
+                ids[p] = table[key >> a.page_shift];
+                if ((unsigned)ids[p] >= (unsigned)a.pages) {     // as paged_page
+                    if (a.err) set_err(a.err, QV_DERR_TABLE);
+                    ids[p] = 0;
                 }
             }
         }
     };
+    auto issue = [&]() {
+        uint64_t* bar = &full[warp][next_st];
+        unsigned char* dst = ring + next_st * C::STAGE;
+        const int n = NM == 2 && ids[1] >= 0 ? 2 : 1;
+        mbar_arrive_expect_tx(bar, n * piece * (2 * C::ROWB + (Q8 ? 8 : 0)));
+#pragma unroll
+        for (int p = 0; p < NM; ++p) {
+            if (p >= n) continue;
+            const int off = (next_key + p * piece) & page_mask;
+            if (Q8) {
+                tma_load_4d(dst + p * piece * D, &mK, 0, off, h, ids[p], bar);
+                tma_load_4d(dst + C::HALF + p * piece * D, &mV, 0, off, h, ids[p], bar);
+                const size_t row = ((size_t)(ids[p] * (int64_t)a.H + h) << a.page_shift) + off;
+                float* sc = ring_sc + next_st * 2 * KT + p * piece;
+                bulk_load(sc, a.k_scale + row, piece * 4, bar);
+                bulk_load(sc + KT, a.v_scale + row, piece * 4, bar);
+            } else {
+#pragma unroll
+                for (int w = 0; w < D / 64; ++w) {
+                    tma_load_4d(dst + w * KT * 128 + p * piece * 128, &mK, 64 * w, off, h, ids[p], bar);
+                    tma_load_4d(dst + C::HALF + w * KT * 128 + p * piece * 128, &mV, 64 * w, off, h, ids[p], bar);
+                }
+            }
+        }
+        next_key += PF_WARPS * KT;
+        next_st = next_st + 1 == C::STAGES ? 0 : next_st + 1;
+    };
     if (lane == 0) {
-        for (int i = 0; i < C::STAGES && i < mine; ++i) { find_pages(i); issue(i); }
-        find_pages(C::STAGES);
+        for (int i = 0; i < C::STAGES && i < mine; ++i) { find_pages(); issue(); }
+        find_pages();
     }
 
     // query fragments: lane (g, t) holds row 8 q + g; its four slots of a k-step are elements 2t, 2t + 1,
@@ -210,15 +223,15 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
         for (int d = 0; d < ND; ++d) o[q][d][0] = o[q][d][1] = o[q][d][2] = o[q][d][3] = 0.f;
     }
 
-    for (int i = 0; i < mine; ++i) {
-        const int st = i % C::STAGES, k0 = k_begin + (warp + PF_WARPS * i) * KT;
-        bool ok = mbar_wait_bounded(&full[warp][st], (i / C::STAGES) & 1);
+    int stage = 0, phase = 0;
+    for (int k0 = first; k0 < past; k0 += PF_WARPS * KT) {
+        bool ok = mbar_wait_bounded(&full[warp][stage], phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
             if (lane == 0) { s_bad = 1; if (a.err) set_err(a.err, QV_DERR_TIMEOUT); }
             break;
         }
-        unsigned char* kt = ring + st * C::STAGE;
+        unsigned char* kt = ring + stage * C::STAGE;
         unsigned char* vt = kt + C::HALF;
         const uint32_t ka = smem_u32(kt), va = smem_u32(vt);
         float x[NM][NQ][4];              // keys 16 i + g (, + 8) x rows 2t, 2t + 1
@@ -273,7 +286,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
                 const int key = k0 + 16 * i2 + g + 8 * e;
                 float ks = 1.f, lv = 0.f;
                 if constexpr (Q8) {
-                    const float* sc = ring_sc + st * 2 * KT + 16 * i2 + g + 8 * e;
+                    const float* sc = ring_sc + stage * 2 * KT + 16 * i2 + g + 8 * e;
                     ks = sc[0];
                     float vs = sc[KT];
                     vs = vs < PF_MIN_SCALE ? PF_MIN_SCALE : vs;          // also a zero row, whose codes are 0
@@ -380,10 +393,11 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
             }
         }
         __syncwarp();
-        if (lane == 0 && i + C::STAGES < mine) {
-            issue(i + C::STAGES);
-            find_pages(i + C::STAGES + 1);
+        if (lane == 0 && next_key < past) {
+            issue();
+            find_pages();
         }
+        if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
     }
     // the warps' states join
 #pragma unroll
@@ -455,9 +469,10 @@ template <int DT, int D, bool Q8> static int pf_launch(const PagedArgs& a, cudaS
     CUtensorMap mK, mV;
     const int page = 1 << a.page_shift;
     const bool few8 = a.max_q * a.G <= 8;
+    const int piece = page < C::KT ? page : C::KT;
     const CUtensorMapSwizzle sw = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-    if (!paged_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages, PF_PIECE, sw) ||
-        !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, PF_PIECE, sw))
+    if (!paged_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages, piece, sw) ||
+        !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, piece, sw))
         return QV_EINVAL;
     auto kernel = few8 ? paged_few_kernel<DT, D, Q8, 1> : paged_few_kernel<DT, D, Q8, 2>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
