@@ -2,6 +2,8 @@
 // token or tile belongs to, and the arguments of the attention kernels.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace qv {
@@ -120,6 +122,19 @@ __device__ __forceinline__ int2 paged_find_tile(const PagedArgs& a, int tile, in
         before += __shfl_sync(0xffffffffu, incl, 31);
     }
     return make_int2(-1, 0);
+}
+
+// Raise a kernel's dynamic shared-memory limit once per device (`seen`: a bit per
+// device, one word per kernel), so that later launches make no attribute call.
+template <typename K> inline cudaError_t paged_smem(K kernel, size_t bytes, std::atomic<uint64_t>* seen) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (seen->load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) seen->fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // Index of the last entry of the ascending cu[0..B] that is <= t, below B.

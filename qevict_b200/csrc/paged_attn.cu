@@ -181,25 +181,23 @@ static size_t paged_ws_bytes(const PagedPlan& p, int total_q, int Hq, int D) {
 }
 
 // ---------------------------------------------------------------- launch
-template <int DT, int D, bool Q8, int BM>
+template <int D, bool Q8, int BM>
 static int simt_launch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
     constexpr size_t bytes = paged_simt_smem<D, BM>();
-    if (bytes > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(paged_simt_kernel<DT, D, Q8, BM>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e != cudaSuccess) return set_cuda_error(e);
-    }
-    paged_simt_kernel<DT, D, Q8, BM><<<dim3((unsigned)p.tiles, a.H, p.splits), PS_THREADS, bytes, s>>>(a);
+    static std::atomic<uint64_t> seen{0};
+    const cudaError_t e = paged_smem(paged_simt_kernel<D, Q8, BM>, bytes, &seen);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    paged_simt_kernel<D, Q8, BM><<<dim3((unsigned)p.tiles, a.H, p.splits), PS_THREADS, bytes, s>>>(a);
     return check_launch();
 }
 
-template <int DT, int D, bool Q8> static int simt_dispatch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
-    return p.rows == 16 ? simt_launch<DT, D, Q8, 16>(a, p, s) : simt_launch<DT, D, Q8, 64>(a, p, s);
+template <int D, bool Q8> static int simt_dispatch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
+    return p.rows == 16 ? simt_launch<D, Q8, 16>(a, p, s) : simt_launch<D, Q8, 64>(a, p, s);
 }
 
 template <int DT, int D> static int paged_launch(const PagedArgs& a, const PagedPlan& p, bool q8, cudaStream_t s) {
     int rc;
-    if constexpr (DT == QV_F32) rc = q8 ? simt_dispatch<DT, D, true>(a, p, s) : simt_dispatch<DT, D, false>(a, p, s);
+    if constexpr (DT == QV_F32) rc = q8 ? simt_dispatch<D, true>(a, p, s) : simt_dispatch<D, false>(a, p, s);
     else if (p.kernel == PK_FEW) rc = paged_few_launch(a, DT, D, q8, s);
     else rc = paged_tc_launch(a, DT, D, q8, p.tiles, s);
     if (rc != QV_OK || p.splits == 1) return rc;
@@ -248,7 +246,7 @@ extern "C" int qv_paged_attention(const qv_paged_cache* c, int32_t batch, int32_
         return QV_EINVAL;
     const int G = q_heads / c->kv_heads;
     const PagedPlan p = paged_plan(c->dtype, batch, c->kv_heads, G, c->head_dim, total_q, max_q, max_kv);
-    if (p.tiles * c->kv_heads > 0x7fffffff) return QV_EINVAL;
+    if (p.tiles * c->kv_heads > 0x7fffffff || (int64_t)batch * c->kv_heads > 0x7fffffff) return QV_EINVAL;
     const size_t need = paged_ws_bytes(p, total_q, q_heads, c->head_dim);
     if (need > workspace_bytes) return QV_ESPACE;
     if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return QV_EINVAL;

@@ -475,7 +475,8 @@ template <int DT, int D, bool Q8> static int pf_launch(const PagedArgs& a, cudaS
         !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, piece, sw))
         return QV_EINVAL;
     auto kernel = few8 ? paged_few_kernel<DT, D, Q8, 1> : paged_few_kernel<DT, D, Q8, 2>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    static std::atomic<uint64_t> seen[2] = {{0}, {0}};
+    const cudaError_t e = paged_smem(kernel, C::SMEM, &seen[few8]);
     if (e != cudaSuccess) return set_cuda_error(e);
     kernel<<<dim3((unsigned)(a.B * a.H), a.splits), PF_THREADS, C::SMEM, s>>>(mK, mV, a);
     return check_launch();

@@ -694,8 +694,8 @@ template <int DT, int D, bool Q8> static int pt_launch(const PagedArgs& a, int64
     if (!pt_map_q(&mQ, a, DT, D) || !paged_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages, page, sw) ||
         !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, page, sw))
         return QV_EINVAL;
-    const cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<DT, D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)C::SMEM);
+    static std::atomic<uint64_t> seen{0};
+    const cudaError_t e = paged_smem(paged_tc_kernel<DT, D, Q8>, C::SMEM, &seen);
     if (e != cudaSuccess) return set_cuda_error(e);
     paged_tc_kernel<DT, D, Q8><<<dim3((unsigned)(tiles * a.H), a.splits), C::THREADS, C::SMEM, s>>>(mQ, mK, mV, a);
     return check_launch();
