@@ -126,12 +126,13 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // to 4000 keys 119 / 161 us with 1 / 2, a 2048-token prompt 43 / 86 us with 1 / 3.
 static int choose_splits(int64_t blocks, int slots, int max_kv, bool equal, double start, double key_us, double merge_bytes,
                          int least_keys) {
-    const double steps = (double)ceil_div(max_kv, 128);
-    const int64_t most = ceil_div(max_kv, least_keys);
+    const int64_t steps = ceil_div(max_kv, 128), most = ceil_div(max_kv, least_keys);
     int best = 1;
     double best_t = 1e30;
-    for (int n = 1; n <= most && n <= 1024; ++n) {
-        const double one = start + key_us * steps / n;
+    for (int64_t each = steps; each > 0; each = each > 64 ? each * 7 / 8 : each - 1) {   // steps per split
+        const int n = (int)ceil_div(steps, each);
+        if (n > most || n > 1024) break;
+        const double one = start + key_us * each;
         double t = equal ? (double)ceil_div(blocks * n, slots) * one
                          : fmax(one, (double)blocks * (start * n + key_us * steps / 2) / slots);
         if (n > 1) t += 3.0 + 2.0 * n * merge_bytes / 4e6;
@@ -144,7 +145,7 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int
     PagedPlan p;
     const bool few = (int64_t)max_q * G <= 16;
     p.kernel = dt == QV_F32 ? PK_SIMT : few ? PK_FEW : PK_TC;
-    p.rows = few ? 16 : 64;
+    p.rows = few ? 16 : (int64_t)max_q * G <= 64 ? 64 : 128;
     // tokens (times G: rows) per tile; every sequence ends in at most one partial
     // tile, and none is longer than max_q
     const int64_t unit = p.kernel == PK_TC ? 1 : G, per = p.kernel == PK_TC ? 2 * (128 / G) : p.rows;
@@ -166,7 +167,8 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int
     } else if (p.kernel == PK_TC) {
         n = choose_splits(p.tiles * H, 148, max_kv, equal, 5.0, 2.0 * D / 128, merge, 512);
     } else {
-        n = choose_splits(p.tiles * H, 2 * 148, max_kv, equal, 5.0, p.rows == 64 ? 13.0 * D / 128 : 4.0, merge, 256);
+        n = choose_splits(p.tiles * H, p.rows == 128 ? 148 : 2 * 148, max_kv, equal, 5.0, (p.rows == 16 ? 4.0 : p.rows == 64 ? 20.0 : 26.0) * D / 128,
+                          merge, 256);
     }
     if (n < 1) n = 1;
     p.chunk = (int)(ceil_div(ceil_div(max_kv, n), 128) * 128);
@@ -192,7 +194,8 @@ static int simt_launch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
 }
 
 template <int D, bool Q8> static int simt_dispatch(const PagedArgs& a, const PagedPlan& p, cudaStream_t s) {
-    return p.rows == 16 ? simt_launch<D, Q8, 16>(a, p, s) : simt_launch<D, Q8, 64>(a, p, s);
+    if (p.rows == 16) return simt_launch<D, Q8, 16>(a, p, s);
+    return p.rows == 64 ? simt_launch<D, Q8, 64>(a, p, s) : simt_launch<D, Q8, 128>(a, p, s);
 }
 
 template <int DT, int D> static int paged_launch(const PagedArgs& a, const PagedPlan& p, bool q8, cudaStream_t s) {

@@ -3,24 +3,37 @@
 //
 // A block takes BM query rows (row r of a chunk is token r / G, head r % G of
 // one KV head's group, so that the group shares every K and V row it reads)
-// and one range of keys, 64 at a time:  S = Q K^T, running maximum m and sum l
-// of exp2(S - m), O = O exp2(m_old - m) + P V.  16 x 16 threads, each with
-// BM/16 rows x 4 keys of S and BM/16 rows x D/16 columns of O in registers;
-// K, V and P tiles in shared memory, P in K's place.  Rows are padded by four
-// floats so that the 16-byte reads of eight neighbouring rows fall on
-// different banks.
+// and one range of keys, a tile at a time:  S = Q K^T, running maximum m and sum l
+// of exp2(S - m), O = O exp2(m_old - m) + P V.  16 x 16 threads, each with BM/16
+// rows of S and O in registers; K, V and P tiles in shared memory, P in K's place.
+// Rows are padded by four floats so that the 16-byte reads of eight neighbouring
+// rows fall on different banks.
+//
+// Bound by shared memory's reads: a 16-byte read takes four cycles a warp whether
+// lanes share addresses or not, so a 4 x 4 block of S per thread (64 rows) reads
+// for twice as long as it multiplies; 8 x 8 (128 rows, 128 keys, one block per SM)
+// for as long.
 #pragma once
 
 #include "paged.cuh"
 
 namespace qv {
 
-constexpr int PS_KEYS = 64;
 constexpr int PS_THREADS = 256;
 
+// Keys per tile: as many as rows, at least 64.
+constexpr int paged_simt_keys(int BM) { return BM > 64 ? BM : 64; }
+
 template <int D, int BM> constexpr size_t paged_simt_smem() {
-    return sizeof(float) * (BM + 2 * PS_KEYS) * (D + 4);
+    const int K = paged_simt_keys(BM), KP = K * (D + 4) > BM * (K + 4) ? K * (D + 4) : BM * (K + 4);   // K, then P
+    return sizeof(float) * ((BM + K) * (D + 4) + KP);
 }
+
+// 16 bytes into shared memory in the background.
+__device__ __forceinline__ void ps_copy16(float* dst, const float* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void ps_copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ uint64_t ps_pack(float lo, float hi) {
     uint64_t r;
@@ -42,12 +55,16 @@ __device__ __forceinline__ uint64_t ps_mul2(uint64_t a, uint64_t b) {
 }
 
 template <int D, bool Q8, int BM>
-__global__ void __launch_bounds__(PS_THREADS, 2) paged_simt_kernel(const PagedArgs a) {
-    constexpr int LD = D + 4, RM = BM / 16, NC = D / 64, CH = D / 8, LP = PS_KEYS + 4;
+__global__ void __launch_bounds__(PS_THREADS, BM > 64 ? 1 : 2) paged_simt_kernel(const PagedArgs a) {
+    constexpr int LD = D + 4, RM = BM / 16, NC = D / 64, CH = D / 8;
+    constexpr int KEYS = paged_simt_keys(BM), RK = KEYS / 16, LP = KEYS + 4;
+    constexpr bool AHEAD = KEYS == 64;    // tiles loaded ahead through registers
+    // QK sums: even and odd elements in pairs, where the registers allow
+    constexpr bool PAIR = RM * RK <= 16;
     extern __shared__ __align__(16) float ps_sm[];
     float* sQ = ps_sm;                    // [BM][LD]
-    float* sK = sQ + BM * LD;             // [64][LD], then P [BM][PS_KEYS + 4]
-    float* sV = sK + PS_KEYS * LD;        // [64][LD]
+    float* sK = sQ + BM * LD;             // [KEYS][LD], then P [BM][LP]
+    float* sV = sK + (KEYS * LD > BM * LP ? KEYS * LD : BM * LP);
     float* sP = sK;
     __shared__ int2 s_tile;
     const int h = blockIdx.y, sp = blockIdx.z;
@@ -94,75 +111,116 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_simt_kernel(const PagedAr
 #pragma unroll
         for (int c = 0; c < NC; ++c) o[i][c][0] = o[i][c][1] = ps_pack(0.f, 0.f);
     }
-    // A thread loads 4-element chunk tx of rows ty, ty + 16, ... (and chunk tx + 16): K of the next tile while P V
-    // runs, V while Q K^T does, both through registers.  Keys past the range give 0: their P is 0 and V must be
-    // finite.
-    constexpr int LR = PS_KEYS / 16, LC = D / 64;
-    float4 pre[LR][LC];
-    auto fetch = [&](const void* pages, const float* scales, int k0) {
+    // A thread loads 4-element chunk tx of rows ty, ty + 16, ... (and chunk tx + 16).  Tiles of 64 keys go through
+    // registers, K of the next tile while P V runs, V while Q K^T does; larger ones are copied straight to shared
+    // memory, V while Q K^T runs.  Keys past the range give 0: their P is 0 and V must be finite.
+    constexpr int LR = KEYS / 16, LC = D / 64;
+    float4 pre[AHEAD ? LR : 1][LC];
+    auto row_of = [&](int key) {
+        return (((size_t)paged_page(a, b, key) * a.H + h) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+    };
+    auto load4 = [&](const void* pages, float sc, size_t row, int col) {
+        if constexpr (Q8) {
+            const char4 e = *reinterpret_cast<const char4*>(reinterpret_cast<const int8_t*>(pages) + row * D + col);
+            return make_float4(e.x * sc, e.y * sc, e.z * sc, e.w * sc);
+        } else {
+            return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(pages) + row * D + col);
+        }
+    };
+    // start: load a tile (ahead: into registers, otherwise towards dst)
+    auto start = [&](const void* pages, const float* scales, int k0, float* dst) {
 #pragma unroll
         for (int r = 0; r < LR; ++r) {
             const int key = k0 + ty + 16 * r;
             const bool in = key < k_end;
-            const size_t row = in ? (((size_t)paged_page(a, b, key) * a.H + h) << a.page_shift) + (key & ((1 << a.page_shift) - 1)) : 0;
+            const size_t row = in ? row_of(key) : 0;
             float sc = 0.f;
             if (Q8 && in) sc = scales[row];
 #pragma unroll
             for (int c = 0; c < LC; ++c) {
-                pre[r][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (!in) continue;
-                if constexpr (Q8) {
-                    const char4 e = *reinterpret_cast<const char4*>(reinterpret_cast<const int8_t*>(pages) + row * D + 4 * tx + 64 * c);
-                    pre[r][c] = make_float4(e.x * sc, e.y * sc, e.z * sc, e.w * sc);
-                } else {
-                    pre[r][c] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(pages) + row * D + 4 * tx + 64 * c);
-                }
+                float* at = dst + (ty + 16 * r) * LD + 4 * tx + 64 * c;
+                if (AHEAD) pre[AHEAD ? r : 0][c] = in ? load4(pages, sc, row, 4 * tx + 64 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                else if (!Q8 && in) ps_copy16(at, reinterpret_cast<const float*>(pages) + row * D + 4 * tx + 64 * c);
+                else *reinterpret_cast<float4*>(at) = in ? load4(pages, sc, row, 4 * tx + 64 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
     };
-    auto put = [&](float* dst) {
+    // finish: its elements are in dst (this thread's; a barrier follows)
+    auto finish = [&](float* dst) {
+        if constexpr (AHEAD) {
 #pragma unroll
-        for (int r = 0; r < LR; ++r)
+            for (int r = 0; r < LR; ++r)
 #pragma unroll
-            for (int c = 0; c < LC; ++c) *reinterpret_cast<float4*>(dst + (ty + 16 * r) * LD + 4 * tx + 64 * c) = pre[r][c];
+                for (int c = 0; c < LC; ++c) *reinterpret_cast<float4*>(dst + (ty + 16 * r) * LD + 4 * tx + 64 * c) = pre[r][c];
+        } else {
+            ps_copies_done();
+        }
     };
 
-    if (k_begin < k_end) fetch(a.k, a.k_scale, k_begin);
-    for (int k0 = k_begin; k0 < k_end; k0 += PS_KEYS) {
+    if (AHEAD && k_begin < k_end) start(a.k, a.k_scale, k_begin, sK);
+    for (int k0 = k_begin; k0 < k_end; k0 += KEYS) {
         __syncthreads();                  // the last tile's P and V have been read
-        put(sK);
+        if (!AHEAD) start(a.k, a.k_scale, k0, sK);
+        finish(sK);
         __syncthreads();
-        fetch(a.v, a.v_scale, k0);
-        uint64_t acc2[RM][4];             // even and odd elements' sums
-#pragma unroll
-        for (int i = 0; i < RM; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc2[i][j] = ps_pack(0.f, 0.f);
-#pragma unroll 4
-        for (int d = 0; d < D; d += 4) {
-            ulonglong2 q4[RM], k4[4];
-#pragma unroll
-            for (int i = 0; i < RM; ++i) q4[i] = *reinterpret_cast<const ulonglong2*>(sQ + (ty * RM + i) * LD + d);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) k4[j] = *reinterpret_cast<const ulonglong2*>(sK + (tx + 16 * j) * LD + d);
+        start(a.v, a.v_scale, k0, sV);
+        float acc[RM][RK];
+        if constexpr (PAIR) {
+            uint64_t acc2[RM][RK];
 #pragma unroll
             for (int i = 0; i < RM; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc2[i][j] = ps_fma2(q4[i].y, k4[j].y, ps_fma2(q4[i].x, k4[j].x, acc2[i][j]));
+                for (int j = 0; j < RK; ++j) acc2[i][j] = ps_pack(0.f, 0.f);
+#pragma unroll 4
+            for (int d = 0; d < D; d += 4) {
+                ulonglong2 q4[RM], k4[RK];
+#pragma unroll
+                for (int i = 0; i < RM; ++i) q4[i] = *reinterpret_cast<const ulonglong2*>(sQ + (ty * RM + i) * LD + d);
+#pragma unroll
+                for (int j = 0; j < RK; ++j) k4[j] = *reinterpret_cast<const ulonglong2*>(sK + (tx + 16 * j) * LD + d);
+#pragma unroll
+                for (int i = 0; i < RM; ++i)
+#pragma unroll
+                    for (int j = 0; j < RK; ++j)
+                        acc2[i][j] = ps_fma2(q4[i].y, k4[j].y, ps_fma2(q4[i].x, k4[j].x, acc2[i][j]));
+            }
+#pragma unroll
+            for (int i = 0; i < RM; ++i)
+#pragma unroll
+                for (int j = 0; j < RK; ++j) {
+                    float e, f;
+                    ps_unpack(acc2[i][j], e, f);
+                    acc[i][j] = e + f;
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < RM; ++i)
+#pragma unroll
+                for (int j = 0; j < RK; ++j) acc[i][j] = 0.f;
+            // (two elements at a time: the next ones' reads fit beside the sums)
+#pragma unroll 8
+            for (int d = 0; d < D; d += 2) {
+                float2 q2[RM], k2[RK];
+#pragma unroll
+                for (int i = 0; i < RM; ++i) q2[i] = *reinterpret_cast<const float2*>(sQ + (ty * RM + i) * LD + d);
+#pragma unroll
+                for (int j = 0; j < RK; ++j) k2[j] = *reinterpret_cast<const float2*>(sK + (tx + 16 * j) * LD + d);
+#pragma unroll
+                for (int i = 0; i < RM; ++i)
+#pragma unroll
+                    for (int j = 0; j < RK; ++j) acc[i][j] = fmaf(q2[i].y, k2[j].y, fmaf(q2[i].x, k2[j].x, acc[i][j]));
+            }
         }
         __syncthreads();                  // K has been read: P takes its place
-        put(sV);
-        if (k0 + PS_KEYS < k_end) fetch(a.k, a.k_scale, k0 + PS_KEYS);
+        finish(sV);
+        if (AHEAD && k0 + KEYS < k_end) start(a.k, a.k_scale, k0 + KEYS, sK);
 #pragma unroll
         for (int i = 0; i < RM; ++i) {
-            float acc[4], mx = m[i];
+            float mx = m[i];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float e, f;
-                ps_unpack(acc2[i][j], e, f);
-                acc[j] = k0 + tx + 16 * j < limit[i] ? (e + f) * a.scale_log2 : -INFINITY;
-                mx = fmaxf(mx, acc[j]);
+            for (int j = 0; j < RK; ++j) {
+                acc[i][j] = k0 + tx + 16 * j < limit[i] ? acc[i][j] * a.scale_log2 : -INFINITY;
+                mx = fmaxf(mx, acc[i][j]);
             }
 #pragma unroll
             for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
@@ -175,15 +233,15 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_simt_kernel(const PagedAr
 #pragma unroll
                 for (int j = 0; j < 2; ++j) o[i][c][j] = ps_mul2(o[i][c][j], ps_pack(f, f));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float p = exp2f(acc[j] - base);
+            for (int j = 0; j < RK; ++j) {
+                const float p = exp2f(acc[i][j] - base);
                 l[i] += p;
                 sP[(ty * RM + i) * LP + tx + 16 * j] = p;
             }
         }
         __syncthreads();
 #pragma unroll 2
-        for (int k = 0; k < PS_KEYS; k += 4) {
+        for (int k = 0; k < KEYS; k += 4) {
             float4 p4[RM];
 #pragma unroll
             for (int i = 0; i < RM; ++i) p4[i] = *reinterpret_cast<const float4*>(sP + (ty * RM + i) * LP + k);
