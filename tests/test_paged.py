@@ -247,6 +247,11 @@ def test_native_refuses_bad_arguments():
                 dict(cache=ctypes.byref(cache_desc(head_dim=96)))):
         assert attn(**bad) == N.QV_EINVAL, bad
     assert attn(batch=0) == attn(total=0) == attn(mq=0) == N.QV_OK
+    for scale in (0.0, -0.125, math.inf, math.nan):
+        assert L.qv_paged_attention(c, 1, 4, FAKE, 2, FAKE, FAKE, 1, 1, 32, FAKE, 256, scale, 1, FAKE, None, 0,
+                                    None) == N.QV_EINVAL
+    assert L.qv_paged_gather(ctypes.byref(cache_desc(bits=8, k_scale=FAKE, v_scale=FAKE + 4)), 1, FAKE, 1, FAKE, FAKE,
+                             1, FAKE, FAKE, None) == N.QV_EINVAL
     # a call that needs a workspace and gets none, or too little
     need = L.qv_paged_attention_workspace_bytes(c, 1, 4, 1, 1, 32768)
     assert need > 0
@@ -443,6 +448,9 @@ SHAPES = [   # q_lens, kv_lens, Hq, H, D, page
     ([5, 64], [0, 20], 8, 1, 64, 16),                                  # more new tokens than cached: rows that see nothing
     ([300, 200], [300, 1999], 3, 1, 128, 64),
     ([513], [640], 16, 8, 128, 128),
+    ([9, 70], [200, 1500], 16, 1, 128, 32),                            # groups that do not divide a tile's rows
+    ([33, 2], [33, 700], 14, 2, 64, 16),
+    ([60], [260], 11, 1, 128, 64),
 ]
 
 
@@ -469,6 +477,102 @@ def test_attention_large_and_growing_logits(q_lens, kv_lens, dt, q8):
     check_attention(g, q_lens, kv_lens, 8, 2, 64, 32, dt, q8, std=3e-3)
     if dt != FP16:
         check_attention(g, q_lens, kv_lens, 8, 2, 64, 32, dt, q8, std=1e4, qstd=1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,q8", [(BF16, False), (FP16, False), (FP32, False), (BF16, True), (FP16, True), (FP32, True)])
+@pytest.mark.parametrize("n", [1, 150])
+def test_attention_rising_and_falling_logits(n, dt, q8):
+    """Logits that climb by several hundred along the keys, so that every tile's maximum is far above the last
+    one's, and the same keys falling."""
+    L, D, page = 1200, 128, 64
+    g = gen(17)
+    pool = Pool(g, [L, L], 1, D, page, dt, q8)
+    c = pool.cache
+    u = torch.nn.functional.normalize(rand(g, D), dim=-1)
+    for b in range(2):
+        pos = torch.arange(L, device=DEV)
+        size = (pos if b == 0 else L - 1 - pos).float() / L * 40
+        rows = (size[:, None, None] * u + 0.05 * rand(g, L, 1, D))
+        sl = c.slots(pool.bt, torch.full_like(pos, b), pos)
+        if q8:
+            s = rows.abs().amax(-1) / 127
+            code = (rows / s[..., None]).round()
+            c.k_pages[sl // page, :, sl % page], c.k_scale[sl // page, :, sl % page] = code.to(torch.int8), s
+            pool.ks[b] = code.double() * s.double()[..., None]
+        else:
+            c.k_pages[sl // page, :, sl % page] = rows.to(dt)
+            pool.ks[b] = rows.to(dt).double()
+    q = (u * 120 + 0.05 * rand(g, 2 * n, 4, D)).to(dt)      # logits up to 40 * 120 / sqrt(128) = 424
+    out = c.attend(q, pool.bt, pool.lens, cu([n, n]), max_q=n)
+    assert c.read_error() == 0
+    for b in range(2):
+        o, mag, big = ref_attention(q[b * n:(b + 1) * n], pool.ks[b], pool.vs[b])
+        bound = attention_bound(o, mag, big, L, D, dt, float(pool.vs[b].abs().max()))
+        assert bool(((out[b * n:(b + 1) * n].double() - o).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("n", [1, 150])
+def test_attention_int8_zero_and_uneven_rows(n, dt):
+    """INT8 rows of zeros (a scale of 0) in K and in V, and value scales over ten orders of magnitude."""
+    L, D, page = 400, 64, 32
+    g = gen(19)
+    pool = Pool(g, [L], 1, D, page, dt, True)
+    c = pool.cache
+    pos = torch.arange(L, device=DEV)
+    sl = c.slots(pool.bt, torch.zeros_like(pos), pos)
+    pg, off = sl // page, sl % page
+    for x, sc, keep, every in ((c.k_pages, c.k_scale, pool.ks, 7), (c.v_pages, c.v_scale, pool.vs, 5)):
+        zero = pos % every == 3
+        factor = torch.ones(L, device=DEV) if x is c.k_pages else 10.0 ** (-10 * torch.rand(L, generator=g, device=DEV))
+        x[pg[zero], :, off[zero]] = 0
+        s = torch.where(zero, 0.0, sc[pg, 0, off] * factor)
+        sc[pg, 0, off] = s
+        keep[0] = x[pg, :, off].double() * s.double()[:, None, None]
+    q = rand(g, n, 4, D).to(dt)
+    out = c.attend(q, pool.bt, pool.lens, cu([n]), max_q=n)
+    o, mag, big = ref_attention(q, pool.ks[0], pool.vs[0])
+    # P carries the value scale: what rounds to 0 in fp16 is half a step of 2^-24 of the largest P times its scale
+    bound = attention_bound(o, mag, big, L, D, dt, float(pool.vs[0].abs().max()))
+    assert bool(((out.double() - o).abs() <= bound).all())
+    # every value row zero: zero, whatever the logits
+    c.v_scale[pg, 0, off] = 0
+    c.v_pages[pg, :, off] = 0
+    assert bool((c.attend(q, pool.bt, pool.lens, cu([n]), max_q=n) == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("n", [1, 150])
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+def test_attention_rows_that_are_not_finite(n, dt, q8):
+    """A NaN key shows in every row that sees it, a NaN query row in itself alone; other sequences and heads keep
+    their bits."""
+    g = gen(23)
+    H, G, D, page, L = 2, 4, 128, 64, 300
+    pool = Pool(g, [L, L], H, D, page, dt, q8)
+    c = pool.cache
+    q = rand(g, 2 * n, H * G, D).to(dt)
+    kw = dict(max_q=n, max_kv=L)
+    want = c.attend(q, pool.bt, pool.lens, cu([n, n]), **kw)
+    bad = q.clone()
+    bad[n, 1, 5] = math.nan
+    got = c.attend(bad, pool.bt, pool.lens, cu([n, n]), **kw)
+    assert bool(got[n, 1].isnan().all())
+    keep = torch.ones(2 * n, H * G, dtype=torch.bool, device=DEV)
+    keep[n, 1] = False
+    assert torch.equal(got[keep], want[keep])
+    # the first key of sequence 1, head 0
+    page0 = int(pool.bt[1, 0])
+    if q8:
+        c.k_scale[page0, 0, 0] = math.nan
+    else:
+        c.k_pages[page0, 0, 0, 3] = math.nan
+    got = c.attend(q, pool.bt, pool.lens, cu([n, n]), **kw)
+    assert bool(got[n:, :G].isnan().all())
+    assert torch.equal(got[:n], want[:n]) and torch.equal(got[n:, G:], want[n:, G:])
 
 
 @pytest.mark.gpu
@@ -513,7 +617,8 @@ def test_attention_refusals():
     for bad in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q.cpu()), dict(cu_q=cu([3]).long()),
                 dict(cu_q=cu([3])[:1]), dict(kv_lens=pool.lens.repeat(2)), dict(block_table=pool.bt.long()),
                 dict(block_table=pool.bt[0]), dict(max_kv=33), dict(max_kv=-1), dict(max_q=-1),
-                dict(out=torch.empty(3, 4, 32, dtype=BF16, device=DEV)), dict(q=q.transpose(0, 1))):
+                dict(out=torch.empty(3, 4, 32, dtype=BF16, device=DEV)), dict(q=q.transpose(0, 1)), dict(scale=0.0),
+                dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan)):
         with pytest.raises(N.QevictError):
             pool.cache.attend(**{**ok, **bad})
     small = paged.PagedKVCache(2, 2, 96, 16, BF16)
