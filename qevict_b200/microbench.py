@@ -18,6 +18,9 @@ INT8 Q-cache tokens, 1000 steps.
         (Llama-2-7B MHA layer, fp16, 16384-token prompts, planted attention
         spikes that force promotions and demotions every cycle; under torchrun
         the batch is split over the ranks)
+    python -m qevict_b200.microbench --paged 8192 [--batch 64] [--chunk 1] [--bits 16] [--steps 50]
+        (one layer over a paged full-context cache: rotate + write the new
+        tokens, then attention over the pages)
 """
 
 import argparse
@@ -131,6 +134,59 @@ def run_prefill(S=8192, batch=1, steps=5, quiet=False, dtype=torch.bfloat16):
     ms = a.elapsed_time(b) / steps
     flops = 2.0 * S * S * D * Hq * batch
     res = {"prefill_tokens": S, "batch": batch, "ms_per_layer": ms, "tflops_causal": flops / (ms * 1e-3) / 1e12}
+    if not quiet:
+        print(json.dumps(res))
+    return res
+
+
+def run_paged(context=8192, batch=64, chunk=1, bits=16, steps=50, warmup=5, page=64, quiet=False, dtype=torch.bfloat16):
+    """One layer's step over a paged full-context cache at the Llama-3-8B layer
+    shape: `chunk` new tokens of each of `batch` sequences with `context` cached
+    tokens (the new ones included) are rotated and written (paged_append), then
+    attend to their sequences' pages (paged_attention).  Pages lie in random
+    order; L2 is flushed before every step.  Reports us per step of both parts,
+    the attention's GB/s of cached rows and its causal TFLOP/s."""
+    from .paged import PagedKVCache, rope_table
+    g = torch.Generator(device="cuda")
+    g.manual_seed(0)
+    Hq, per = H * G, (context + page - 1) // page
+    cache = PagedKVCache(batch * per, H, D, page, dtype, bits=bits if bits == 8 else None)
+    for x in (cache.k_pages, cache.v_pages):
+        x.copy_(torch.randint(-127, 128, x.shape, generator=g, device="cuda", dtype=torch.int8) if bits == 8
+                else torch.randn(x.shape, generator=g, device="cuda", dtype=dtype))
+    if bits == 8:
+        cache.k_scale.fill_(1 / 64)
+        cache.v_scale.fill_(1 / 64)
+    block = torch.randperm(batch * per, generator=g, device="cuda").to(torch.int32).view(batch, per)
+    T = batch * chunk
+    qkv = torch.randn(T, (Hq + 2 * H) * D, generator=g, device="cuda").to(dtype)
+    q, k, v = (x.view(T, -1, D) for x in qkv.split([Hq * D, H * D, H * D], 1))
+    seq = torch.arange(batch, device="cuda").repeat_interleave(chunk)
+    pos = (torch.arange(T, device="cuda") % chunk) + (context - chunk)
+    slots, positions = cache.slots(block, seq, pos), pos.int()
+    lens = torch.full((batch,), context, dtype=torch.int32, device="cuda")
+    cu_q = torch.arange(0, T + 1, chunk, dtype=torch.int32, device="cuda")
+    table = rope_table(context, D, 500000.0)
+    out = torch.empty(T, Hq, D, dtype=dtype, device="cuda")
+    flush = torch.empty(64 * 1024 * 1024, dtype=torch.float32, device="cuda")
+    evs = []
+    for _ in range(warmup + steps):
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+        flush.zero_()
+        torch.cuda._sleep(200000)
+        ev[0].record()
+        qr = cache.append(q, k, v, slots, positions, table)
+        ev[1].record()
+        cache.attend(qr, block, lens, cu_q, max_q=chunk, max_kv=context, out=out)
+        ev[2].record()
+        evs.append(ev)
+    torch.cuda.synchronize()
+    app, att = (sorted(e[i].elapsed_time(e[i + 1]) * 1e3 for e in evs[warmup:])[steps // 2] for i in range(2))
+    row = D * cache.k_pages.element_size() + (4 if bits == 8 else 0)
+    pairs = batch * (chunk * context - chunk * (chunk - 1) / 2)
+    res = {"context": context, "batch": batch, "chunk": chunk, "bits": bits, "append_us": app, "attention_us": att,
+           "attention_GBps": 2 * batch * context * H * row / att / 1e3, "attention_tflops": 4 * D * Hq * pairs / att / 1e6,
+           "error_word": cache.read_error()}
     if not quiet:
         print(json.dumps(res))
     return res
@@ -263,7 +319,13 @@ def main():
     ap.add_argument("--prefill", type=int, default=0, help="time one layer's prefill lane at this prompt length")
     ap.add_argument("--mha-spikes", action="store_true", help="the batch-sharded MHA workload with planted spikes")
     ap.add_argument("--nofold", action="store_true", help="time the attention without its vote-ledger fold")
+    ap.add_argument("--paged", type=int, default=0, help="time a step over a paged cache of this many tokens per sequence")
+    ap.add_argument("--chunk", type=int, default=1, help="new tokens per sequence of --paged")
+    ap.add_argument("--bits", type=int, default=16, choices=(8, 16), help="page type of --paged")
     a = ap.parse_args()
+    if a.paged:
+        run_paged(a.paged, a.batch, a.chunk, a.bits, a.steps if a.steps != 1000 else 50)
+        return
     if a.mha_spikes:
         run_mha_spikes(batch=a.batch if a.batch != 64 else 16, steps=a.steps if a.steps != 1000 else 256,
                        warmup=a.warmup)
