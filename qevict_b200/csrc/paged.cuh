@@ -124,6 +124,41 @@ __device__ __forceinline__ int2 paged_find_tile(const PagedArgs& a, int tile, in
     return make_int2(-1, 0);
 }
 
+// The same tiles in another order, for blocks that are dealt out as SMs come
+// free: sequences over half of max_kv first, then those over a quarter, an
+// eighth, and the rest, and in each sequence the last tile first (the longest
+// where causal), so that no long tile starts last.
+__device__ __forceinline__ int2 paged_find_tile_longest(const PagedArgs& a, int tile, int tile_tokens) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int cls = 0; cls < 4; ++cls) {
+        const int lo_kv = cls < 3 ? a.max_kv >> (cls + 1) : -1, hi_kv = cls > 0 ? a.max_kv >> cls : 0x7fffffff;   // (lo, hi]
+        for (int b0 = 0; b0 < a.B; b0 += 32) {
+            const int b = b0 + lane;
+            int n = 0;
+            if (b < a.B) {
+                const int kv = min(max(a.kv_lens[b], 0), a.max_kv);
+                const int lo = min(max(a.cu_q[b], 0), a.total_q), hi = min(max(a.cu_q[b + 1], 0), a.total_q);
+                if (kv > lo_kv && kv <= hi_kv) n = (min(max(hi - lo, 0), a.max_q) + tile_tokens - 1) / tile_tokens;
+            }
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, before + incl > tile);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                const int last = before + __shfl_sync(0xffffffffu, incl, src) - 1;
+                return make_int2(b0 + src, last - tile);
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    return make_int2(-1, 0);
+}
+
 // Raise a kernel's dynamic shared-memory limit once per device (`seen`: a bit per
 // device, one word per kernel), so that later launches make no attribute call.
 template <typename K> inline cudaError_t paged_smem(K kernel, size_t bytes, std::atomic<uint64_t>* seen) {

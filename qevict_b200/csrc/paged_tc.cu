@@ -164,8 +164,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
     const int QT = PT_KEYS / a.G;                        // tokens per row tile
 
     if (warp == 0) {
-        // tiles from the end: the longest rows of a causal prompt first
-        const int2 t = paged_find_tile(a, (int)(gridDim.x / a.H) - 1 - (int)(blockIdx.x / a.H), 1, 2 * QT);
+        const int2 t = paged_find_tile_longest(a, blockIdx.x / a.H, 2 * QT);
         if (lane == 0) s_tile = t;
     }
     __syncthreads();
