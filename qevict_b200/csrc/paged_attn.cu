@@ -157,11 +157,11 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int
     int n;
     if (p.kernel == PK_FEW) {
         // blocks that fit at once: three per SM (two with more than eight rows).  Few
-        // sequences: one round of blocks (a quarter more where lengths differ), of at
-        // least 128 keys; many: rounds enough to even out, of at least 1024
+        // sequences: one round of blocks (two per SM for a single one; a quarter more
+        // where lengths differ), of at least 128 keys; many: rounds enough to even out, of at least 1024
         const int64_t per_round = ((int64_t)max_q * G <= 8 ? 3 : 2) * 148, blocks = (int64_t)B * H;
         int64_t most;
-        if (2 * blocks <= per_round) { n = (int)((B > 1 ? per_round * 5 / 4 : per_round) / blocks); most = ceil_div(max_kv, 128); }
+        if (2 * blocks <= per_round) { n = (int)((B > 1 ? per_round * 5 / 4 : 2 * 148) / blocks); most = ceil_div(max_kv, 128); }
         else { n = (int)ceil_div(6 * per_round, blocks); most = ceil_div(max_kv, 1024); }
         if (n > most) n = (int)most;
     } else if (p.kernel == PK_TC) {
@@ -171,6 +171,7 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int
                           merge, 256);
     }
     if (n < 1) n = 1;
+    // a multiple of every kernel's tile times its warps
     p.chunk = (int)(ceil_div(ceil_div(max_kv, n), 128) * 128);
     if (p.chunk < 128) p.chunk = 128;
     p.splits = (int)ceil_div(max_kv, p.chunk);

@@ -90,6 +90,15 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
     __shared__ __align__(8) uint64_t full[PF_WARPS][C::STAGES];
     __shared__ float s_m[PF_WARPS][16], s_l[PF_WARPS][16];
     __shared__ int s_bad;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < PF_WARPS * C::STAGES; ++i) mbar_init(&full[0][0] + i, 1);
+        s_bad = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&mK);
+        prefetch_tensormap(&mV);
+    }
+    // launched while the kernel before still ran; what is launched on this one starts only when that has ended
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, sp = blockIdx.y;
     const PagedSeq s = paged_seq(a, b);
@@ -105,13 +114,6 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char* ring = sm + warp * C::STAGES * C::STAGE;
     float* ring_sc = reinterpret_cast<float*>(sm + PF_WARPS * C::STAGES * C::STAGE) + warp * C::STAGES * 2 * KT;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < PF_WARPS * C::STAGES; ++i) mbar_init(&full[0][0] + i, 1);
-        s_bad = 0;
-        fence_barrier_init();
-        prefetch_tensormap(&mK);
-        prefetch_tensormap(&mV);
-    }
     __syncthreads();
 
     // lane 0 loads: tile i of this warp holds the keys from k_begin + (warp + 4 i) KT on
@@ -478,8 +480,8 @@ template <int DT, int D, bool Q8> static int pf_launch(const PagedArgs& a, cudaS
     static std::atomic<uint64_t> seen[2] = {{0}, {0}};
     const cudaError_t e = paged_smem(kernel, C::SMEM, &seen[few8]);
     if (e != cudaSuccess) return set_cuda_error(e);
-    kernel<<<dim3((unsigned)(a.B * a.H), a.splits), PF_THREADS, C::SMEM, s>>>(mK, mV, a);
-    return check_launch();
+    const cudaError_t f = launch_pdl(kernel, dim3((unsigned)(a.B * a.H), a.splits), dim3(PF_THREADS), C::SMEM, s, mK, mV, a);
+    return f == cudaSuccess ? check_launch() : set_cuda_error(f);
 }
 
 template <int DT> static int pf_dispatch(const PagedArgs& a, int D, bool q8, cudaStream_t s) {
