@@ -18,8 +18,9 @@
 //
 // (Measured and left out, 8192-token prompt at D = 128, 443 us: a quarter of the
 // exponentials as a polynomial on the FMA pipe, 462 us; the two tiles' softmax
-// warps taking turns at the exponentials, 456 us.  Without any exponentials it
-// takes 443 us too: the tensor pipe at the clock that its power allows bounds it.)
+// warps taking turns at the exponentials, 456 us; two threads to a row, 494 us.
+// Without any exponentials it takes 443 us too: the tensor pipe at the clock that
+// its power allows bounds it.)
 //
 // INT8 pages: codes become exact 16-bit integers in shared memory (six extra
 // warps); the row scales ks, vs of a key stay in fp32: the logit is S c ks, and the
