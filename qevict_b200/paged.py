@@ -87,15 +87,15 @@ def _bad(name, expected, x):
 def _heads(name, x, tokens, dim, dtype, dev):
     """A [tokens, heads, head_dim] tensor whose heads are contiguous within a token (a view of a
     packed projection will do); returns (tokens, heads, token stride)."""
-    shape = x.shape
-    if (len(shape) != 3 or shape[2] != dim or (tokens is not None and shape[0] != tokens) or x.dtype is not dtype
-            or x.device != dev):
-        raise _bad(name, f"[{'tokens' if tokens is None else tokens}, heads, {dim}] {dtype} on {dev}", x)
-    st = x.stride()
-    n, h, _ = shape
-    if st[2] != 1 or (st[1] != dim and h != 1):
-        raise N.QevictError(f"{name}: a token's heads must be contiguous, got strides {st}")
-    return n, h, st[0] if n > 1 else h * dim
+    if x.ndim != 3 or x.dtype is not dtype or x.device != dev:
+        raise _bad(name, f"[tokens, heads, {dim}] {dtype} on {dev}", x)
+    n, h, d = x.shape
+    st, sh, sd = x.stride()
+    if d != dim or n != (n if tokens is None else tokens):
+        raise _bad(name, f"[{'tokens' if tokens is None else tokens}, heads, {dim}]", x)
+    if sd != 1 or (sh != dim and h != 1):
+        raise N.QevictError(f"{name}: a token's heads must be contiguous, got strides {(st, sh, sd)}")
+    return n, h, st if n > 1 else h * dim
 
 
 def _vector(name, x, shape, dtype, dev):
@@ -103,18 +103,15 @@ def _vector(name, x, shape, dtype, dev):
         raise _bad(name, f"a contiguous {shape} {dtype} tensor on {dev}", x)
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
 def _launch(dev, name, *args):
     """Call a native entry point on the current stream of `dev`."""
     fn = getattr(N.lib(), name)
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, _raw_stream(dev.index))
+    i = dev.index
+    if torch.cuda.current_device() == i:
+        rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev.index))
+            rc = fn(*args, _raw_stream(i))
     if rc:
         N.check(rc, name)
 
@@ -131,26 +128,31 @@ def _pool(k_pages, v_pages, k_scale, v_scale, dtype, err):
             or not k_pages.is_contiguous() or not v_pages.is_contiguous()):
         raise _bad("pages", "k and v contiguous [pages, kv_heads, page_size, head_dim] of one type and device; v", v_pages)
     P, H, S, D = shape
-    _pool_sizes(S, D)
-    q8 = pt is torch.int8
-    if q8:
+    if S not in _PAGE_SIZES or not 8 <= D <= 256 or D % 8:
+        _pool_sizes(S, D)
+    ks = vs = None
+    if pt is torch.int8:
         if k_scale is None or v_scale is None:
             raise N.QevictError("INT8 pages need k_scale and v_scale")
         _vector("k_scale", k_scale, (P, H, S), torch.float32, dev)
         _vector("v_scale", v_scale, (P, H, S), torch.float32, dev)
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
     elif pt is not dtype:
         raise N.QevictError(f"pages of {pt} do not go with {dtype} rows")
     elif k_scale is not None or v_scale is not None:
         raise N.QevictError("k_scale and v_scale go with INT8 pages only")
     if err is not None:
         _vector("err", err, (1,), torch.int32, dev)
-    c = N.QvPagedCache(k_pages.data_ptr(), v_pages.data_ptr(), _p(k_scale), _p(v_scale), _p(err), P, H, S, D, code,
-                       8 if q8 else 0)
+        err = err.data_ptr()
+    c = N.QvPagedCache(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, err, P, H, S, D, code, 0 if ks is None else 8)
     return c, dev, H, S, D
 
 
+_PAGE_SIZES = (16, 32, 64, 128)
+
+
 def _pool_sizes(page_size, head_dim):
-    if page_size not in (16, 32, 64, 128):
+    if page_size not in _PAGE_SIZES:
         raise N.QevictError(f"page_size {page_size} is not 16, 32, 64 or 128")
     _head_dim(head_dim)
 
@@ -161,14 +163,16 @@ def _head_dim(D):
 
 
 def _turn(tokens, dim, dtype, dev, positions, table, q_weight, k_weight):
-    """Checked (max_pos, rot_dim) of the rotation, and the norm weights."""
+    """Checked rotation and norm weights: (q_weight, k_weight, table, max_pos, rot_dim, positions), pointers or None."""
     if q_weight is not None:
         _vector("q_weight", q_weight, (dim,), dtype, dev)
+        q_weight = q_weight.data_ptr()
     if k_weight is not None:
         _vector("k_weight", k_weight, (dim,), dtype, dev)
+        k_weight = k_weight.data_ptr()
     if table is None:
-        return 0, 0
-    if table.dim() != 2 or table.dtype is not torch.float32 or not table.is_contiguous() or table.device != dev:
+        return q_weight, k_weight, None, 0, 0, None
+    if table.ndim != 2 or table.dtype is not torch.float32 or table.device != dev or not table.is_contiguous():
         raise _bad("table", f"a contiguous [max_pos, rot_dim] fp32 tensor on {dev} (rope_table)", table)
     max_pos, rot = table.shape
     if not 8 <= rot <= dim or rot % 8:
@@ -176,7 +180,7 @@ def _turn(tokens, dim, dtype, dev, positions, table, q_weight, k_weight):
     if positions is None:
         raise N.QevictError("a rotation needs positions")
     _vector("positions", positions, (tokens,), torch.int32, dev)
-    return max_pos, rot
+    return q_weight, k_weight, table.data_ptr(), max_pos, rot, positions.data_ptr()
 
 
 def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
@@ -188,22 +192,23 @@ def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=No
     interleaved.  Returns contiguous (q, k), or fills out=(q_out, k_out), which may be q and k themselves
     where those are contiguous.  A position outside the table gives NaN.  (qv_qk_norm_rope)"""
     dt, dev = q.dtype, q.device
-    if not q.is_cuda or dt not in _DTYPES or q.dim() != 3:
+    code = _DTYPES.get(dt)
+    if not q.is_cuda or code is None or q.ndim != 3:
         raise _bad("q", "a [tokens, heads, head_dim] fp32, bf16 or fp16 CUDA tensor", q)
     D = q.shape[2]
-    _head_dim(D)
+    if not 8 <= D <= 256 or D % 8:
+        _head_dim(D)
     T, Hq, qs = _heads("q", q, None, D, dt, dev)
     _, H, ks = _heads("k", k, T, D, dt, dev)
-    max_pos, rot = _turn(T, D, dt, dev, positions, table, q_weight, k_weight)
+    qw, kw, tab, max_pos, rot, pos = _turn(T, D, dt, dev, positions, table, q_weight, k_weight)
     if out is None:
-        qo = torch.empty(T, Hq, D, dtype=dt, device=dev)
-        ko = torch.empty(T, H, D, dtype=dt, device=dev)
+        qo, ko = q.new_empty(T, Hq, D), q.new_empty(T, H, D)
     else:
         qo, ko = out
         _vector("out[0]", qo, (T, Hq, D), dt, dev)
         _vector("out[1]", ko, (T, H, D), dt, dev)
-    _launch(dev, "qv_qk_norm_rope", T, Hq, H, D, _DTYPES[dt], q.data_ptr(), qs, k.data_ptr(), ks, _p(q_weight),
-            _p(k_weight), eps, _p(table), max_pos, rot, int(interleaved), _p(positions), qo.data_ptr(), ko.data_ptr())
+    _launch(dev, "qv_qk_norm_rope", T, Hq, H, D, code, q.data_ptr(), qs, k.data_ptr(), ks, qw, kw, eps, tab, max_pos,
+            rot, bool(interleaved), pos, qo.data_ptr(), ko.data_ptr())
     return qo, ko
 
 
@@ -221,22 +226,23 @@ def paged_append(q, k, v, slots, positions, table, k_pages, v_pages, *, k_scale=
     if kh != H or vh != H:
         raise N.QevictError(f"k and v must have the pool's {H} heads, got {kh} and {vh}")
     _vector("slots", slots, (T,), torch.int64, dev)
-    max_pos, rot = _turn(T, D, dt, dev, positions, table, q_weight, k_weight)
+    qw, kw, tab, max_pos, rot, pos = _turn(T, D, dt, dev, positions, table, q_weight, k_weight)
     if q_out is None:
-        q_out = torch.empty(T, Hq, D, dtype=dt, device=dev)
+        q_out = q.new_empty(T, Hq, D)
     else:
         _vector("q_out", q_out, (T, Hq, D), dt, dev)
-    _launch(dev, "qv_paged_append", ctypes.byref(c), T, Hq, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-            _p(q_weight), _p(k_weight), eps, _p(table), max_pos, rot, int(interleaved),
-            _p(positions) if table is not None else None, slots.data_ptr(), q_out.data_ptr())
+    _launch(dev, "qv_paged_append", ctypes.byref(c), T, Hq, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, qw,
+            kw, eps, tab, max_pos, rot, bool(interleaved), pos, slots.data_ptr(), q_out.data_ptr())
     return q_out
 
 
 def _tables(block_table, kv_lens, cu, dev):
-    if block_table.dim() != 2 or not block_table.shape[1]:
-        raise _bad("block_table", "[batch, max_pages]", block_table)
+    if (block_table.ndim != 2 or block_table.dtype is not torch.int32 or block_table.device != dev
+            or not block_table.is_contiguous()):
+        raise _bad("block_table", f"a contiguous [batch, max_pages] int32 tensor on {dev}", block_table)
     B, width = block_table.shape
-    _vector("block_table", block_table, (B, width), torch.int32, dev)
+    if not width:
+        raise _bad("block_table", "pages", block_table)
     _vector("kv_lens", kv_lens, (B,), torch.int32, dev)
     _vector("cumulative lengths", cu, (B + 1,), torch.int32, dev)
     return B, width
@@ -254,7 +260,7 @@ def paged_gather(k_pages, v_pages, block_table, kv_lens, cu_kv, total, *, k_scal
         raise N.QevictError("total must not be negative")
     if out is None:
         ko = torch.empty(total, H, D, dtype=dt, device=dev)
-        vo = torch.empty(total, H, D, dtype=dt, device=dev)
+        vo = torch.empty_like(ko)
     else:
         ko, vo = out
         _vector("out[0]", ko, (total, H, D), dt, dev)
@@ -288,7 +294,7 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
     if max_q < 0 or not 0 <= max_kv <= width * S:
         raise N.QevictError(f"max_q {max_q} and max_kv {max_kv} must be lengths, max_kv at most the block table's {width * S}")
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=dt, device=dev)
+        out = q.new_empty(T, Hq, D)
     else:
         _vector("out", out, (T, Hq, D), dt, dev)
     cp = ctypes.byref(c)
@@ -296,8 +302,8 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
     # from torch's allocator at each call: a captured graph gets one of its own
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     _launch(dev, "qv_paged_attention", cp, B, Hq, block_table.data_ptr(), width, kv_lens.data_ptr(), cu_q.data_ptr(),
-            T, max_q, max_kv, q.data_ptr(), qs, 1.0 / math.sqrt(D) if scale is None else scale, int(causal),
-            out.data_ptr(), _p(ws), wsb)
+            T, max_q, max_kv, q.data_ptr(), qs, D ** -0.5 if scale is None else scale, bool(causal),
+            out.data_ptr(), ws.data_ptr() if wsb else None, wsb)
     return out
 
 
