@@ -427,7 +427,7 @@ extern "C" int qv_qk_norm_rope(int32_t tokens, int32_t q_heads, int32_t kv_heads
     if (tokens == 0) return QV_OK;
     const int rc = heads_check(a, tokens, dtype);
     if (rc != QV_OK) return rc;
-    if (!k_out || !al16(k_out)) return QV_EINVAL;
+    if (!k_out || !al16(k_out) || k_out == q_out) return QV_EINVAL;
     return heads_dispatch<PH_ROWS_ONLY>(a, tokens, dtype, (cudaStream_t)stream);
 }
 
@@ -463,7 +463,7 @@ extern "C" int qv_paged_gather(const qv_paged_cache* c, int32_t batch, const int
     if (batch < 0 || total < 0) return QV_EINVAL;
     if (batch == 0 || total == 0) return QV_OK;
     if (!block_table || max_pages <= 0 || !kv_lens || !cu_kv || !k_out || !v_out) return QV_EINVAL;
-    if (!al16(k_out) || !al16(v_out)) return QV_EINVAL;
+    if (!al16(k_out) || !al16(v_out) || k_out == v_out) return QV_EINVAL;
     GatherArgs a = {c->k, c->v, c->k_scale, c->v_scale, c->err, block_table, kv_lens, cu_kv, k_out, v_out,
                     c->pages, c->kv_heads, c->head_dim, paged_shift(c->page_size), max_pages, batch, total};
     const int g = (int)(((int64_t)total + PG_TOKENS - 1) / PG_TOKENS);

@@ -93,70 +93,57 @@ __device__ __forceinline__ int paged_page(const PagedArgs& a, int b, int key) {
     return p;
 }
 
-// The sequence that holds tile `tile` when every chunk of n tokens (up to
-// max_q) is cut into ceil(n * rows_per_token / tile_rows) tiles: (sequence,
-// tile within it), or sequence -1 past the last tile.  Called by one full warp.
+// The sequence that holds a block's tile, and the tile within it (-1 past the
+// last).  Every chunk of n tokens (up to max_q) is cut into ceil(n *
+// rows_per_token / tile_rows) tiles; they are dealt out longest first, so that no
+// long one starts last: sequences over half of max_kv, over a quarter, over an
+// eighth, the rest, and in each sequence the last tile first (the longest where
+// causal).  Called by one full warp: each lane counts a run of sequences.
 __device__ __forceinline__ int2 paged_find_tile(const PagedArgs& a, int tile, int rows_per_token, int tile_rows) {
+    auto tiles_of = [&](int b) {
+        const int lo = min(max(a.cu_q[b], 0), a.total_q), hi = min(max(a.cu_q[b + 1], 0), a.total_q);
+        return (int)(((long long)min(max(hi - lo, 0), a.max_q) * rows_per_token + tile_rows - 1) / tile_rows);
+    };
+    if (a.B == 1) {
+        const int n = tiles_of(0);
+        return tile < n ? make_int2(0, n - 1 - tile) : make_int2(-1, 0);
+    }
+    auto class_of = [&](int b) {
+        const int kv = a.kv_lens[b];
+        return kv > a.max_kv >> 1 ? 0 : kv > a.max_kv >> 2 ? 1 : kv > a.max_kv >> 3 ? 2 : 3;
+    };
     const int lane = threadIdx.x & 31;
+    const int per = (a.B + 31) / 32, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
+    int cnt[4] = {0, 0, 0, 0};
+    for (int b = b0; b < b1; ++b) {
+        const int n = tiles_of(b), c = class_of(b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cnt[i] += c == i ? n : 0;
+    }
     int before = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        const int b = b0 + lane;
-        int n = 0;
-        if (b < a.B) {
-            const int lo = min(max(a.cu_q[b], 0), a.total_q), hi = min(max(a.cu_q[b + 1], 0), a.total_q);
-            const long long rows = (long long)min(max(hi - lo, 0), a.max_q) * rows_per_token;
-            n = (int)((rows + tile_rows - 1) / tile_rows);
-        }
-        int incl = n;
+    int2 hit = make_int2(-1, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int incl = cnt[i];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += y;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > tile);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            const int start = before + __shfl_sync(0xffffffffu, incl - n, src);
-            return make_int2(b0 + src, tile - start);
+        int mine = before + incl - cnt[i];
+        if (tile >= mine && tile < mine + cnt[i]) {
+            for (int b = b0; b < b1; ++b) {
+                if (class_of(b) != i) continue;
+                const int n = tiles_of(b);
+                if (tile < mine + n) { hit = make_int2(b, mine + n - 1 - tile); break; }
+                mine += n;
+            }
         }
         before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    return make_int2(-1, 0);
-}
-
-// The same tiles in another order, for blocks that are dealt out as SMs come
-// free: sequences over half of max_kv first, then those over a quarter, an
-// eighth, and the rest, and in each sequence the last tile first (the longest
-// where causal), so that no long tile starts last.
-__device__ __forceinline__ int2 paged_find_tile_longest(const PagedArgs& a, int tile, int tile_tokens) {
-    const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int cls = 0; cls < 4; ++cls) {
-        const int lo_kv = cls < 3 ? a.max_kv >> (cls + 1) : -1, hi_kv = cls > 0 ? a.max_kv >> cls : 0x7fffffff;   // (lo, hi]
-        for (int b0 = 0; b0 < a.B; b0 += 32) {
-            const int b = b0 + lane;
-            int n = 0;
-            if (b < a.B) {
-                const int kv = min(max(a.kv_lens[b], 0), a.max_kv);
-                const int lo = min(max(a.cu_q[b], 0), a.total_q), hi = min(max(a.cu_q[b + 1], 0), a.total_q);
-                if (kv > lo_kv && kv <= hi_kv) n = (min(max(hi - lo, 0), a.max_q) + tile_tokens - 1) / tile_tokens;
-            }
-            int incl = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += y;
-            }
-            const unsigned hit = __ballot_sync(0xffffffffu, before + incl > tile);
-            if (hit) {
-                const int src = __ffs(hit) - 1;
-                const int last = before + __shfl_sync(0xffffffffu, incl, src) - 1;
-                return make_int2(b0 + src, last - tile);
-            }
-            before += __shfl_sync(0xffffffffu, incl, 31);
-        }
-    }
-    return make_int2(-1, 0);
+    const int src = __ffs(__ballot_sync(0xffffffffu, hit.x >= 0)) - 1;
+    if (src < 0) return make_int2(-1, 0);
+    return make_int2(__shfl_sync(0xffffffffu, hit.x, src), __shfl_sync(0xffffffffu, hit.y, src));
 }
 
 // Raise a kernel's dynamic shared-memory limit once per device (`seen`: a bit per

@@ -13,8 +13,8 @@
 // m_x is a reference, not the running maximum: softmax is the same for any m, and
 // P only has to stay in its type's range.  The first tile sets m to its maximum
 // (fp16: 2^7 below, so that P spans 2^-31 .. 2^8 relative to it); later tiles use
-// it at once and move it only where P would pass 2^60 (fp16: 2^15), rescaling
-// O_x and l_x.  So almost no tile waits for a maximum or touches O in TMEM.
+// it and move it only where P would pass 2^24 (fp16: 2^15), rescaling O_x and l_x.
+// So almost no tile touches O in TMEM.
 //
 // (Measured and left out, 8192-token prompt at D = 128, 443 us: a quarter of the
 // exponentials as a polynomial on the FMA pipe, 462 us; the two tiles' softmax
@@ -53,7 +53,7 @@ template <int DT, int D, bool Q8> struct PtCfg {
     static constexpr int RAW = PT_KEYS * D;                 // one tile of codes
     static constexpr int RAWS = Q8 ? 2 : 0;
     // a row's reference is set this far (base 2) below a maximum, and moves when a logit exceeds it by FAR
-    static constexpr float BELOW = DT == QV_F16 ? 7.f : 0.f, FAR = DT == QV_F16 ? 15.f : 60.f;
+    static constexpr float BELOW = DT == QV_F16 ? 7.f : 0.f, FAR = DT == QV_F16 ? 15.f : 24.f;
     static constexpr int THREADS = Q8 ? 512 : 384;
     // registers per thread after the split (the launch holds 128 x 512 or 168 x 384 of them)
     static constexpr int REGS_SOFTMAX = Q8 ? 192 : 208, REGS_OTHER = Q8 ? 64 : 88;
@@ -165,7 +165,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
     const int QT = PT_KEYS / a.G;                        // tokens per row tile
 
     if (warp == 0) {
-        const int2 t = paged_find_tile_longest(a, blockIdx.x / a.H, 2 * QT);
+        const int2 t = paged_find_tile(a, blockIdx.x / a.H, 1, 2 * QT);
         if (lane == 0) s_tile = t;
     }
     __syncthreads();

@@ -77,7 +77,7 @@ def rope_table(max_pos, rot_dim, theta=10000.0, scaling=None, device="cuda"):
 
 # Checks format their message only when they fail: a decode step's calls are
 # short enough for the host's time per call to count.
-_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(dev).cuda_stream without building the object
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # current_stream(dev).cuda_stream, 2 us sooner
 
 
 def _bad(name, expected, x):
@@ -207,6 +207,8 @@ def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=No
         qo, ko = out
         _vector("out[0]", qo, (T, Hq, D), dt, dev)
         _vector("out[1]", ko, (T, H, D), dt, dev)
+        if T and qo.data_ptr() == ko.data_ptr():
+            raise N.QevictError("out: q and k must be two tensors")
     _launch(dev, "qv_qk_norm_rope", T, Hq, H, D, code, q.data_ptr(), qs, k.data_ptr(), ks, qw, kw, eps, tab, max_pos,
             rot, bool(interleaved), pos, qo.data_ptr(), ko.data_ptr())
     return qo, ko
@@ -265,6 +267,8 @@ def paged_gather(k_pages, v_pages, block_table, kv_lens, cu_kv, total, *, k_scal
         ko, vo = out
         _vector("out[0]", ko, (total, H, D), dt, dev)
         _vector("out[1]", vo, (total, H, D), dt, dev)
+        if total and ko.data_ptr() == vo.data_ptr():
+            raise N.QevictError("out: k and v must be two tensors")
     _launch(dev, "qv_paged_gather", ctypes.byref(c), B, block_table.data_ptr(), width, kv_lens.data_ptr(),
             cu_kv.data_ptr(), total, ko.data_ptr(), vo.data_ptr())
     return ko, vo

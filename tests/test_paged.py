@@ -268,6 +268,7 @@ def test_native_refuses_bad_arguments():
                 dict(ko=FAKE + 8), dict(table=FAKE + 4)):
         assert rope(**bad) == N.QV_EINVAL, bad
     assert rope(T=0) == N.QV_OK
+    assert rope(qo=FAKE, ko=FAKE) == N.QV_EINVAL         # one buffer for both
     assert L.qv_paged_append(c, 1, 2, FAKE, 128, FAKE, 128, FAKE, 128, None, None, 0.0, None, 0, 0, 0, None, None,
                              FAKE, None) == N.QV_EINVAL
     assert L.qv_paged_append(c, 1, 2, FAKE, 128, FAKE, 128, None, 128, None, None, 0.0, None, 0, 0, 0, None, FAKE,
@@ -467,6 +468,19 @@ def test_attention(shape, dt, q8):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,q8", [(BF16, False), (FP16, True), (FP32, False)])
+@pytest.mark.parametrize("most", [1, 7])
+def test_attention_many_sequences(most, dt, q8):
+    """More sequences than a block has threads, some with nothing new, lengths over two orders of magnitude."""
+    r = torch.Generator().manual_seed(most)
+    B = 700
+    q_lens = torch.randint(0, most + 1, (B,), generator=r)
+    kv_lens = torch.maximum(q_lens, (2.0 ** (9 * torch.rand(B, generator=r))).long())
+    q_lens[5], kv_lens[5] = most, 900
+    check_attention(gen(41), q_lens.tolist(), kv_lens.tolist(), 4, 1, 64, 16, dt, q8, max_q=most, max_kv=900)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt,q8", [(BF16, False), (FP16, False), (BF16, True), (FP16, True), (FP32, False)])
 @pytest.mark.parametrize("q_lens,kv_lens", [([1], [900]), ([300], [900])])
 def test_attention_large_and_growing_logits(q_lens, kv_lens, dt, q8):
@@ -621,6 +635,11 @@ def test_attention_refusals():
                 dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan)):
         with pytest.raises(N.QevictError):
             pool.cache.attend(**{**ok, **bad})
+    two = torch.empty(20, 2, 64, dtype=BF16, device=DEV)
+    with pytest.raises(N.QevictError):
+        pool.cache.gather(pool.bt, pool.lens, cu([20]), 20, out=(two, two))
+    with pytest.raises(N.QevictError):
+        paged.qk_norm_rope(two, two.clone(), out=(two, two))
     small = paged.PagedKVCache(2, 2, 96, 16, BF16)
     with pytest.raises(N.QevictError):
         small.attend(rand(g, 3, 4, 96).to(BF16), pool.bt, pool.lens, cu([3]))
