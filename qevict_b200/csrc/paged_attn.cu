@@ -19,7 +19,7 @@ int paged_cache_check(const qv_paged_cache* c);
 int paged_shift(int page);
 
 int paged_tc_launch(const PagedArgs& a, int dt, int D, bool q8, int64_t tiles, cudaStream_t s);
-int paged_few_launch(const PagedArgs& a, int dt, int D, bool q8, cudaStream_t s);
+int paged_few_launch(const PagedArgs& a, int dt, int D, bool q8, bool wide, cudaStream_t s);
 
 constexpr int PC_THREADS = 256;
 
@@ -110,6 +110,7 @@ enum PagedKernel { PK_SIMT, PK_TC, PK_FEW };
 struct PagedPlan {
     PagedKernel kernel;
     int rows;      // query rows per tile (PK_SIMT)
+    bool wide;     // eight warps per block (PK_FEW)
     int64_t tiles; // upper bound of the query tiles of a KV head
     int splits, chunk;
 };
@@ -142,7 +143,7 @@ static int choose_splits(int64_t blocks, int slots, int max_kv, bool equal, doub
 }
 
 static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int max_q, int max_kv) {
-    PagedPlan p;
+    PagedPlan p = {};
     const bool few = (int64_t)max_q * G <= 16;
     p.kernel = dt == QV_F32 ? PK_SIMT : few ? PK_FEW : PK_TC;
     p.rows = few ? 16 : (int64_t)max_q * G <= 64 ? 64 : 128;
@@ -161,7 +162,12 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int
         // where lengths differ), of at least 128 keys; many: rounds enough to even out, of at least 1024
         const int64_t per_round = ((int64_t)max_q * G <= 8 ? 3 : 2) * 148, blocks = (int64_t)B * H;
         int64_t most;
-        if (2 * blocks <= per_round) { n = (int)((B > 1 ? per_round * 5 / 4 : 2 * 148) / blocks); most = ceil_div(max_kv, 128); }
+        // Short and few: one block of eight warps reads a sequence's head alone (512
+        // keys 6.1 us, as with four splits and their merge, which is a launch
+        // more; 8 uneven sequences of up to 1000 keys 9.2 against 9.5)
+        p.wide = blocks <= 148 && max_kv <= (B > 1 ? 1024 : 512);
+        if (p.wide) { n = 1; most = 1; }
+        else if (2 * blocks <= per_round) { n = (int)((B > 1 ? per_round * 5 / 4 : 2 * 148) / blocks); most = ceil_div(max_kv, 128); }
         else { n = (int)ceil_div(6 * per_round, blocks); most = ceil_div(max_kv, 1024); }
         if (n > most) n = (int)most;
     } else if (p.kernel == PK_TC) {
@@ -202,7 +208,7 @@ template <int D, bool Q8> static int simt_dispatch(const PagedArgs& a, const Pag
 template <int DT, int D> static int paged_launch(const PagedArgs& a, const PagedPlan& p, bool q8, cudaStream_t s) {
     int rc;
     if constexpr (DT == QV_F32) rc = q8 ? simt_dispatch<D, true>(a, p, s) : simt_dispatch<D, false>(a, p, s);
-    else if (p.kernel == PK_FEW) rc = paged_few_launch(a, DT, D, q8, s);
+    else if (p.kernel == PK_FEW) rc = paged_few_launch(a, DT, D, q8, p.wide, s);
     else rc = paged_tc_launch(a, DT, D, q8, p.tiles, s);
     if (rc != QV_OK || p.splits == 1) return rc;
     const int64_t rows = (int64_t)a.total_q * a.H * a.G;

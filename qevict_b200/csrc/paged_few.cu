@@ -37,18 +37,18 @@
 
 namespace qv {
 
-constexpr int PF_WARPS = 4;
-constexpr int PF_THREADS = 32 * PF_WARPS;
 constexpr float PF_BELOW = 7.f, PF_LAZY = 15.f;
 constexpr float PF_MIN_SCALE = 7.8886090522101181e-31f;   // 2^-100: a smaller value scale counts as this
 
-template <int D, bool Q8> struct PfCfg {
+// W warps: 4, several blocks per SM; 8, one block per SM, for short sequences
+// that a block then reads alone, without a merge after it.
+template <int D, bool Q8, int W> struct PfCfg {
     static constexpr int KT = D == 128 && !Q8 ? 16 : 32;            // keys per tile
     static constexpr int ROWB = Q8 ? D : 2 * D;                     // bytes of a cached row
     static constexpr int HALF = KT * ROWB, STAGE = 2 * HALF;        // K, V
-    static constexpr int STAGES = 16 * 1024 / STAGE;                // 64 KB per block in all
+    static constexpr int STAGES = (W == 4 ? 16 : 24) * 1024 / STAGE;   // 64 or 192 KB per block in all
     static constexpr int STATE = 16 * (D + 4) * 4;                  // a warp's output at the end, in its ring's place
-    static constexpr size_t SMEM = 1024 + (size_t)PF_WARPS * STAGES * (STAGE + (Q8 ? 2 * KT * 4 : 0));
+    static constexpr size_t SMEM = 1024 + (size_t)W * STAGES * (STAGE + (Q8 ? 2 * KT * 4 : 0));
     static_assert(STATE <= STAGES * STAGE, "state");
 };
 
@@ -77,10 +77,11 @@ __device__ __forceinline__ uint32_t pf_codes(uint32_t u, uint32_t v, uint32_t se
 }
 
 // NQ: n-tiles of 8 query rows.
-template <int DT, int D, bool Q8, int NQ>
-__global__ void __launch_bounds__(PF_THREADS, NQ == 1 ? 3 : 2)
+template <int DT, int D, bool Q8, int NQ, int W>
+__global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NQ == 1 ? 3 : 2)
 paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const PagedArgs a) {
-    using C = PfCfg<D, Q8>;
+    using C = PfCfg<D, Q8, W>;
+    constexpr int PF_WARPS = W, PF_THREADS = 32 * W;
     using T = typename Elt<DT>::T;
     constexpr int MT = Q8 ? QV_F16 : DT;                 // type of the products
     constexpr bool HILO = MT == QV_BF16;
@@ -466,31 +467,33 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
 bool paged_map_pages(CUtensorMap* m, const void* base, int dt, bool q8, int D, int page, int H, int pages, int box_rows,
                      CUtensorMapSwizzle codes);
 
-template <int DT, int D, bool Q8> static int pf_launch(const PagedArgs& a, cudaStream_t s) {
-    using C = PfCfg<D, Q8>;
+template <int DT, int D, bool Q8, int W> static int pf_launch(const PagedArgs& a, cudaStream_t s) {
+    using C = PfCfg<D, Q8, W>;
     CUtensorMap mK, mV;
-    const int page = 1 << a.page_shift;
-    const bool few8 = a.max_q * a.G <= 8;
-    const int piece = page < C::KT ? page : C::KT;
+    const int page = 1 << a.page_shift, piece = page < C::KT ? page : C::KT;
     const CUtensorMapSwizzle sw = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     if (!paged_map_pages(&mK, a.k, DT, Q8, D, page, a.H, a.pages, piece, sw) ||
         !paged_map_pages(&mV, a.v, DT, Q8, D, page, a.H, a.pages, piece, sw))
         return QV_EINVAL;
-    auto kernel = few8 ? paged_few_kernel<DT, D, Q8, 1> : paged_few_kernel<DT, D, Q8, 2>;
+    const bool few8 = a.max_q * a.G <= 8;
+    auto kernel = few8 ? paged_few_kernel<DT, D, Q8, 1, W> : paged_few_kernel<DT, D, Q8, 2, W>;
     static std::atomic<uint64_t> seen[2] = {{0}, {0}};
     const cudaError_t e = paged_smem(kernel, C::SMEM, &seen[few8]);
     if (e != cudaSuccess) return set_cuda_error(e);
-    const cudaError_t f = launch_pdl(kernel, dim3((unsigned)(a.B * a.H), a.splits), dim3(PF_THREADS), C::SMEM, s, mK, mV, a);
+    const cudaError_t f = launch_pdl(kernel, dim3((unsigned)(a.B * a.H), a.splits), dim3(32 * W), C::SMEM, s, mK, mV, a);
     return f == cudaSuccess ? check_launch() : set_cuda_error(f);
 }
 
-template <int DT> static int pf_dispatch(const PagedArgs& a, int D, bool q8, cudaStream_t s) {
-    if (D == 128) return q8 ? pf_launch<DT, 128, true>(a, s) : pf_launch<DT, 128, false>(a, s);
-    return q8 ? pf_launch<DT, 64, true>(a, s) : pf_launch<DT, 64, false>(a, s);
+template <int DT, int D, bool Q8> static int pf_width(const PagedArgs& a, bool wide, cudaStream_t s) {
+    return wide ? pf_launch<DT, D, Q8, 8>(a, s) : pf_launch<DT, D, Q8, 4>(a, s);
+}
+template <int DT> static int pf_dispatch(const PagedArgs& a, int D, bool q8, bool wide, cudaStream_t s) {
+    if (D == 128) return q8 ? pf_width<DT, 128, true>(a, wide, s) : pf_width<DT, 128, false>(a, wide, s);
+    return q8 ? pf_width<DT, 64, true>(a, wide, s) : pf_width<DT, 64, false>(a, wide, s);
 }
 
-int paged_few_launch(const PagedArgs& a, int dt, int D, bool q8, cudaStream_t s) {
-    return dt == QV_BF16 ? pf_dispatch<QV_BF16>(a, D, q8, s) : pf_dispatch<QV_F16>(a, D, q8, s);
+int paged_few_launch(const PagedArgs& a, int dt, int D, bool q8, bool wide, cudaStream_t s) {
+    return dt == QV_BF16 ? pf_dispatch<QV_BF16>(a, D, q8, wide, s) : pf_dispatch<QV_F16>(a, D, q8, wide, s);
 }
 
 }  // namespace qv
