@@ -258,8 +258,9 @@ int qv_prefill_read_error(const void* workspace, size_t workspace_bytes, int32_t
  * Pool: k, v [pages][kv_heads][page_size][head_dim] in dtype, or (bits = 8)
  * INT8 codes with one fp32 scale per row, k_scale / v_scale
  * [pages][kv_heads][page_size]: value = code * scale (attention may take a value
- * scale below 2^-100 as 2^-100).  Token j of a sequence b
- * lives in page block_table[b][j / page_size] at offset j % page_size.
+ * scale below 2^-60 as 2^-60, and a sequence's value scales reach up to 2^49).
+ * Token j of a sequence b lives in page block_table[b][j / page_size] at offset
+ * j % page_size.
  * Calls check what the device-side tables hold and stay inside their buffers;
  * what they find wrong sets bits of *err (when not NULL): a page id or a
  * position outside its table QV_DERR_TABLE (attention then reads page 0, the

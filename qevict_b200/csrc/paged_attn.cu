@@ -162,9 +162,8 @@ static PagedPlan paged_plan(int dt, int B, int H, int G, int D, int total_q, int
         // where lengths differ), of at least 128 keys; many: rounds enough to even out, of at least 1024
         const int64_t per_round = ((int64_t)max_q * G <= 8 ? 3 : 2) * 148, blocks = (int64_t)B * H;
         int64_t most;
-        // Short and few: one block of eight warps reads a sequence's head alone (512
-        // keys 6.1 us, as with four splits and their merge, which is a launch
-        // more; 8 uneven sequences of up to 1000 keys 9.2 against 9.5)
+        // Short and few: one block of eight warps reads a sequence's head alone, no
+        // splits and no merge (measured in paged_few.cu)
         p.wide = blocks <= 148 && max_kv <= (B > 1 ? 1024 : 512);
         if (p.wide) { n = 1; most = 1; }
         else if (2 * blocks <= per_round) { n = (int)((B > 1 ? per_round * 5 / 4 : 2 * 148) / blocks); most = ceil_div(max_kv, 128); }

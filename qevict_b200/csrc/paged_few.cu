@@ -5,12 +5,15 @@
 // Bound by HBM: every cached row is read once for at most 16 query rows, two
 // orders of magnitude below the tensor cores' balance, so the work is keeping
 // loads in flight.  A block takes one KV head of one sequence and a range of its
-// keys; each of its four warps walks its own tiles of 16 or 32 keys through a
+// keys; each of its warps walks its own tiles of 16 or 32 keys through a
 // ring of its own in shared memory (TMA, one elected lane, one mbarrier per
 // stage), so that no barrier couples the warps until their states join at the
-// end.  Three blocks share an SM (two with more than eight rows): one's start and
-// end hide behind the others' loads.  64 sequences over up to 8192 INT8 tokens:
-// 108 us, 122 us with two blocks and rings of three stages instead of two.
+// end.  Blocks of four warps with 64 KB of rings: three share an SM (two with more
+// than eight rows), and one's start and end hide behind the others' loads.  64
+// sequences over up to 8192 INT8 tokens: 108 us, 122 us with two blocks and rings of
+// three stages instead of two.  Short sequences that a block reads alone take eight
+// warps with 192 KB (512 keys 6.1 us, as four splits and their merge take with a
+// launch more; 8 uneven sequences of up to 1000 keys 9.2 against 9.5).
 //
 // Per tile, with warp-level MMA (m16n8k16) and the cached rows as the M side, so
 // that up to 8 query rows cost one n-tile and no padding of the conversions:
@@ -38,7 +41,11 @@
 namespace qv {
 
 constexpr float PF_BELOW = 7.f, PF_LAZY = 15.f;
-constexpr float PF_MIN_SCALE = 7.8886090522101181e-31f;   // 2^-100: a smaller value scale counts as this
+// 2^-60: a smaller value scale counts as this, a zero row's 0 too.  P carries the
+// scale and the sum divides by it, so a zero row of weight 2^-24 still counts (P is
+// a normal number) beside value scales up to 2^49 = 2^(126 + 7 - 60 - 24).  fp16's
+// own scales are 2^-31 .. 2^9.
+constexpr float PF_MIN_SCALE = 8.6736173798840355e-19f;
 
 // W warps: 4, several blocks per SM; 8, one block per SM, for short sequences
 // that a block then reads alone, without a merge after it.
@@ -117,7 +124,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
     float* ring_sc = reinterpret_cast<float*>(sm + PF_WARPS * C::STAGES * C::STAGE) + warp * C::STAGES * 2 * KT;
     __syncthreads();
 
-    // lane 0 loads: tile i of this warp holds the keys from k_begin + (warp + 4 i) KT on
+    // lane 0 loads: tile i of this warp holds the keys from k_begin + (warp + W i) KT on
     // (a TMA box is a whole tile, or at 16-token pages 16 of its keys)
     const int mine = tiles > warp ? (tiles - warp + PF_WARPS - 1) / PF_WARPS : 0;
     const int first = k_begin + warp * KT, past = first + mine * PF_WARPS * KT;

@@ -44,7 +44,7 @@ namespace qv {
 constexpr int PT_KEYS = 128;
 constexpr int PT_SLAB = 16384;            // 128 rows x 64 16-bit elements, 128-byte swizzle
 constexpr int PT_SC = 4;                  // tiles of row scales held (INT8)
-constexpr float PT_MIN_SCALE = 7.8886090522101181e-31f;   // 2^-100: a smaller value scale counts as this
+constexpr float PT_MIN_SCALE = 8.6736173798840355e-19f;   // 2^-60: a smaller value scale counts as this (fp16's own start at 2^-31)
 
 template <int DT, int D, bool Q8> struct PtCfg {
     static constexpr int NS = D / 64;                       // slabs per operand tile

@@ -558,6 +558,30 @@ def test_attention_int8_zero_and_uneven_rows(n, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,size", [(BF16, 2.0 ** 40), (BF16, 2.0 ** -40), (FP16, 2.0 ** 13), (FP16, 2.0 ** -14),
+                                     (FP32, 2.0 ** 40), (FP32, 2.0 ** -40)])
+@pytest.mark.parametrize("n", [1, 150])
+def test_attention_int8_zero_rows_beside_large_and_small_values(n, dt, size):
+    """INT8 value rows of zeros beside rows of any size: their probabilities count in the sum all the same."""
+    L, D, page = 400, 64, 32
+    g = gen(29)
+    pool = Pool(g, [L], 1, D, page, dt, True)
+    c = pool.cache
+    pos = torch.arange(L, device=DEV)
+    sl = c.slots(pool.bt, torch.zeros_like(pos), pos)
+    pg, off = sl // page, sl % page
+    zero = pos % 3 == 1
+    c.v_pages[pg[zero], :, off[zero]] = 0
+    c.v_scale[pg, 0, off] = torch.where(zero, 0.0, c.v_scale[pg, 0, off] * size)
+    pool.vs[0] = c.v_pages[pg, :, off].double() * c.v_scale[pg, :, off].double()[..., None]
+    q = rand(g, n, 4, D).to(dt)
+    out = c.attend(q, pool.bt, pool.lens, cu([n]), max_q=n)
+    o, mag, big = ref_attention(q, pool.ks[0], pool.vs[0])
+    bound = attention_bound(o, mag, big, L, D, dt, float(pool.vs[0].abs().max()))
+    assert bool(((out.double() - o).abs() <= bound).all()), float(((out.double() - o).abs() / bound).max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("q8", [False, True])
 @pytest.mark.parametrize("n", [1, 150])
 @pytest.mark.parametrize("dt", [BF16, FP16, FP32])
