@@ -314,13 +314,14 @@ int qv_paged_gather(const qv_paged_cache* c, int32_t batch, const int32_t* block
  * elements) and the last of its kv_lens[b] cached tokens; causal: each sees the
  * keys up to its own, otherwise all.  A row that sees no key gives 0; rows
  * outside every chunk are left as they were.  max_q and max_kv are upper bounds
- * of the chunk and cached lengths (max_kv <= max_pages * page_size): they size
- * the launch, so a captured call serves any lengths below them.  Of a longer
- * chunk the rows past max_q are left as they were, a longer sequence is cut.  out [total_q][q_heads][head_dim].  head_dim 64
- * or 128, q_heads / kv_heads up to 16, scale > 0.  Sums run in a fixed order.  Rows of one
- * tile share their P.V products, so a K or V row that is not finite can reach
- * rows of its own sequence that do not see it; what lies behind a sequence's
- * last token, in its pages or others, is never used. */
+ * of the chunk and cached lengths (max_kv <= max_pages * page_size, and 2^30):
+ * they size the launch, so a captured call serves any lengths below them.  Of a
+ * longer chunk the rows past max_q are left as they were, a longer sequence is
+ * cut.  out [total_q][q_heads][head_dim] (it may be q where that is contiguous).
+ * head_dim 64 or 128, q_heads / kv_heads up to 16, scale > 0.  Sums run in a fixed
+ * order.  Rows of one tile share their P.V products, so a K or V row that is not
+ * finite can reach rows of its own sequence that do not see it; what lies behind
+ * a sequence's last token, in its pages or others, is never used. */
 size_t qv_paged_attention_workspace_bytes(const qv_paged_cache* c, int32_t batch, int32_t q_heads, int32_t total_q,
                                           int32_t max_q, int32_t max_kv);
 int qv_paged_attention(const qv_paged_cache* c, int32_t batch, int32_t q_heads, const int32_t* block_table,

@@ -223,7 +223,7 @@ using namespace qv;
 
 static bool attn_dims_ok(const qv_paged_cache* c, int32_t batch, int32_t q_heads, int32_t total_q, int32_t max_q,
                          int32_t max_kv) {
-    if (batch < 0 || total_q < 0 || max_q < 0 || max_kv < 0 || q_heads <= 0) return false;
+    if (batch < 0 || total_q < 0 || max_q < 0 || max_kv < 0 || max_kv > 1 << 30 || q_heads <= 0) return false;
     if (c->head_dim != 64 && c->head_dim != 128) return false;
     if (q_heads % c->kv_heads || q_heads / c->kv_heads > 16 || c->kv_heads > 65535) return false;
     return (int64_t)total_q * q_heads <= 0x7fffffff;

@@ -25,6 +25,7 @@ import torch
 
 from . import _native as N
 
+_INT_MAX = 2 ** 31 - 1
 _DTYPES = {torch.float32: N.QV_F32, torch.bfloat16: N.QV_BF16, torch.float16: N.QV_F16}
 
 
@@ -91,11 +92,23 @@ def _heads(name, x, tokens, dim, dtype, dev):
         raise _bad(name, f"[tokens, heads, {dim}] {dtype} on {dev}", x)
     n, h, d = x.shape
     st, sh, sd = x.stride()
-    if d != dim or n != (n if tokens is None else tokens):
+    if d != dim or n != (n if tokens is None else tokens) or n > _INT_MAX:
         raise _bad(name, f"[{'tokens' if tokens is None else tokens}, heads, {dim}]", x)
     if sd != 1 or (sh != dim and h != 1):
         raise N.QevictError(f"{name}: a token's heads must be contiguous, got strides {(st, sh, sd)}")
     return n, h, st if n > 1 else h * dim
+
+
+def _apart(name, out, *reads):
+    """Refuse an output that shares memory with what the call reads, unless it is reads[0] itself (each block reads
+    its rows before it writes them)."""
+    a = out.data_ptr()
+    z = a + out.numel() * out.element_size()
+    for i, x in enumerate(reads):
+        b = x.data_ptr()
+        n = x.numel() and (sum((d - 1) * s for d, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+        if a < b + n and b < z and (i or a != b or not x.is_contiguous()):
+            raise N.QevictError(f"{name} shares memory with another tensor of the call")
 
 
 def _vector(name, x, shape, dtype, dev):
@@ -175,6 +188,8 @@ def _turn(tokens, dim, dtype, dev, positions, table, q_weight, k_weight):
     if table.ndim != 2 or table.dtype is not torch.float32 or table.device != dev or not table.is_contiguous():
         raise _bad("table", f"a contiguous [max_pos, rot_dim] fp32 tensor on {dev} (rope_table)", table)
     max_pos, rot = table.shape
+    if max_pos > _INT_MAX:
+        raise _bad("table", "fewer positions", table)
     if not 8 <= rot <= dim or rot % 8:
         raise N.QevictError(f"table: rot_dim {rot} is not a multiple of 8 up to head_dim {dim}")
     if positions is None:
@@ -207,8 +222,8 @@ def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=No
         qo, ko = out
         _vector("out[0]", qo, (T, Hq, D), dt, dev)
         _vector("out[1]", ko, (T, H, D), dt, dev)
-        if T and qo.data_ptr() == ko.data_ptr():
-            raise N.QevictError("out: q and k must be two tensors")
+        _apart("out[0]", qo, q, k, ko)
+        _apart("out[1]", ko, k, q)
     _launch(dev, "qv_qk_norm_rope", T, Hq, H, D, code, q.data_ptr(), qs, k.data_ptr(), ks, qw, kw, eps, tab, max_pos,
             rot, bool(interleaved), pos, qo.data_ptr(), ko.data_ptr())
     return qo, ko
@@ -233,6 +248,7 @@ def paged_append(q, k, v, slots, positions, table, k_pages, v_pages, *, k_scale=
         q_out = q.new_empty(T, Hq, D)
     else:
         _vector("q_out", q_out, (T, Hq, D), dt, dev)
+        _apart("q_out", q_out, q, k, v)
     _launch(dev, "qv_paged_append", ctypes.byref(c), T, Hq, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, qw,
             kw, eps, tab, max_pos, rot, bool(interleaved), pos, slots.data_ptr(), q_out.data_ptr())
     return q_out
@@ -258,8 +274,8 @@ def paged_gather(k_pages, v_pages, block_table, kv_lens, cu_kv, total, *, k_scal
     dt = k_pages.dtype if dtype is None else dtype
     c, dev, H, _, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
     B, width = _tables(block_table, kv_lens, cu_kv, dev)
-    if total < 0:
-        raise N.QevictError("total must not be negative")
+    if not 0 <= total <= _INT_MAX:
+        raise N.QevictError(f"total {total} is not a number of rows")
     if out is None:
         ko = torch.empty(total, H, D, dtype=dt, device=dev)
         vo = torch.empty_like(ko)
@@ -267,8 +283,8 @@ def paged_gather(k_pages, v_pages, block_table, kv_lens, cu_kv, total, *, k_scal
         ko, vo = out
         _vector("out[0]", ko, (total, H, D), dt, dev)
         _vector("out[1]", vo, (total, H, D), dt, dev)
-        if total and ko.data_ptr() == vo.data_ptr():
-            raise N.QevictError("out: k and v must be two tensors")
+        _apart("out[0]", ko, k_pages, vo, v_pages)
+        _apart("out[1]", vo, k_pages, v_pages)
     _launch(dev, "qv_paged_gather", ctypes.byref(c), B, block_table.data_ptr(), width, kv_lens.data_ptr(),
             cu_kv.data_ptr(), total, ko.data_ptr(), vo.data_ptr())
     return ko, vo
@@ -283,8 +299,8 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
     kv_lens[b] (int32 [batch]) cached tokens; block_table int32 [batch, max_pages].  Causal: each token sees the
     keys up to its own.  A row that sees no key gives 0; rows of no chunk are left as they were (out) or
     undefined.  max_q / max_kv: upper bounds of the chunk and cached lengths, which size the launch (default:
-    T, and all that the block table can hold); a captured call serves any lengths below them.  scale
-    (positive) defaults to D^-1/2.  (qv_paged_attention)"""
+    T, and all that the block table can hold); a captured call serves any lengths below them.  out may be q
+    where that is contiguous.  scale (positive) defaults to D^-1/2.  (qv_paged_attention)"""
     dt = q.dtype
     c, dev, H, S, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
     if D != 64 and D != 128:
@@ -293,14 +309,15 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
     if Hq % H or Hq // H > 16:
         raise N.QevictError(f"{Hq} query heads are not 1 to 16 times the pool's {H}")
     B, width = _tables(block_table, kv_lens, cu_q, dev)
-    max_q = T if max_q is None else max_q
+    max_q = T if max_q is None else min(max_q, T)
     max_kv = width * S if max_kv is None else max_kv
-    if max_q < 0 or not 0 <= max_kv <= width * S:
-        raise N.QevictError(f"max_q {max_q} and max_kv {max_kv} must be lengths, max_kv at most the block table's {width * S}")
+    if max_q < 0 or not 0 <= max_kv <= width * S or max_kv > 1 << 30:
+        raise N.QevictError(f"max_q {max_q} and max_kv {max_kv} must be lengths, max_kv at most the block table's {width * S} and 2^30")
     if out is None:
         out = q.new_empty(T, Hq, D)
     else:
         _vector("out", out, (T, Hq, D), dt, dev)
+        _apart("out", out, q)
     cp = ctypes.byref(c)
     wsb = N.lib().qv_paged_attention_workspace_bytes(cp, B, Hq, T, max_q, max_kv)
     # from torch's allocator at each call: a captured graph gets one of its own

@@ -803,3 +803,66 @@ def test_chunked_prompt_then_decode(bits):
     ref, mag, big = ref_attention(torch.cat(rot[0])[:n0], kb, vb)
     bound = attention_bound(ref, mag, big, n0, D, dt, float(vb.abs().max())) * 2 + mag * half(dt) * (2 * 2 * big + 2)
     assert bool(((po[0].double() - mine).abs() <= bound).all())
+
+
+def test_native_refuses_lengths_past_2_30():
+    L, c = N.lib(), ctypes.byref(cache_desc())
+    big = (1 << 30) + 1
+    assert L.qv_paged_attention_workspace_bytes(c, 1, 2, 1, 1, big) == 0
+    assert L.qv_paged_attention(c, 1, 2, FAKE, 1 << 27, FAKE, FAKE, 1, 1, big, FAKE, 128, 1.0, 1, FAKE, FAKE, 1 << 40,
+                                None) == N.QV_EINVAL
+
+
+@pytest.mark.gpu
+def test_numbers_past_32_bits_are_not_cut():
+    g = gen(41)
+    pool = Pool(g, [20], 2, 64, 16, BF16, False)
+    q = rand(g, 3, 4, 64).to(BF16)
+    want = pool.cache.attend(q, pool.bt, pool.lens, cu([3]))
+    assert torch.equal(pool.cache.attend(q, pool.bt, pool.lens, cu([3]), max_q=2 ** 32), want)
+    with pytest.raises(N.QevictError):
+        pool.cache.attend(q, pool.bt, pool.lens, cu([3]), max_kv=2 ** 32 + 20)
+    two = torch.empty(20, 2, 64, dtype=BF16, device=DEV)
+    with pytest.raises(N.QevictError):
+        pool.cache.gather(pool.bt, pool.lens, cu([20]), 2 ** 32 + 20)
+    with pytest.raises(N.QevictError):
+        pool.cache.gather(pool.bt, pool.lens, cu([20]), 2 ** 32 + 20, out=(two, two.clone()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,q8", [(BF16, False), (BF16, True), (FP16, False), (FP32, False)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [700, 20]), ([1], [5000]), ([200, 1, 40], [900, 30, 40])])
+def test_outputs_in_place_and_overlapping(q_lens, kv_lens, dt, q8):
+    """An output in its input's place gives the same bits; any other overlap is refused."""
+    g = gen(43)
+    pool = Pool(g, kv_lens, 2, 128, 32, dt, q8)
+    c, n = pool.cache, sum(q_lens)
+    buf = rand(g, 3 * n, 8, 128).to(dt)
+    q = buf[:n]
+    kw = dict(block_table=pool.bt, kv_lens=pool.lens, cu_q=cu(q_lens), max_q=max(q_lens))
+    want = c.attend(q, **kw)
+    mine = q.clone()
+    assert c.attend(mine, out=mine, **kw) is mine and torch.equal(mine, want)
+    with pytest.raises(N.QevictError):
+        c.attend(buf.view(-1, 128)[4:4 + 8 * n].view(n, 8, 128), out=q, **kw)
+    with pytest.raises(N.QevictError):       # a strided view of the rows it would write over
+        c.attend(buf[::2][:n], out=q, **kw) if n > 1 else c.attend(q, out=q[:, :4], **kw)
+    k, v = buf[n:2 * n], buf[2 * n:]
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    table = paged.rope_table(n, 128)
+    want = paged.qk_norm_rope(q, k, pos, table)
+    for out in ((k, q), (q, q), (v, v), (q, buf.view(-1, 128)[4:4 + 8 * n].view(n, 8, 128))):
+        with pytest.raises(N.QevictError):
+            paged.qk_norm_rope(q, k, pos, table, out=out)
+    a, b = q.clone(), k.clone()
+    paged.qk_norm_rope(a, b, pos, table, out=(a, b))
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    slots = torch.full((n,), -1, dtype=torch.int64, device=DEV)
+    kk = torch.zeros(n, 2, 128, dtype=dt, device=DEV)
+    vv = torch.zeros(8 * n, 128, dtype=dt, device=DEV)
+    with pytest.raises(N.QevictError):
+        c.append(q, kk, vv.view(4 * n, 2, 128)[:n], slots, pos, table, q_out=vv.view(n, 8, 128))
+    a = q.clone()
+    assert torch.equal(c.append(a, kk, kk, slots, pos, table, q_out=a), want[0])
+    with pytest.raises(N.QevictError):
+        c.gather(pool.bt, pool.lens, cu(kv_lens), n, out=(vv[:2 * n].view(n, 2, 128), vv[1:1 + 2 * n].view(n, 2, 128)))
