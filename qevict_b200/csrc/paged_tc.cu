@@ -8,7 +8,11 @@
 // with P_x as the TMEM operand.  The two row tiles alternate: while one's 128
 // softmax threads work (one row each), the tensor cores run the other's two
 // products, so a key tile costs the larger of 2 x 2 products and the
-// exponentials (16 per clock and SM) instead of their sum.
+// exponentials (16 per clock and SM) instead of their sum.  The (x, j) pairs take
+// two or three S buffers in turn (what O leaves of TMEM's 512 columns), so that at
+// D = 64, or once only one row tile has keys left, S of a later tile is ready when a
+// tile's softmax ends: 17 chunks and single tokens at D = 64 102 us (114 with one
+// buffer per row tile), four 512-token chunks over INT8 pages 241 (272).
 //
 // m_x is a reference, not the running maximum: softmax is the same for any m, and
 // P only has to stay in its type's range.  The first tile sets m to its maximum
@@ -43,7 +47,6 @@ namespace qv {
 
 constexpr int PT_KEYS = 128;
 constexpr int PT_SLAB = 16384;            // 128 rows x 64 16-bit elements, 128-byte swizzle
-constexpr int PT_SC = 4;                  // tiles of row scales held (INT8)
 constexpr float PT_MIN_SCALE = 8.6736173798840355e-19f;   // 2^-60: a smaller value scale counts as this (fp16's own start at 2^-31)
 
 template <int DT, int D, bool Q8> struct PtCfg {
@@ -52,15 +55,16 @@ template <int DT, int D, bool Q8> struct PtCfg {
     static constexpr int SLOTS = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8);   // K and V tiles in turn
     static constexpr int RAW = PT_KEYS * D;                 // one tile of codes
     static constexpr int RAWS = Q8 ? 2 : 0;
+    static constexpr int NB = D == 64 ? 3 : 2;              // S buffers: what of TMEM's 512 columns O leaves
+    static constexpr int SC = D == 64 ? 8 : 4;              // tiles of row scales held (INT8)
     // a row's reference is set this far (base 2) below a maximum, and moves when a logit exceeds it by FAR
     static constexpr float BELOW = DT == QV_F16 ? 7.f : 0.f, FAR = DT == QV_F16 ? 15.f : 24.f;
     static constexpr int THREADS = Q8 ? 512 : 384;
     // registers per thread after the split (the launch holds 128 x 512 or 168 x 384 of them)
     static constexpr int REGS_SOFTMAX = Q8 ? 192 : 208, REGS_OTHER = Q8 ? 64 : 88;
-    // Q, slots, codes, and the row scales as loaded (2) and prepared (PT_SC x 3)
-    static_assert(!Q8 || 2 * PT_SC - SLOTS >= 2, "scale ring");
+    // Q, slots, codes, and the row scales as loaded (2) and prepared (SC x 3)
     static constexpr size_t SMEM = 1024 + 2 * SLOT + SLOTS * SLOT + RAWS * RAW +
-                                   (Q8 ? (2 + PT_SC * 3) * PT_KEYS * 4 : 0);
+                                   (Q8 ? (2 + SC * 3) * PT_KEYS * 4 : 0);
     static_assert(SMEM <= 232448 - 512, "shared memory");
 };
 
@@ -147,16 +151,16 @@ __global__ void __launch_bounds__(PtCfg<DT, D, Q8>::THREADS, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
                 const __grid_constant__ CUtensorMap mV, const PagedArgs a) {
     using C = PtCfg<DT, D, Q8>;
-    constexpr int NS = C::NS, SLOT = C::SLOT, SLOTS = C::SLOTS;
+    constexpr int NS = C::NS, SLOT = C::SLOT, SLOTS = C::SLOTS, NB = C::NB, PT_SC = C::SC;
     extern __shared__ unsigned char pt_raw[];
     unsigned char* sm = pt_raw + ((1024u - (smem_u32(pt_raw) & 1023u)) & 1023u);
     unsigned char* sQ = sm;                              // [2][NS] slabs
     unsigned char* sKV = sQ + 2 * SLOT;                  // [SLOTS]: K0, V0, K1, V1, ...
     unsigned char* sRaw = sKV + SLOTS * SLOT;            // [RAWS] tiles of codes
     float* sRawSc = reinterpret_cast<float*>(sRaw + C::RAWS * C::RAW);   // [2][128] as loaded: ks, vs
-    float* sSc = sRawSc + 2 * PT_KEYS;                   // [PT_SC][3][128]: c ks and vs, or (fp16) c ks, log2 vs, 1 / vs
+    float* sSc = sRawSc + 2 * PT_KEYS;                   // [SC][3][128]: c ks and vs, or (fp16) c ks, log2 vs, 1 / vs
     __shared__ __align__(8) uint64_t q_full, kv_full[SLOTS], kv_empty[SLOTS], raw_full[2], raw_empty[2], sc_full[PT_SC];
-    __shared__ __align__(8) uint64_t s_full[2], p_full[2][2], o_full[2], tail, done;
+    __shared__ __align__(8) uint64_t s_full[NB], p_full[NB][2], o_full[NB], o_last[2], tail, done;
     __shared__ uint32_t s_taddr;
     __shared__ int2 s_tile;
     __shared__ int s_quit;
@@ -196,8 +200,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&kv_full[i], Q8 ? 6 : 1); mbar_init(&kv_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 6);
+        for (int i = 0; i < 2; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 6); mbar_init(&o_last[i], 1); }
+        for (int i = 0; i < NB; ++i) {
             mbar_init(&s_full[i], 1); mbar_init(&o_full[i], 1);
             mbar_init(&p_full[i][0], 4); mbar_init(&p_full[i][1], 4);
         }
@@ -210,7 +214,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t taddr = s_taddr;      // S (P over it): [0, 128), [128, 256); O: [256, 256 + D), [384, 384 + D)
+    const uint32_t taddr = s_taddr;      // NB x 128 columns of S (P over it), then O of the two row tiles
+    constexpr int O_AT = 128 * NB;
+    static_assert(O_AT + 2 * D <= 512, "TMEM columns");
+    // The (row tile, key tile) pairs in the order of their products, the two row tiles in turn while both have keys
+    // left (the second has at least as many as the first, or none); pair `step` uses buffer step % NB.
+    const int both = nt[1] > 0 ? nt[0] : 0, steps = nt[0] + nt[1];
     volatile int* quit = &s_quit;
 
     if (warp < 8) {
@@ -218,7 +227,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
         // ------------------------------------------------------------ softmax of row tile x
         const int x = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t ts = taddr + lane_off + 128 * x, to = taddr + lane_off + 256 + 128 * x;
+        const uint32_t to = taddr + lane_off + O_AT + D * x;
         const int i = r / a.G;
         const int tok_x = x ? tok[1] : tok[0], tn = x ? nt[1] : nt[0];
         const bool live = i < (x ? cnt[1] : cnt[0]);
@@ -232,10 +241,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
         const float cl = a.scale_log2;
         const uint64_t c2 = pt_pack(cl, cl);
         bool ok = true;
+        int step = 0, before = 0;            // this tile's pair, the one before
         for (int j = 0; j < tn; ++j) {
-            ok = pt_wait(&s_full[x], j & 1, quit, a.err);
-            // (an entry is refilled once K of tile j + 1 has been released, which follows
-            // this tile's P: 2 PT_SC - SLOTS >= 2 steps of the ring lie between)
+            before = step;
+            step = j < both ? 2 * j + x : both + j;
+            const int buf = step % NB;
+            const uint32_t ts = taddr + lane_off + 128 * buf;
+            ok = pt_wait(&s_full[buf], (step / NB) & 1, quit, a.err);
             if (Q8 && ok) ok = pt_wait(&sc_full[j % PT_SC], (j / PT_SC) & 1, quit, a.err);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -243,7 +255,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
             if (idle) {                      // no live row in this warp: P may hold anything there
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) { mbar_arrive(&p_full[x][0]); mbar_arrive(&p_full[x][1]); }
+                if (lane == 0) { mbar_arrive(&p_full[buf][0]); mbar_arrive(&p_full[buf][1]); }
                 continue;
             }
             float v[128];
@@ -289,7 +301,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
                 m = mn;
                 l2 = pt_mul2(l2, pt_both(f));
                 if (j > 0) {
-                    // S(j) is complete, so P.V of every earlier tile is
+                    ok = __all_sync(0xffffffffu, pt_wait(&o_full[before % NB], (before / NB) & 1, quit, a.err));   // P.V of the tile before
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll
                     for (int w = 0; w < D / 16; ++w) {
                         float o[16];
@@ -343,7 +357,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[x][w >> 1]);
+                    if (lane == 0) mbar_arrive(&p_full[buf][w >> 1]);
                 }
             }
             l2 = pt_add2(acc[0], acc[1]);
@@ -351,7 +365,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
         float l0, l1;
         pt_unpack(l2, l0, l1);
         const float l = l0 + l1;
-        if (tn > 0) ok = ok && pt_wait(&o_full[x], 0, quit, a.err);
+        if (tn > 0) ok = ok && pt_wait(&o_last[x], 0, quit, a.err);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
@@ -486,61 +500,63 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
                 };
                 bool ok = wait(&q_full, 0);
                 tc_fence_after();
-                auto scores = [&](int x, int j) {
-                    const uint64_t q = dq + x * (SLOT >> 4), k = dk + ((2 * j) % SLOTS) * (SLOT >> 4);
-                    if (one) {
-#pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) {
-                            constexpr int S4 = PT_SLAB >> 4;
-                            umma_ss(taddr + 128 * x, q + (kk >> 2) * S4 + (kk & 3) * 2, k + (kk >> 2) * S4 + (kk & 3) * 2, id_s, kk > 0);
-                        }
-                        umma_commit(&s_full[x]);
-                    }
-                };
                 auto wait_tile = [&](int it) {
                     bool o = wait(&kv_full[it % SLOTS], (it / SLOTS) & 1);
                     if (!Q8 && o && cut && it == 2 * n - 1) o = wait(&tail, 0);
                     tc_fence_after();
                     return o;
                 };
-                if (ok) ok = wait_tile(0);
-                if (ok) {
+                // pair `step`: row tile, key tile, and whether no later pair reads the key tile
+                auto pair = [&](int step, int& x, int& j, bool& last) {
+                    const bool two = step < 2 * both;
+                    x = two ? step & 1 : nt[1] > 0;
+                    j = two ? step >> 1 : step - both;
+                    last = x == 1 || j >= nt[1];
+                };
+                auto scores = [&](int step) {
+                    int x, j;
+                    bool last;
+                    pair(step, x, j, last);
+                    if (!wait_tile(2 * j)) return false;
+                    const uint64_t q = dq + x * (SLOT >> 4), k = dk + ((2 * j) % SLOTS) * (SLOT >> 4);
+                    const uint32_t to = taddr + 128 * (step % NB);
+                    if (one) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        if (nt[x] > 0) scores(x, 0);
-                    if (one) umma_commit(&kv_empty[0]);
-                }
-                for (int j = 0; j < n && ok; ++j) {
-                    bool v_in = false, k_in = false;
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        if (!ok || j >= nt[x]) continue;
-                        const bool last_user = x == 1 || j >= nt[1];
-                        if (!v_in) { ok = wait_tile(2 * j + 1); v_in = true; }
-                        const uint64_t v = dv + ((2 * j + 1) % SLOTS) * (SLOT >> 4);
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            if (ok) ok = wait(&p_full[x][hf], j & 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            if (one) {
-#pragma unroll
-                                for (int kk = 4 * hf; kk < 4 * hf + 4; ++kk)
-                                    umma_ts(taddr + 256 + 128 * x, taddr + 128 * x + 8 * kk, v + kk * 128, id_o, j > 0 || kk > 0);
-                            }
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            constexpr int S4 = PT_SLAB >> 4;
+                            umma_ss(to, q + (kk >> 2) * S4 + (kk & 3) * 2, k + (kk >> 2) * S4 + (kk & 3) * 2, id_s, kk > 0);
                         }
-                        if (!ok) continue;
+                        umma_commit(&s_full[step % NB]);
+                        if (last) umma_commit(&kv_empty[(2 * j) % SLOTS]);
+                    }
+                    return true;
+                };
+                for (int i = 0; i < NB && i < steps && ok; ++i) ok = scores(i);
+                for (int i = 0; i < steps && ok; ++i) {
+                    int x, j;
+                    bool last;
+                    pair(i, x, j, last);
+                    ok = wait_tile(2 * j + 1);
+                    const uint64_t v = dv + ((2 * j + 1) % SLOTS) * (SLOT >> 4);
+                    const uint32_t ps = taddr + 128 * (i % NB), to = taddr + O_AT + D * x;
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        if (ok) ok = wait(&p_full[i % NB][hf], (i / NB) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
                         if (one) {
-                            if (j + 1 == nt[x]) umma_commit(&o_full[x]);
-                            if (last_user) umma_commit(&kv_empty[(2 * j + 1) % SLOTS]);
-                        }
-                        if (j + 1 < nt[x]) {
-                            if (!k_in) { ok = wait_tile(2 * j + 2); k_in = true; }
-                            if (!ok) continue;
-                            scores(x, j + 1);
-                            if (one && (x == 1 || j + 1 >= nt[1])) umma_commit(&kv_empty[(2 * j + 2) % SLOTS]);
+#pragma unroll
+                            for (int kk = 4 * hf; kk < 4 * hf + 4; ++kk)
+                                umma_ts(to, ps + 8 * kk, v + kk * 128, id_o, j > 0 || kk > 0);
                         }
                     }
+                    if (!ok) break;
+                    if (one) {
+                        umma_commit(&o_full[i % NB]);
+                        if (j + 1 == (x ? nt[1] : nt[0])) umma_commit(&o_last[x]);
+                        if (last) umma_commit(&kv_empty[(2 * j + 1) % SLOTS]);
+                    }
+                    if (i + NB < steps) ok = scores(i + NB);
                 }
                 // no MMA is in flight when the TMEM is released
                 if (one) umma_commit(&done);
