@@ -123,8 +123,9 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // uneven (half of the longest on average, dealt out longest first: the sum over
 // the slots, or the longest block); the merge writes and reads every split's
 // fp32 rows once.  Measured for the tcgen05 kernel: four 512-token chunks over
-// up to 16384 INT8 keys 264 / 289 / 275 us with 2 / 3 / 4 splits, 17 sequences of up
-// to 4000 keys 119 / 161 us with 1 / 2, a 2048-token prompt 43 / 86 us with 1 / 3.
+// up to 16384 INT8 keys 314 / 330 / 241 / 272 / 237 us with 1 .. 5 splits (3 taken),
+// 17 sequences of up to 4000 keys 102 / 158 us with 1 / 2, a 2048-token prompt
+// 43 / 85 us with 1 / 2.
 static int choose_splits(int64_t blocks, int slots, int max_kv, bool equal, double start, double key_us, double merge_bytes,
                          int least_keys) {
     const int64_t steps = ceil_div(max_kv, 128), most = ceil_div(max_kv, least_keys);

@@ -20,11 +20,14 @@
 // it and move it only where P would pass 2^24 (fp16: 2^15), rescaling O_x and l_x.
 // So almost no tile touches O in TMEM.
 //
-// (Measured and left out, 8192-token prompt at D = 128, 443 us: a quarter of the
-// exponentials as a polynomial on the FMA pipe, 462 us; the two tiles' softmax
-// warps taking turns at the exponentials, 456 us; two threads to a row, 494 us.
-// Without any exponentials it takes 443 us too: the tensor pipe at the clock that
-// its power allows bounds it.)
+// (Measured and left out, 8192-token prompt at D = 128, 437-443 us: a quarter of
+// the exponentials as a polynomial on the FMA pipe, 462 us; the two tiles' softmax
+// warps taking turns at the exponentials, 456 us; two threads to a row, 494 us; no
+// row maximum, the reference moving where a tile's sum of P is too large, 455-468.
+// Without any exponentials it takes as long: the tensor pipe at the clock that its
+// power allows bounds it.  At D = 64 (347 us, 346 without exponentials) the bound
+// is the softmax warps' dependent instructions: two warps per scheduler issue in
+// 39 % of its cycles.)
 //
 // INT8 pages: codes become exact 16-bit integers in shared memory (six extra
 // warps); the row scales ks, vs of a key stay in fp32: the logit is S c ks, and the
