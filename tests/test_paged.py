@@ -866,3 +866,37 @@ def test_outputs_in_place_and_overlapping(q_lens, kv_lens, dt, q8):
     assert torch.equal(c.append(a, kk, kk, slots, pos, table, q_out=a), want[0])
     with pytest.raises(N.QevictError):
         c.gather(pool.bt, pool.lens, cu(kv_lens), n, out=(vv[:2 * n].view(n, 2, 128), vv[1:1 + 2 * n].view(n, 2, 128)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,q8", [(BF16, False), (FP16, False), (BF16, True), (FP16, True)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,G,causal", [(20, 4, True), (40, 4, True), (33, 1, False), (129, 1, True), (8, 8, True)])
+def test_attention_moving_reference_of_one_and_two_row_tiles(n, G, causal, D, dt, q8):
+    """Logits that climb by 10 (base 2) or more from key tile to key tile, for one row tile alone, two of unlike key
+    counts, and a second one of a single row; and a chunk longer than its sequence, whose first rows see nothing."""
+    L, page = 1500, 32
+    g = gen(47)
+    lens = [L, L - 700, n // 2]
+    pool = Pool(g, lens, 1, D, page, dt, q8)
+    c = pool.cache
+    u = torch.nn.functional.normalize(rand(g, D), dim=-1)
+    for b, m in enumerate(lens):
+        pos = torch.arange(m, device=DEV)
+        rows = (pos.float() / L * 20)[:, None, None] * u + 0.05 * rand(g, m, 1, D)
+        sl = c.slots(pool.bt, torch.full_like(pos, b), pos)
+        if q8:
+            s = rows.abs().amax(-1) / 127
+            code = (rows / s[..., None]).round()
+            c.k_pages[sl // page, :, sl % page], c.k_scale[sl // page, :, sl % page] = code.to(torch.int8), s
+            pool.ks[b] = code.double() * s.double()[..., None]
+        else:
+            c.k_pages[sl // page, :, sl % page] = rows.to(dt)
+            pool.ks[b] = rows.to(dt).double()
+    q = (u * 120 + 0.05 * rand(g, 3 * n, G, D)).to(dt)
+    out = c.attend(q, pool.bt, pool.lens, cu([n, n, n]), max_q=n, causal=causal)
+    assert c.read_error() == 0
+    for b, m in enumerate(lens):
+        o, mag, big = ref_attention(q[b * n:(b + 1) * n], pool.ks[b], pool.vs[b], causal)
+        bound = attention_bound(o, mag, big, m, D, dt, float(pool.vs[b].abs().max()))
+        assert bool(((out[b * n:(b + 1) * n].double() - o).abs() <= bound).all()), b
