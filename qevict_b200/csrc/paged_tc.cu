@@ -59,7 +59,9 @@ template <int DT, int D, bool Q8> struct PtCfg {
     static constexpr int RAW = PT_KEYS * D;                 // one tile of codes
     static constexpr int RAWS = Q8 ? 2 : 0;
     static constexpr int NB = D == 64 ? 3 : 2;              // S buffers: what of TMEM's 512 columns O leaves
-    static constexpr int SC = D == 64 ? 8 : 4;              // tiles of row scales held (INT8)
+    // Tiles of row scales held (INT8).  Entry j is rewritten for tile j + SC, once the slot of that tile's K is free:
+    // at D = 128 after P.V of tile j + 2, at D = 64 after S of tile j + 5, which follows P of tile j + 2 at least.
+    static constexpr int SC = D == 64 ? 8 : 4;
     // a row's reference is set this far (base 2) below a maximum, and moves when a logit exceeds it by FAR
     static constexpr float BELOW = DT == QV_F16 ? 7.f : 0.f, FAR = DT == QV_F16 ? 15.f : 24.f;
     static constexpr int THREADS = Q8 ? 512 : 384;
@@ -221,7 +223,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
     constexpr int O_AT = 128 * NB;
     static_assert(O_AT + 2 * D <= 512, "TMEM columns");
     // The (row tile, key tile) pairs in the order of their products, the two row tiles in turn while both have keys
-    // left (the second has at least as many as the first, or none); pair `step` uses buffer step % NB.
+    // left (the second has at least as many as the first, or none); pair `step` uses buffer step % NB.  S of pair
+    // step + NB is issued behind P.V of pair step, so a buffer's barriers (s_full, p_full, o_full) are never more than
+    // a phase ahead of a warp that waits on them by parity; the last P.V of a row tile has a barrier of its own
+    // (o_last), since the other row tile goes on using the buffers.
     const int both = nt[1] > 0 ? nt[0] : 0, steps = nt[0] + nt[1];
     volatile int* quit = &s_quit;
 
