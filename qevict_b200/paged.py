@@ -104,11 +104,15 @@ def _apart(name, out, *reads):
     its rows before it writes them)."""
     a = out.data_ptr()
     z = a + out.numel() * out.element_size()
+    if a == z:
+        return
     for i, x in enumerate(reads):
         b = x.data_ptr()
-        n = x.numel() and (sum((d - 1) * s for d, s in zip(x.shape, x.stride())) + 1) * x.element_size()
-        if a < b + n and b < z and (i or a != b or not x.is_contiguous()):
-            raise N.QevictError(f"{name} shares memory with another tensor of the call")
+        if b >= z or (b == a and i == 0 and x.is_contiguous()) or not x.numel():
+            continue
+        if b < a and b + x.element_size() * (sum((d - 1) * s for d, s in zip(x.shape, x.stride())) + 1) <= a:
+            continue
+        raise N.QevictError(f"{name} shares memory with another tensor of the call")
 
 
 def _vector(name, x, shape, dtype, dev):
