@@ -305,7 +305,8 @@ int qv_paged_append(const qv_paged_cache* c, int32_t tokens, int32_t q_heads, co
                     qv_stream_t stream);
 /* The cached rows as contiguous tensors: k_out, v_out [total][kv_heads][head_dim] in
  * dtype, sequence b's first kv_lens[b] tokens from row cu_kv[b] (cu_kv [batch + 1],
- * ascending); other rows are left as they were. */
+ * ascending); other rows are left as they were.  Outputs that share memory with one
+ * another, the pool or the tables are refused. */
 int qv_paged_gather(const qv_paged_cache* c, int32_t batch, const int32_t* block_table, int32_t max_pages,
                     const int32_t* kv_lens, const int32_t* cu_kv, int32_t total, void* k_out, void* v_out,
                     qv_stream_t stream);

@@ -463,7 +463,16 @@ extern "C" int qv_paged_gather(const qv_paged_cache* c, int32_t batch, const int
     if (batch < 0 || total < 0) return QV_EINVAL;
     if (batch == 0 || total == 0) return QV_OK;
     if (!block_table || max_pages <= 0 || !kv_lens || !cu_kv || !k_out || !v_out) return QV_EINVAL;
-    if (!al16(k_out) || !al16(v_out) || k_out == v_out) return QV_EINVAL;
+    if (!al16(k_out) || !al16(v_out)) return QV_EINVAL;
+    // a block writes rows that others still read: nothing in place
+    const size_t out_bytes = (size_t)total * c->kv_heads * c->head_dim * elt_size(c->dtype), sb = pool_scale_bytes(c);
+    const Span ko = span(k_out, out_bytes), vo = span(v_out, out_bytes);
+    for (const Span& o : {ko, vo})
+        if (meets(o, {span(c->k, pool_bytes(c)), span(c->v, pool_bytes(c)), span(c->k_scale, sb), span(c->v_scale, sb),
+                      span(block_table, (size_t)batch * max_pages * 4), span(kv_lens, (size_t)batch * 4),
+                      span(cu_kv, ((size_t)batch + 1) * 4), span(c->err, 4)}))
+            return QV_EINVAL;
+    if (meets(ko, {vo})) return QV_EINVAL;
     GatherArgs a = {c->k, c->v, c->k_scale, c->v_scale, c->err, block_table, kv_lens, cu_kv, k_out, v_out,
                     c->pages, c->kv_heads, c->head_dim, paged_shift(c->page_size), max_pages, batch, total};
     const int g = (int)(((int64_t)total + PG_TOKENS - 1) / PG_TOKENS);

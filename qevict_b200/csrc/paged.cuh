@@ -3,6 +3,7 @@
 #pragma once
 
 #include <atomic>
+#include <initializer_list>
 
 #include "common.cuh"
 
@@ -144,6 +145,22 @@ __device__ __forceinline__ int2 paged_find_tile(const PagedArgs& a, int tile, in
     const int src = __ffs(__ballot_sync(0xffffffffu, hit.x >= 0)) - 1;
     if (src < 0) return make_int2(-1, 0);
     return make_int2(__shfl_sync(0xffffffffu, hit.x, src), __shfl_sync(0xffffffffu, hit.y, src));
+}
+
+// A buffer of a call (none: 0 bytes), for the host's check of what may not overlap.
+struct Span { uintptr_t at; size_t bytes; };
+inline Span span(const void* p, size_t bytes) { return {reinterpret_cast<uintptr_t>(p), p ? bytes : 0}; }
+inline bool meets(Span a, std::initializer_list<Span> others) {
+    for (const Span& b : others)
+        if (a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes) return true;
+    return false;
+}
+// The pool's rows, and its row scales (none without INT8).
+inline size_t pool_bytes(const qv_paged_cache* c) {
+    return (size_t)c->pages * c->kv_heads * c->page_size * c->head_dim * (c->bits == 8 ? 1 : elt_size(c->dtype));
+}
+inline size_t pool_scale_bytes(const qv_paged_cache* c) {
+    return c->bits == 8 ? (size_t)c->pages * c->kv_heads * c->page_size * sizeof(float) : 0;
 }
 
 // Raise a kernel's dynamic shared-memory limit once per device (`seen`: a bit per

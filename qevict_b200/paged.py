@@ -99,16 +99,18 @@ def _heads(name, x, tokens, dim, dtype, dev):
     return n, h, st if n > 1 else h * dim
 
 
-def _apart(name, out, *reads):
-    """Refuse an output that shares memory with what the call reads, unless it is reads[0] itself (each block reads
-    its rows before it writes them)."""
+def _apart(name, out, *reads, inplace=None):
+    """Refuse an output that shares memory with a tensor that the call reads.  It may take the place of `inplace`, of the
+    same shape and contiguous, where the caller's kernel reads each row in the block that writes it, before it does."""
     a = out.data_ptr()
     z = a + out.numel() * out.element_size()
     if a == z:
         return
-    for i, x in enumerate(reads):
+    if inplace is not None and not (inplace.data_ptr() == a and inplace.is_contiguous()):
+        reads += (inplace,)
+    for x in reads:
         b = x.data_ptr()
-        if b >= z or (b == a and i == 0 and x.is_contiguous()) or not x.numel():
+        if b >= z or not x.numel():
             continue
         if b < a and b + x.element_size() * (sum((d - 1) * s for d, s in zip(x.shape, x.stride())) + 1) <= a:
             continue
@@ -226,8 +228,8 @@ def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=No
         qo, ko = out
         _vector("out[0]", qo, (T, Hq, D), dt, dev)
         _vector("out[1]", ko, (T, H, D), dt, dev)
-        _apart("out[0]", qo, q, k, ko)
-        _apart("out[1]", ko, k, q)
+        _apart("out[0]", qo, k, ko, inplace=q)
+        _apart("out[1]", ko, q, inplace=k)
     _launch(dev, "qv_qk_norm_rope", T, Hq, H, D, code, q.data_ptr(), qs, k.data_ptr(), ks, qw, kw, eps, tab, max_pos,
             rot, bool(interleaved), pos, qo.data_ptr(), ko.data_ptr())
     return qo, ko
@@ -252,7 +254,7 @@ def paged_append(q, k, v, slots, positions, table, k_pages, v_pages, *, k_scale=
         q_out = q.new_empty(T, Hq, D)
     else:
         _vector("q_out", q_out, (T, Hq, D), dt, dev)
-        _apart("q_out", q_out, q, k, v)
+        _apart("q_out", q_out, k, v, inplace=q)
     _launch(dev, "qv_paged_append", ctypes.byref(c), T, Hq, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, qw,
             kw, eps, tab, max_pos, rot, bool(interleaved), pos, slots.data_ptr(), q_out.data_ptr())
     return q_out
@@ -274,7 +276,8 @@ def paged_gather(k_pages, v_pages, block_table, kv_lens, cu_kv, total, *, k_scal
                  out=None, err=None):
     """The cached rows as contiguous (k, v) [total, kv_heads, D] in dtype (default: the pages' own; INT8 pages
     need it): the first kv_lens[b] tokens of sequence b from row cu_kv[b] on, cu_kv [batch + 1] ascending int32;
-    rows of no sequence are left as they were (out) or undefined.  (qv_paged_gather)"""
+    rows of no sequence are left as they were (out) or undefined.  out may not share memory with the pool or with
+    anything else that the call reads.  (qv_paged_gather)"""
     dt = k_pages.dtype if dtype is None else dtype
     c, dev, H, _, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
     B, width = _tables(block_table, kv_lens, cu_kv, dev)
@@ -321,7 +324,7 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
         out = q.new_empty(T, Hq, D)
     else:
         _vector("out", out, (T, Hq, D), dt, dev)
-        _apart("out", out, q)
+        _apart("out", out, inplace=q)
     cp = ctypes.byref(c)
     wsb = N.lib().qv_paged_attention_workspace_bytes(cp, B, Hq, T, max_q, max_kv)
     # from torch's allocator at each call: a captured graph gets one of its own

@@ -900,3 +900,62 @@ def test_attention_moving_reference_of_one_and_two_row_tiles(n, G, causal, D, dt
         o, mag, big = ref_attention(q[b * n:(b + 1) * n], pool.ks[b], pool.vs[b], causal)
         bound = attention_bound(o, mag, big, m, D, dt, float(pool.vs[b].abs().max()))
         assert bool(((out[b * n:(b + 1) * n].double() - o).abs() <= bound).all()), b
+
+
+# ------------------------------------------------------------------ buffers that share memory
+def at(n):
+    """The n-th of a row of addresses a GB apart, which no refused call touches."""
+    return FAKE + (n << 30)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_native_gather_refuses_outputs_on_what_it_reads(q8):
+    L = N.lib()
+    c = cache_desc(k=at(1), v=at(2), err=at(9), pages=4, kv_heads=1, page_size=16, head_dim=64, bits=8 if q8 else 0,
+                   k_scale=at(3) if q8 else None, v_scale=at(4) if q8 else None)
+
+    def gather(ko, vo, bt=at(5), lens=at(6), cu_kv=at(7)):
+        return L.qv_paged_gather(ctypes.byref(c), 2, bt, 2, lens, cu_kv, 20, ko, vo, None)
+    pool, rows = 4 * 16 * 64 * (1 if q8 else 2), 20 * 64 * 2
+    for base, size in [(at(1), pool), (at(2), pool), (at(5), 16), (at(6), 8), (at(7), 12), (at(9), 4)] + (
+            [(at(3), 256), (at(4), 256)] if q8 else []):
+        # at its first byte, at its last 16, and ending on its first 16
+        for o in (base, base + (size - 1) // 16 * 16, base - rows + 16):
+            assert gather(o, at(20)) == N.QV_EINVAL
+            assert gather(at(20), o) == N.QV_EINVAL
+    for o in (at(20), at(20) + rows - 16, at(20) - rows + 16):
+        assert gather(at(20), o) == N.QV_EINVAL
+
+
+def test_an_output_is_only_in_place_where_the_call_says_so():
+    """The pool's memory as a row list (one KV head), from its first byte or elsewhere."""
+    pool = torch.zeros(4, 1, 16, 64)
+    out = pool.view(-1, 1, 64)[:20]
+    for o in (out, pool.view(-1, 1, 64)[1:21], pool.view(-1, 1, 64)[44:]):
+        with pytest.raises(N.QevictError):
+            paged._apart("out", o, pool, torch.zeros(20, 1, 64))
+    q = torch.zeros(20, 1, 64)
+    paged._apart("out", q, pool, inplace=q)
+    with pytest.raises(N.QevictError):
+        paged._apart("out", q, q, inplace=q)
+    with pytest.raises(N.QevictError):
+        paged._apart("out", q[:10], pool, inplace=q[::2])
+    paged._apart("out", q[10:], q[:10], inplace=pool)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+def test_gather_refuses_outputs_on_its_pool(q8):
+    g = gen(53)
+    pool = Pool(g, [20, 9], 1, 64, 16, BF16, q8)
+    c, free = pool.cache, torch.empty(29, 1, 64, dtype=BF16, device=DEV)
+    before = [x.clone() for x in (c.k_pages, c.v_pages)]
+    for x in (c.k_pages, c.v_pages) + ((c.k_scale, c.v_scale) if q8 else ()):
+        rows = x.view(-1).view(BF16)[: x.numel() * x.element_size() // 128 * 64].view(-1, 1, 64)
+        for n in (29, 1):
+            o = rows[:n] if len(rows) >= n else rows
+            lens, total = torch.full_like(pool.lens, len(o) // 2), len(o)
+            for out in ((o, free[:total]), (free[:total], o)):
+                with pytest.raises(N.QevictError):
+                    c.gather(pool.bt, lens, cu([total // 2, total // 2]), total, out=out)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, (c.k_pages, c.v_pages)))
