@@ -265,7 +265,9 @@ int qv_prefill_read_error(const void* workspace, size_t workspace_bytes, int32_t
  * what they find wrong sets bits of *err (when not NULL): a page id or a
  * position outside its table QV_DERR_TABLE (attention then reads page 0, the
  * read-back leaves the row), a slot behind the pool or a length above its
- * bound QV_DERR_CAPACITY (not written / cut to the bound). */
+ * bound QV_DERR_CAPACITY (not written / cut to the bound).
+ * What a call writes may not share memory with anything else of the call, but
+ * for the places named below: such a call is refused (QV_EINVAL). */
 typedef struct qv_paged_cache {
     void* k;
     void* v;
@@ -305,8 +307,7 @@ int qv_paged_append(const qv_paged_cache* c, int32_t tokens, int32_t q_heads, co
                     qv_stream_t stream);
 /* The cached rows as contiguous tensors: k_out, v_out [total][kv_heads][head_dim] in
  * dtype, sequence b's first kv_lens[b] tokens from row cu_kv[b] (cu_kv [batch + 1],
- * ascending); other rows are left as they were.  Outputs that share memory with one
- * another, the pool or the tables are refused. */
+ * ascending); other rows are left as they were. */
 int qv_paged_gather(const qv_paged_cache* c, int32_t batch, const int32_t* block_table, int32_t max_pages,
                     const int32_t* kv_lens, const int32_t* cu_kv, int32_t total, void* k_out, void* v_out,
                     qv_stream_t stream);

@@ -393,6 +393,32 @@ static int heads_check(const HeadArgs& a, int64_t tokens, int dt) {
     return QV_OK;
 }
 
+// Whether outputs share memory with one another or with what the call reads.  A row is read by the block that writes it,
+// before it does: the queries (and, without pages, the keys) may be written in place where they are contiguous.
+static bool heads_overlap(const HeadArgs& a, int64_t tokens, int dt, const qv_paged_cache* c) {
+    const size_t e = elt_size(dt), n = (size_t)tokens, w = (size_t)a.D * e;
+    auto rows = [&](const void* p, int64_t stride, int heads) { return span(p, ((n - 1) * (size_t)stride + (size_t)heads * a.D) * e); };
+    const Span q = rows(a.q, a.qs, a.Hq), k = rows(a.k, a.ks, a.H), v = rows(a.v, a.vs, a.H);
+    const Span qw = span(a.qw, w), kw = span(a.kw, w), table = span(a.table, (size_t)a.max_pos * a.rot * 4);
+    const Span pos = span(a.table ? a.pos : nullptr, n * 4), slots = span(a.slots, n * 8), err = span(a.err, 4);
+    auto in_place = [&](Span in, Span out) { return in.at == out.at && in.bytes == out.bytes; };
+    auto taken = [&](Span o) { return meets(o, {v, qw, kw, table, pos, slots, err}); };
+    const Span qo = span(a.q_out, n * a.Hq * w);
+    if (taken(qo) || meets(qo, {k}) || (meets(qo, {q}) && !in_place(q, qo))) return true;
+    if (!c) {
+        const Span ko = span(a.k_out, n * a.H * w);
+        return taken(ko) || meets(ko, {q, qo}) || (meets(ko, {k}) && !in_place(k, ko));
+    }
+    const size_t pb = pool_bytes(c), sb = pool_scale_bytes(c);
+    const Span pool[4] = {span(c->k, pb), span(c->v, pb), span(c->k_scale, sb), span(c->v_scale, sb)};
+    for (int i = 0; i < 4; ++i) {
+        if (taken(pool[i]) || meets(pool[i], {q, k, qo})) return true;
+        for (int j = 0; j < i; ++j)
+            if (meets(pool[i], {pool[j]})) return true;
+    }
+    return false;
+}
+
 template <int DT, int MODE> static int heads_launch(const HeadArgs& a, int64_t tokens, cudaStream_t s) {
     // Few tokens: large blocks, one for each kind of head (a decode step's latency).  Many: one small block per
     // token, so that a thread has rows enough to pay for the token's table row and slot; 16383 tokens of 64
@@ -427,7 +453,7 @@ extern "C" int qv_qk_norm_rope(int32_t tokens, int32_t q_heads, int32_t kv_heads
     if (tokens == 0) return QV_OK;
     const int rc = heads_check(a, tokens, dtype);
     if (rc != QV_OK) return rc;
-    if (!k_out || !al16(k_out) || k_out == q_out) return QV_EINVAL;
+    if (!k_out || !al16(k_out) || heads_overlap(a, tokens, dtype, nullptr)) return QV_EINVAL;
     return heads_dispatch<PH_ROWS_ONLY>(a, tokens, dtype, (cudaStream_t)stream);
 }
 
@@ -451,6 +477,7 @@ extern "C" int qv_paged_append(const qv_paged_cache* c, int32_t tokens, int32_t 
     if (rc != QV_OK) return rc;
     const int64_t per16 = 16 / (int64_t)elt_size(c->dtype);
     if (!v || !al16(v) || !slots || v_stride < (int64_t)a.H * a.D || v_stride % per16) return QV_EINVAL;
+    if (heads_overlap(a, tokens, c->dtype, c)) return QV_EINVAL;
     return c->bits == 8 ? heads_dispatch<PH_PAGES8>(a, tokens, c->dtype, (cudaStream_t)stream)
                         : heads_dispatch<PH_PAGES>(a, tokens, c->dtype, (cudaStream_t)stream);
 }

@@ -260,6 +260,17 @@ extern "C" int qv_paged_attention(const qv_paged_cache* c, int32_t batch, int32_
     const size_t need = paged_ws_bytes(p, total_q, q_heads, c->head_dim);
     if (need > workspace_bytes) return QV_ESPACE;
     if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return QV_EINVAL;
+    // out may be q where that is contiguous (a block reads the rows that it writes, and no others' heads); nothing else
+    // that is written may be read
+    const size_t e = elt_size(c->dtype), row = (size_t)q_heads * c->head_dim, sb = pool_scale_bytes(c);
+    const Span qs = span(q, ((size_t)(total_q - 1) * q_stride + row) * e), o = span(out, (size_t)total_q * row * e);
+    const Span ws = span(workspace, need);
+    for (const Span& x : {o, ws})
+        if (meets(x, {span(c->k, pool_bytes(c)), span(c->v, pool_bytes(c)), span(c->k_scale, sb), span(c->v_scale, sb),
+                      span(block_table, (size_t)batch * max_pages * 4), span(kv_lens, (size_t)batch * 4),
+                      span(cu_q, ((size_t)batch + 1) * 4), span(c->err, 4)}))
+            return QV_EINVAL;
+    if (meets(ws, {qs, o}) || (meets(o, {qs}) && !(o.at == qs.at && o.bytes == qs.bytes))) return QV_EINVAL;
     PagedArgs a = {};
     a.k = c->k; a.v = c->v; a.k_scale = c->k_scale; a.v_scale = c->v_scale; a.err = c->err;
     a.block_table = block_table; a.kv_lens = kv_lens; a.cu_q = cu_q; a.q = q; a.out = out;

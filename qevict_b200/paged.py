@@ -12,6 +12,10 @@ tensors' device, none of which synchronises:
   paged_attention  chunks of new tokens, from one token to whole prompts,
                    over the pages
 
+What a call writes (outputs, and the pool of paged_append) may not share memory
+with anything else of the call: refused, but for the in-place outputs that are
+named below.
+
 PagedKVCache holds a pool and calls them.  Pools are [pages, kv_heads,
 page_size, head_dim] in the model's dtype or INT8 with one fp32 scale per row
 ([pages, kv_heads, page_size]); token j of sequence b lives in page
@@ -238,9 +242,9 @@ def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=No
 def paged_append(q, k, v, slots, positions, table, k_pages, v_pages, *, k_scale=None, v_scale=None, q_weight=None,
                  k_weight=None, eps=1e-6, interleaved=False, q_out=None, err=None):
     """qk_norm_rope with the keys and the values v [T, kv_heads, D] written into the pool: token t to slots[t]
-    (int64, page * page_size + offset; negative: not written).  Returns the queries.  INT8 pages get
-    scale = max|row| / 127 and code = rint(row / scale) of the fp32 row.  A slot must appear at most once per
-    call; err collects device errors (PagedKVCache.read_error).  (qv_paged_append)"""
+    (int64, page * page_size + offset; negative: not written).  Returns the queries (q_out may be q where that is
+    contiguous).  INT8 pages get scale = max|row| / 127 and code = rint(row / scale) of the fp32 row.  A slot must
+    appear at most once per call; err collects device errors (PagedKVCache.read_error).  (qv_paged_append)"""
     dt = q.dtype
     c, dev, H, _, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
     T, Hq, qs = _heads("q", q, None, D, dt, dev)
@@ -276,8 +280,7 @@ def paged_gather(k_pages, v_pages, block_table, kv_lens, cu_kv, total, *, k_scal
                  out=None, err=None):
     """The cached rows as contiguous (k, v) [total, kv_heads, D] in dtype (default: the pages' own; INT8 pages
     need it): the first kv_lens[b] tokens of sequence b from row cu_kv[b] on, cu_kv [batch + 1] ascending int32;
-    rows of no sequence are left as they were (out) or undefined.  out may not share memory with the pool or with
-    anything else that the call reads.  (qv_paged_gather)"""
+    rows of no sequence are left as they were (out) or undefined.  (qv_paged_gather)"""
     dt = k_pages.dtype if dtype is None else dtype
     c, dev, H, _, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
     B, width = _tables(block_table, kv_lens, cu_kv, dev)

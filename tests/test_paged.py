@@ -959,3 +959,102 @@ def test_gather_refuses_outputs_on_its_pool(q8):
                 with pytest.raises(N.QevictError):
                     c.gather(pool.bt, lens, cu([total // 2, total // 2]), total, out=out)
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, (c.k_pages, c.v_pages)))
+
+
+def around(base, size, rows):
+    """Addresses of `rows` bytes that meet [base, base + size) at its first byte, its last 16, and from below."""
+    return [base, base + (size - 1) // 16 * 16, base - rows + 16]
+
+
+@pytest.mark.parametrize("dt", [N.QV_F32, N.QV_BF16])
+@pytest.mark.parametrize("q8", [False, True])
+def test_native_attention_refuses_written_buffers_on_others(q8, dt):
+    L, e = N.lib(), 4 if dt == N.QV_F32 else 2
+    c = cache_desc(k=at(1), v=at(2), err=at(9), pages=4, kv_heads=2, page_size=16, head_dim=64, dtype=dt,
+                   bits=8 if q8 else 0, k_scale=at(3) if q8 else None, v_scale=at(4) if q8 else None)
+    cp, T, row = ctypes.byref(c), 3, 4 * 64
+    need = L.qv_paged_attention_workspace_bytes(cp, 2, 4, T, 1, 32 * 1024)
+
+    def attn(out=at(20), ws=at(30), qs=row):
+        return L.qv_paged_attention(cp, 2, 4, at(5), 2048, at(6), at(7), T, 1, 32 * 1024, at(8), qs, 1.0, 1, out, ws,
+                                    need, None)
+    pool = 4 * 2 * 16 * 64 * (1 if q8 else e)
+    reads = [(at(1), pool), (at(2), pool), (at(5), 2 * 2048 * 4), (at(6), 8), (at(7), 12), (at(9), 4)] + (
+        [(at(3), 512), (at(4), 512)] if q8 else [])
+    assert need > 0
+    for base, size in reads:
+        for o in around(base, size, T * row * e):
+            assert attn(out=o) == N.QV_EINVAL
+        for o in around(base, size, need):
+            assert attn(ws=o) == N.QV_EINVAL
+    for o in around(at(8), T * row * e, need):
+        assert attn(ws=o) == N.QV_EINVAL
+    assert attn(ws=at(20)) == attn(ws=at(20) + T * row * e - 16) == N.QV_EINVAL
+    # queries: in their place only where they are contiguous, not shifted
+    assert attn(out=at(8) + 16) == attn(out=at(8) - 16) == attn(out=at(8), qs=2 * row) == N.QV_EINVAL
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_native_head_kernels_refuse_written_buffers_on_others(q8):
+    L, T, D, H, Hq = N.lib(), 3, 64, 1, 2
+    qb, kb = T * Hq * D * 2, T * H * D * 2
+    reads = [(at(11), kb), (at(12), D * 2), (at(13), D * 2), (at(14), 8 * D * 4), (at(15), T * 4)]   # k, weights, table, positions
+
+    def rope(qo=at(20), ko=at(21), qs=Hq * D, ks=H * D):
+        return L.qv_qk_norm_rope(T, Hq, H, D, N.QV_BF16, at(10), qs, at(11), ks, at(12), at(13), 0.0, at(14), 8, D, 0,
+                                 at(15), qo, ko, None)
+    for base, size in reads:
+        assert all(rope(qo=o) == N.QV_EINVAL for o in around(base, size, qb))
+        if base != at(11):
+            assert all(rope(ko=o) == N.QV_EINVAL for o in around(base, size, kb))
+    assert all(rope(ko=o) == N.QV_EINVAL for o in around(at(10), qb, kb) + around(at(20), qb, kb))
+    assert rope(qo=at(10) + 16) == rope(qo=at(10), qs=2 * Hq * D) == N.QV_EINVAL
+    assert rope(ko=at(11) + 16) == rope(ko=at(11), ks=2 * H * D) == N.QV_EINVAL
+
+    def append(qo=at(20), qs=Hq * D, values=at(16), **kw):
+        d = dict(k=at(1), v=at(2), err=at(9), pages=4, kv_heads=H, page_size=16, head_dim=D, bits=8 if q8 else 0,
+                 k_scale=at(3) if q8 else None, v_scale=at(4) if q8 else None)
+        c = cache_desc(**{**d, **kw})
+        return L.qv_paged_append(ctypes.byref(c), T, Hq, at(10), qs, at(11), H * D, values, H * D, at(12), at(13), 0.0,
+                                 at(14), 8, D, 0, at(15), at(17), qo, None)
+    reads += [(at(16), kb), (at(17), T * 8), (at(9), 4)]      # v, slots, the error word
+    pool = 4 * H * 16 * D * (1 if q8 else 2)
+    scales = [("k_scale", at(3)), ("v_scale", at(4))] if q8 else []
+    for base, size in reads + [(at(1), pool), (at(2), pool)] + [(b, 256) for _, b in scales]:
+        assert all(append(qo=o) == N.QV_EINVAL for o in around(base, size, qb))
+    assert append(qo=at(10) + 16) == append(qo=at(10), qs=2 * Hq * D) == N.QV_EINVAL
+    # the pool on what the call reads, and its parts on one another
+    for base, size in reads + [(at(10), qb)]:
+        for name, n in [("k", pool), ("v", pool)] + [(s, 256) for s, _ in scales]:
+            assert all(append(**{name: o}) == N.QV_EINVAL for o in around(base, size, n)), (base, name)
+    assert append(values=at(2) + 32) == append(k=at(2)) == append(k=at(2) + pool - 16) == N.QV_EINVAL
+    if q8:
+        assert append(k_scale=at(4)) == append(k_scale=at(1)) == append(v_scale=at(2) + pool - 16) == N.QV_EINVAL
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+def test_outputs_on_the_pool_and_shared_pools_are_refused(q8):
+    g = gen(59)
+    pool = Pool(g, [20], 1, 64, 16, BF16, q8)
+    c, T = pool.cache, 3
+    q, k, v = rand(g, T, 4, 64).to(BF16), rand(g, T, 1, 64).to(BF16), rand(g, T, 1, 64).to(BF16)
+    slots = torch.arange(T, device=DEV)
+    on = [x.view(-1).view(BF16)[: T * 4 * 64].view(T, 4, 64) for x in (c.k_pages, c.v_pages)]
+    before = [x.clone() for x in (c.k_pages, c.v_pages)]
+    for o in on:
+        with pytest.raises(N.QevictError):
+            c.attend(q, pool.bt, pool.lens, cu([T]), out=o)
+        with pytest.raises(N.QevictError):
+            c.append(q, k, v, slots, q_out=o)
+        with pytest.raises(N.QevictError):       # queries read from the pool that the call writes
+            c.append(o, k, v, slots)
+    with pytest.raises(N.QevictError):
+        paged.paged_append(q, k, v, slots, None, None, c.k_pages, c.k_pages, k_scale=c.k_scale, v_scale=c.v_scale)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, (c.k_pages, c.v_pages)))
+    # what may share: reads alone (one tensor for keys and values), and outputs in their input's place
+    paged.paged_attention(q, c.k_pages, c.k_pages, pool.bt, pool.lens, cu([T]), k_scale=c.k_scale, v_scale=c.k_scale)
+    packed = torch.cat([q, k, v], 1)[:1]
+    want = c.append(packed[:, :4].clone(), packed[:, 4:5], packed[:, 5:], slots[:1])
+    got = c.append(packed[:, :4], packed[:, 4:5], packed[:, 5:], slots[:1], q_out=packed[:, :4])
+    assert got.data_ptr() == packed.data_ptr() and torch.equal(got, want)
