@@ -363,10 +363,21 @@ class PagedKVCache:
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
 
     def slots(self, block_table, seq, pos):
-        """Slots of tokens at index pos [T] of sequences seq [T] (int64 [T])."""
-        pos = pos.long()
-        page = torch.div(pos, self.page_size, rounding_mode="floor")
-        return block_table[seq.long(), page].long() * self.page_size + pos % self.page_size
+        """Slots of tokens at index pos [T] of sequences seq [T] (int64 [T]).  A negative pos gives -1 (append writes
+        nothing); an index outside the block table, or a page that is not the pool's, gives a slot behind the
+        pool (append writes nothing and raises QV_DERR_CAPACITY)."""
+        B, width = block_table.shape
+        pages, size = self.k_pages.shape[0], self.page_size
+        pos, seq = pos.long(), seq.long()
+        before = pos < 0
+        if not B * width:
+            return torch.full_like(pos, pages * size).masked_fill_(before, -1)
+        page = pos >> size.bit_length() - 1
+        outside = (page >= width) | (seq < 0) | (seq >= B)
+        at = torch.add(page, seq, alpha=width).masked_fill_(outside | before, 0)
+        ids = block_table.take(at).long()
+        ids.masked_fill_(outside | (ids < 0), pages)           # an id above the pool's lies behind it as it is
+        return torch.add(pos & size - 1, ids, alpha=size).masked_fill_(before, -1)
 
     def append(self, q, k, v, slots, positions=None, table=None, **kw):
         return paged_append(q, k, v, slots, positions, table, self.k_pages, self.v_pages, k_scale=self.k_scale,

@@ -1058,3 +1058,43 @@ def test_outputs_on_the_pool_and_shared_pools_are_refused(q8):
     want = c.append(packed[:, :4].clone(), packed[:, 4:5], packed[:, 5:], slots[:1])
     got = c.append(packed[:, :4], packed[:, 4:5], packed[:, 5:], slots[:1], q_out=packed[:, :4])
     assert got.data_ptr() == packed.data_ptr() and torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ slots
+def test_slots_of_indices_outside_the_table():
+    """Indices before a sequence are skipped (they do not wrap to the block table's last page); those behind the
+    table, of no sequence, or on a page that is not the pool's lie behind the pool."""
+    c = paged.PagedKVCache(5, 1, 64, 16, BF16, device="cpu")
+    bt = torch.tensor([[3, 1, -1], [0, 5, 2 ** 31 - 1]], dtype=torch.int32)
+    pos = torch.tensor([0, 17, 31, 32, 47, 48, -1, -48, -49, 2 ** 31, 0, 16, 40, 3, 3, -5], dtype=torch.int64)
+    seq = torch.tensor([0, 0, 0, 0, 0, 0, 0, 0, 1, 1, 1, 1, 1, 2, -1, 9], dtype=torch.int32)
+    want = [48, 17, 31, 80, 80, 80, -1, -1, -1, 80, 0, 80, 80, 80, 80, -1]      # 80: anything from there on
+
+    def slots(*args):
+        got = c.slots(*args)
+        assert got.dtype == torch.int64
+        return got.clamp(max=80).tolist()
+    assert slots(bt, seq, pos) == want
+    assert slots(bt, seq[:9], pos[:9].int()) == want[:9]
+    assert slots(bt[:, :0], seq[:8], pos[:8]) == [80] * 6 + [-1] * 2
+    assert slots(bt, seq[:0], pos[:0]) == []
+    # a view of a wider table
+    assert slots(bt[:, :2], seq[:4], pos[:4]) == [48, 17, 31, 80]
+
+
+@pytest.mark.gpu
+def test_append_of_a_padded_batch_through_slots():
+    g = gen(61)
+    c = paged.PagedKVCache(3, 2, 64, 16, BF16)
+    bt = torch.tensor([[2, 0]], dtype=torch.int32, device=DEV)
+    q, k, v = (rand(g, 4, 2, 64).to(BF16) for _ in range(3))
+    seq, pos = torch.zeros(4, dtype=torch.int64, device=DEV), torch.tensor([-1, 20, -7, 3], device=DEV)
+    c.append(q, k, v, c.slots(bt, seq, pos))
+    assert c.read_error() == 0
+    used = torch.zeros(3, 16, dtype=torch.bool, device=DEV)
+    used[0, 4] = used[2, 3] = True
+    assert torch.equal(c.k_pages[0, :, 4], k[1]) and torch.equal(c.v_pages[2, :, 3], v[3])
+    for x in (c.k_pages, c.v_pages):
+        assert bool((x.transpose(1, 2)[~used] == 0).all())
+    c.append(q, k, v, c.slots(bt, seq, pos + 32))            # one behind the table
+    assert c.read_error() == N.QV_DERR_CAPACITY
