@@ -71,6 +71,16 @@ __device__ __forceinline__ uint64_t ph_mul2(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ uint64_t ph_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t ph_sub2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ uint64_t ph_fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
@@ -256,26 +266,39 @@ __global__ void __launch_bounds__(PH_MOST, DT == QV_F32 ? 2 : 3) heads_kernel(co
                 if (!write || r >= nh) continue;
                 const size_t row = row0 + ((size_t)r << a.page_shift);
                 const float scale = __fdiv_rn(m, 127.f);
-                // x / scale as a product (a code differs from the quotient's only where that is within 2^-16 of a
-                // tie); a scale whose reciprocal leaves fp32's range divides; a row that is not finite: codes
-                // of 0 and a scale that is not finite read back as NaN
+                // x / scale as a product, at most 1.5 ulp off: 1.5 2^-17 below 128.  Where that leaves a code open (within
+                // 2^-15 of a tie), or the scale's reciprocal leaves fp32's range, the row's lane divides.  A row that is not
+                // finite: codes of 0 and a scale that is not finite read back as NaN
                 const bool plain = scale > 1e-37f && scale < INFINITY;
                 const float back = plain ? __fdiv_rn(1.f, scale) : 0.f;
+                const uint64_t back2 = ph_pack(back, back), high2 = ph_pack(12582912.f, 12582912.f);
+                int e[8];
+                float off = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    // |f| <= 127 but for its rounding, so the nearest integer is in range; with 1.5 2^23 added it stands in
+                    // the low bits
+                    const uint64_t f2 = ph_mul2(ph_pack(x[j], x[j + 1]), back2), t2 = ph_add2(f2, high2);
+                    float t0, t1, d0, d1;
+                    ph_unpack(t2, t0, t1);
+                    ph_unpack(ph_sub2(f2, ph_sub2(t2, high2)), d0, d1);
+                    off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
+                    e[j] = __float_as_int(t0);
+                    e[j + 1] = __float_as_int(t1);
+                }
+                const bool open = !plain || off > 0.5f - 0x1p-15f;
+                if (open) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        // (a subnormal scale is itself rounded: the quotient may pass 127)
+                        const float f = scale > 0.f && scale < INFINITY ? fminf(fmaxf(__fdiv_rn(x[j], scale), -127.f), 127.f) : 0.f;
+                        e[j] = __float_as_int(__fadd_rn(f, 12582912.f));
+                    }
+                }
                 uint32_t u[2];
 #pragma unroll
-                for (int j = 0; j < 8; j += 4) {
-                    int e[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float f = x[j + k] * back;
-                        if (!plain)   // (a subnormal scale is itself rounded: the quotient may pass 127)
-                            f = scale > 0.f && scale < INFINITY ? fminf(fmaxf(__fdiv_rn(x[j + k], scale), -127.f), 127.f) : 0.f;
-                        // |f| <= 127 but for the rounding of back, so the nearest integer is in range; with 1.5 2^23
-                        // added it stands in the low bits
-                        e[k] = __float_as_int(__fadd_rn(f, 12582912.f));
-                    }
-                    u[j / 4] = __byte_perm(__byte_perm(e[0], e[1], 0x0040), __byte_perm(e[2], e[3], 0x0040), 0x5410);
-                }
+                for (int j = 0; j < 8; j += 4)
+                    u[j / 4] = __byte_perm(__byte_perm(e[j], e[j + 1], 0x0040), __byte_perm(e[j + 2], e[j + 3], 0x0040), 0x5410);
                 *reinterpret_cast<uint2*>(reinterpret_cast<int8_t*>(kind == 2 ? a.vp : a.kp) + row * a.D + 8 * c) = make_uint2(u[0], u[1]);
                 if (c == 0) (kind == 2 ? a.v_scale : a.k_scale)[row] = scale;
             }

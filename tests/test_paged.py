@@ -1098,3 +1098,37 @@ def test_append_of_a_padded_batch_through_slots():
         assert bool((x.transpose(1, 2)[~used] == 0).all())
     c.append(q, k, v, c.slots(bt, seq, pos + 32))            # one behind the table
     assert c.read_error() == N.QV_DERR_CAPACITY
+
+
+# ------------------------------------------------------------------ INT8 codes
+def codes(x):
+    """Codes and scales of rows [..., D] as promised, on the host: IEEE fp32 divisions, ties to even."""
+    x = x.float().cpu()
+    s = x.abs().amax(-1) / torch.tensor(127.0)
+    return (x / s[..., None]).round().to(torch.int8), s
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_int8_codes_are_those_of_the_quotient(D, dt):
+    """Rows as they are (no norm, no rotation), with elements on and beside ties: the code is rint(row / scale)."""
+    g = gen(67)
+    T, H = 700, 2          # (44 pages hold them)
+    x = rand(g, T, 2 * H, D) * torch.exp2(torch.randint(-12, 5, (T, 2 * H, 1), generator=g, device=DEV).float())
+    s = x.abs().amax(-1, keepdim=True) / torch.tensor(127.0, device=DEV)
+    top = x.abs() == x.abs().amax(-1, keepdim=True)
+    # half of the rows: every element but the largest as near to a tie as the type allows, then an ulp to either side
+    tie = (torch.randint(-126, 126, x.shape, generator=g, device=DEV) + 0.5) * s
+    step = torch.randint(-1, 2, x.shape, generator=g, device=DEV) * 2.0 ** -23 * tie
+    x = torch.where(top | (torch.arange(T, device=DEV) % 2 == 0)[:, None, None], x, tie + step).to(dt)
+    if dt == FP32:      # the reciprocal's product alone gives other codes here
+        c, sc = codes(x)
+        assert int(((x.cpu() * (1 / sc[..., None])).round() != c).sum()) > 0
+    c = paged.PagedKVCache(T // 16 + 1, H, D, 16, dt, bits=8)
+    order = torch.randperm(T, generator=g, device=DEV)
+    c.append(x[:, :H], x[:, :H], x[:, H:], order)
+    for pages, scales, rows in ((c.k_pages, c.k_scale, x[:, :H]), (c.v_pages, c.v_scale, x[:, H:])):
+        want, ws = codes(rows)
+        assert torch.equal(scales.transpose(1, 2).reshape(-1, H)[order].cpu(), ws)
+        assert torch.equal(pages.transpose(1, 2).reshape(-1, H, D)[order].cpu(), want)
