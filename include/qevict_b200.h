@@ -257,8 +257,9 @@ int qv_prefill_read_error(const void* workspace, size_t workspace_bytes, int32_t
  *
  * Pool: k, v [pages][kv_heads][page_size][head_dim] in dtype, or (bits = 8)
  * INT8 codes with one fp32 scale per row, k_scale / v_scale
- * [pages][kv_heads][page_size]: value = code * scale (attention may take a value
- * scale below 2^-60 as 2^-60, and a sequence's value scales reach up to 2^49).
+ * [pages][kv_heads][page_size]: value = code * scale, scale >= 0 (attention may
+ * take a value scale below 2^-60 as 2^-60, a sequence's value scales reach up to
+ * 2^49, and a negative one may show as NaN).
  * Token j of a sequence b lives in page block_table[b][j / page_size] at offset
  * j % page_size.
  * Calls check what the device-side tables hold and stay inside their buffers;

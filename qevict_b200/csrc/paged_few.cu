@@ -299,7 +299,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
                     const float* sc = ring_sc + stage * 2 * KT + 16 * i2 + g + 8 * e;
                     ks = sc[0];
                     float vs = sc[KT];
-                    vs = vs < PF_MIN_SCALE ? PF_MIN_SCALE : vs;          // also a zero row, whose codes are 0
+                    vs = fabsf(vs) < PF_MIN_SCALE ? PF_MIN_SCALE : vs;   // also a zero row, whose codes are 0; below: NaN
                     if (edge && key >= s.kv) { ks = 0.f; vs = 1.f; }     // what lies there is not a row
                     lv = __log2f(vs);
                     iv[i2][e] = pf_ex2(-lv);

@@ -626,7 +626,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
                     const bool in = t < rows;
                     sc[t] = in ? ks * a.scale_log2 : 0.f;
                     if constexpr (DT == QV_F16) {
-                        if (vs < PT_MIN_SCALE) vs = PT_MIN_SCALE;    // also a zero row, whose codes are 0
+                        if (fabsf(vs) < PT_MIN_SCALE) vs = PT_MIN_SCALE;   // also a zero row, whose codes are 0; below: NaN
                         sc[PT_KEYS + t] = in ? log2f(vs) : 0.f;
                         sc[2 * PT_KEYS + t] = in ? 1.f / vs : 0.f;
                     } else {

@@ -18,7 +18,8 @@ named below.
 
 PagedKVCache holds a pool and calls them.  Pools are [pages, kv_heads,
 page_size, head_dim] in the model's dtype or INT8 with one fp32 scale per row
-([pages, kv_heads, page_size]); token j of sequence b lives in page
+([pages, kv_heads, page_size]; not negative, value scales of one sequence up to
+2^49, ones below 2^-60 may count as that); token j of sequence b lives in page
 block_table[b, j // page_size] at offset j % page_size.
 """
 

@@ -1132,3 +1132,22 @@ def test_int8_codes_are_those_of_the_quotient(D, dt):
         want, ws = codes(rows)
         assert torch.equal(scales.transpose(1, 2).reshape(-1, H)[order].cpu(), ws)
         assert torch.equal(pages.transpose(1, 2).reshape(-1, H, D)[order].cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("n", [1, 150])
+def test_attention_int8_negative_value_scale_is_not_another_row(n, dt):
+    """A pool filled by someone else: a negative value scale is honoured or shows as NaN, in the rows that see it."""
+    L, D, page = 400, 64, 32
+    g = gen(71)
+    pool = Pool(g, [L], 1, D, page, dt, True)
+    c, key = pool.cache, L - 2
+    pg, off = int(pool.bt[0, key // page]), key % page
+    c.v_scale[pg, 0, off] *= -1
+    pool.vs[0][key] *= -1
+    q = rand(g, n, 4, D).to(dt)
+    out = c.attend(q, pool.bt, pool.lens, cu([n]), max_q=n)
+    o, mag, big = ref_attention(q, pool.ks[0], pool.vs[0])
+    bound = attention_bound(o, mag, big, L, D, dt, float(pool.vs[0].abs().max()))
+    assert bool((((out.double() - o).abs() <= bound) | out.isnan()).all())
