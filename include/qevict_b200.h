@@ -265,8 +265,9 @@ int qv_prefill_read_error(const void* workspace, size_t workspace_bytes, int32_t
  * Calls check what the device-side tables hold and stay inside their buffers;
  * what they find wrong sets bits of *err (when not NULL): a page id or a
  * position outside its table QV_DERR_TABLE (attention then reads page 0, the
- * read-back leaves the row), a slot behind the pool or a length above its
- * bound QV_DERR_CAPACITY (not written / cut to the bound).
+ * read-back leaves the row), a slot behind the pool, a length above its bound or
+ * cumulative lengths that descend, leave the rows or (read-back) do not hold a
+ * sequence's tokens QV_DERR_CAPACITY (not written / cut to what there is).
  * What a call writes may not share memory with anything else of the call, but
  * for the places named below: such a call is refused (QV_EINVAL). */
 typedef struct qv_paged_cache {

@@ -333,6 +333,12 @@ template <int DT, bool Q8>
 __global__ void __launch_bounds__(PG_THREADS) gather_kernel(const GatherArgs a) {
     __shared__ int64_t s_row[PG_TOKENS];   // the token's row of head 0 in the pages, or -1
     const int t0 = blockIdx.x * PG_TOKENS;
+    if (blockIdx.x == 0 && a.err) {        // a sequence cut by the next one's rows, or by the rows there are
+        for (int b = threadIdx.x; b < a.B; b += PG_THREADS) {
+            const int at = a.cu_kv[b], to = a.cu_kv[b + 1], kv = a.kv_lens[b];
+            if (at < 0 || to < at || kv < 0 || kv > to - at || (kv > 0 && at > a.total - kv)) set_err(a.err, QV_DERR_CAPACITY);
+        }
+    }
     if (threadIdx.x < PG_TOKENS) {
         const int t = t0 + threadIdx.x;
         int64_t row = -1;

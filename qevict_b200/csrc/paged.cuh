@@ -79,6 +79,16 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
     return s;
 }
 
+// Raises the error word where a sequence's rows descend or leave the queries.  Once per launch, by 32 threads t of
+// its first block, beside the warp that looks for the tile.
+__device__ __forceinline__ void paged_check_rows(const PagedArgs& a, int t) {
+    if (!a.err) return;
+    for (int b = t; b < a.B; b += 32) {
+        const int at = a.cu_q[b], to = a.cu_q[b + 1];
+        if (at < 0 || to < at || to > a.total_q) set_err(a.err, QV_DERR_CAPACITY);
+    }
+}
+
 // Keys that token i of the chunk sees.
 __device__ __forceinline__ int paged_limit(const PagedArgs& a, const PagedSeq& s, int i) {
     return a.causal ? min(s.kv, s.kv - s.n + i + 1) : s.kv;

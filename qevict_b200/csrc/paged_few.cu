@@ -112,7 +112,13 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
     const PagedSeq s = paged_seq(a, b);
     const int rows = s.live * a.G;
     const bool split = a.splits > 1 && s.kv > a.chunk;
-    if (rows == 0 || (!split && sp > 0)) return;
+    // as paged_check_rows, in one block of the sequence
+    const bool check = h == 0 && sp == 0 && a.err && threadIdx.x == 32 * W - 1;
+    auto rows_ok = [&]() { return a.cu_q[b] == s.q0 && a.cu_q[b + 1] == s.q0 + s.n; };
+    if (rows == 0 || (!split && sp > 0)) {
+        if (check && !rows_ok()) set_err(a.err, QV_DERR_CAPACITY);
+        return;
+    }
     const int last = paged_limit(a, s, s.live - 1);
     const int k_begin = split ? sp * a.chunk : 0;
     const int k_end = split ? min(last, k_begin + a.chunk) : last;
@@ -177,6 +183,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__
         for (int i = 0; i < C::STAGES && i < mine; ++i) { find_pages(); issue(); }
         find_pages();
     }
+    if (check && !rows_ok()) set_err(a.err, QV_DERR_CAPACITY);   // (behind the first loads)
 
     // query fragments: lane (g, t) holds row 8 q + g; its four slots of a k-step are elements 2t, 2t + 1,
     // 2t + 8, 2t + 9, or with INT8 the four consecutive codes of the chunk it reads

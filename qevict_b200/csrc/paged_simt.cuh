@@ -71,6 +71,8 @@ __global__ void __launch_bounds__(PS_THREADS, BM > 64 ? 1 : 2) paged_simt_kernel
     if (threadIdx.x < 32) {
         const int2 t = paged_find_tile(a, blockIdx.x, a.G, BM);
         if (threadIdx.x == 0) s_tile = t;
+    } else if (threadIdx.x < 64 && blockIdx.x == 0 && h == 0 && sp == 0) {
+        paged_check_rows(a, threadIdx.x - 32);
     }
     __syncthreads();
     const int b = s_tile.x;

@@ -177,6 +177,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
         const int2 t = paged_find_tile(a, blockIdx.x / a.H, 1, 2 * QT);
         if (lane == 0) s_tile = t;
     }
+    if (warp == 9 && blockIdx.x == 0 && blockIdx.y == 0) paged_check_rows(a, lane);
     __syncthreads();
     const int b = s_tile.x;
     if (b < 0) return;

@@ -1151,3 +1151,55 @@ def test_attention_int8_negative_value_scale_is_not_another_row(n, dt):
     o, mag, big = ref_attention(q, pool.ks[0], pool.vs[0])
     bound = attention_bound(o, mag, big, L, D, dt, float(pool.vs[0].abs().max()))
     assert bool((((out.double() - o).abs() <= bound) | out.isnan()).all())
+
+
+# ------------------------------------------------------------------ cumulative lengths
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [2, 600])
+def test_gather_reports_rows_that_do_not_hold_a_sequence(B):
+    """Sequences cut by the next one's rows or by the rows there are raise the error word; the rows that exist are read."""
+    g = gen(73)
+    lens = [5] * B
+    pool = Pool(g, lens, 1, 64, 16, BF16, False)
+    c, total = pool.cache, 5 * B
+    ok = cu(lens)
+    want, _ = c.gather(pool.bt, pool.lens, ok, total)
+    assert c.read_error() == 0
+    c.gather(pool.bt, pool.lens, torch.cat([ok[:1], ok[1:] + 2]), total + 2)       # a gap is no fault
+    assert c.read_error() == 0
+
+    def reported(lens, cu_kv, total):
+        c.err.zero_()
+        k, _ = c.gather(pool.bt, lens, cu_kv, total, out=tuple(torch.zeros(total, 1, 64, dtype=BF16, device=DEV) for _ in range(2)))
+        assert c.read_error() == N.QV_DERR_CAPACITY
+        return k
+    assert torch.equal(reported(pool.lens, ok, total - 1), want[:-1])              # fewer rows than tokens
+    more = pool.lens.clone()
+    more[B - 1] += 1
+    assert torch.equal(reported(more, ok, total), want)                            # a length past its rows
+    for i, d in ((0, -1), (B, -1), (1, -6)):
+        bad = ok.clone()
+        bad[i] += d
+        reported(pool.lens, bad, total)
+    less = pool.lens.clone()
+    less[0] = -1
+    reported(less, ok, total)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 60])
+@pytest.mark.parametrize("dt", [BF16, FP32])
+def test_attention_reports_chunks_outside_the_rows(n, dt):
+    g = gen(79)
+    pool = Pool(g, [100, 90], 1, 64, 16, dt, False)
+    c, q, ok = pool.cache, rand(g, 2 * n, 4, 64).to(dt), cu([n, n])
+    want = c.attend(q, pool.bt, pool.lens, ok, max_q=n)
+    assert c.read_error() == 0
+    for i, d in ((0, -1), (2, 1), (1, n + 1)):
+        bad = ok.clone()
+        bad[i] += d
+        got = c.attend(q, pool.bt, pool.lens, bad, max_q=n)
+        assert c.read_error() == N.QV_DERR_CAPACITY
+        if i == 2:
+            assert torch.equal(got[:n], want[:n])        # the other sequence is right
+        c.err.zero_()
