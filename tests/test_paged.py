@@ -1203,3 +1203,25 @@ def test_attention_reports_chunks_outside_the_rows(n, dt):
         if i == 2:
             assert torch.equal(got[:n], want[:n])        # the other sequence is right
         c.err.zero_()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_attention_fp16_keeps_probabilities_down_to_2_31(shape, q8):
+    """The fp16 kernels set a row's reference 2^7 below a maximum, so the largest P is at least 2^7 at the end, and what
+    rounds at fp16's smallest step (2^-24) is off by 2^-25 / 2^7 of the sum for each key.  With INT8 pages P = p vs
+    and the sum is of P / vs: at least 2^7 / (largest scale), each key's product with a code of up to 127 off by 127 2^-25: the
+    same 2^-32 of the largest |v| (127 times its scale)."""
+    q_lens, kv_lens, Hq, H, D, page = SHAPES[shape]
+    pool, q, out = check_attention(gen(200 + shape), q_lens, kv_lens, Hq, H, D, page, FP16, q8, max_q=max(q_lens))
+    at = 0
+    for b, n in enumerate(q_lens):
+        if n and kv_lens[b]:
+            o, mag, big = ref_attention(q[at:at + n], pool.ks[b], pool.vs[b])
+            vmax = float(pool.vs[b].abs().max())
+            bound = attention_bound(o, mag, big, kv_lens[b], D, FP32, vmax) + o.abs() * half(FP16) * 1.001 + (
+                mag * half(FP16) * 1.01 + TINY[FP16] + kv_lens[b] * 2.0 ** -32 * vmax)
+            d = (out[at:at + n].double() - o).abs()
+            assert bool((d <= bound).all()), (b, n, kv_lens[b], float((d / bound).max()))
+        at += n
