@@ -7,14 +7,19 @@ tensors' device, none of which synchronises:
 
   qk_norm_rope     per-head norm and rotation of query and key heads
   paged_append     the same, with the new keys and values written into pages
-  paged_gather     pages read back into contiguous rows (what
-                   model.prefill_attention and StickyLayerState.prefill take)
+  paged_gather     pages read back into contiguous rows [tokens, heads, head_dim]
+                   (as model.prefill_attention takes them)
   paged_attention  chunks of new tokens, from one token to whole prompts,
                    over the pages
 
 What a call writes (outputs, and the pool of paged_append) may not share memory
 with anything else of the call: refused, but for the in-place outputs that are
 named below.
+
+A prompt collected in pages goes to a Sticky layer as the model's own prompt does:
+model.prefill_attention over its rotated queries and the rows read back gives the
+column sums, and StickyLayerState.prefill takes those with K and V transposed to
+[batch, heads, tokens, head_dim].
 
 PagedKVCache holds a pool and calls them.  Pools are [pages, kv_heads,
 page_size, head_dim] in the model's dtype or INT8 with one fp32 scale per row

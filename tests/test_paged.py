@@ -1225,3 +1225,50 @@ def test_attention_fp16_keeps_probabilities_down_to_2_31(shape, q8):
             d = (out[at:at + n].double() - o).abs()
             assert bool((d <= bound).all()), (b, n, kv_lens[b], float((d / bound).max()))
         at += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 8])
+def test_prompt_in_pages_to_a_sticky_layer(bits):
+    """A prompt that came in ragged chunks is read back and becomes a Sticky layer's prompt, which then decodes across
+    evictions: the same bits as the layer built from the rows that the pool holds, without pages."""
+    from qevict_b200.layer_state import StickyLayerState
+    from qevict_b200.model import prefill_attention
+    Hq, H, D, page, dt, om, sink, S, steps = 8, 2, 128, 32, BF16, 32, 32, 32 + 32 * 15, 70
+    g = gen(83)
+    qkv = rand(g, S + steps, Hq + 2 * H, D).to(dt)
+    table = paged.rope_table(1024, D, 500000.0)
+    pos = torch.arange(S + steps, device=DEV, dtype=torch.int32)
+    qr, kr = paged.qk_norm_rope(qkv[:, :Hq], qkv[:, Hq:Hq + H], pos, table)
+    v = qkv[:, Hq + H:].contiguous()
+    c = paged.PagedKVCache(20, H, D, page, dt, bits=bits)
+    bt = torch.randperm(20, generator=g, device=DEV).int()[: S // page].view(1, -1).contiguous()
+    queries, at = [], 0
+    for n in (200, 1, 150, S - 351):
+        rows = slice(at, at + n)
+        slots = c.slots(bt, torch.zeros_like(pos[rows]), pos[rows])
+        queries.append(c.append(qkv[rows, :Hq], qkv[rows, Hq:Hq + H], qkv[rows, Hq + H:], slots, pos[rows], table))
+        at += n
+    q = torch.cat(queries)
+    k1, v1 = c.gather(bt, torch.tensor([S], dtype=torch.int32, device=DEV), cu([S]), S)
+    assert c.read_error() == 0 and torch.equal(q, qr[:S])
+    if bits == 16:
+        k2, v2 = kr[:S], v[:S]
+    else:   # the rows as the pool holds them, by hand
+        def held(pages, scales):
+            ids = bt[0].long()
+            x = pages[ids].float() * scales[ids][..., None]
+            return x.transpose(1, 2).reshape(S, H, D).to(dt)
+        k2, v2 = held(c.k_pages, c.k_scale), held(c.v_pages, c.v_scale)
+    outs = []
+    for kk, vv in ((k1, v1), (k2, v2)):
+        _, colsum = prefill_attention(q[None], kk[None].contiguous(), vv[None].contiguous())
+        layer = StickyLayerState(1, H, Hq // H, D, om, sink, 64, 2, 3, 32, 8, dt)
+        layer.prefill(kk[None].transpose(1, 2), vv[None].transpose(1, 2), colsum)
+        outs.append(torch.stack([layer.step(qr[i].view(1, Hq, D), kr[i].view(1, H, D), v[i].view(1, H, D))
+                                 for i in range(S, S + steps)]))
+        assert layer.read_error() == 0
+        ids, _ = layer.view_sticky(0)
+        outs.append(ids)
+    assert torch.equal(outs[0], outs[2]) and bool(outs[0].isfinite().all())
+    assert torch.equal(torch.as_tensor(outs[1]), torch.as_tensor(outs[3]))
