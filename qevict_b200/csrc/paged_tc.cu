@@ -667,13 +667,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ 
 
 // ---------------------------------------------------------------- host
 static PFN_cuTensorMapEncodeTiled_v12000 pt_encode() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> found{nullptr};   // calls may come from several threads
+    PFN_cuTensorMapEncodeTiled_v12000 fn = found.load(std::memory_order_acquire);
     if (!fn) {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
+            q == cudaDriverEntryPointSuccess) {
             fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+            found.store(fn, std::memory_order_release);
+        }
     }
     return fn;
 }

@@ -1272,3 +1272,35 @@ def test_prompt_in_pages_to_a_sticky_layer(bits):
         outs.append(ids)
     assert torch.equal(outs[0], outs[2]) and bool(outs[0].isfinite().all())
     assert torch.equal(torch.as_tensor(outs[1]), torch.as_tensor(outs[3]))
+
+
+@pytest.mark.gpu
+def test_attention_from_several_threads():
+    """Four host threads at once, each on a stream of its own, over one pool: the bits of the calls made alone."""
+    import threading
+    g = gen(89)
+    pool = Pool(g, [900, 40, 333], 2, 128, 32, BF16, True)
+    jobs = []
+    for n in (1, 2, 3, 33):
+        q = rand(g, 3 * n, 8, 128).to(BF16)
+        jobs.append((q, cu([n] * 3), n, pool.cache.attend(q, pool.bt, pool.lens, cu([n] * 3), max_q=n)))
+    torch.cuda.synchronize()
+    got, faults = [[] for _ in jobs], []
+
+    def work(i):
+        try:
+            q, c, n, _ = jobs[i]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    got[i].append(pool.cache.attend(q, pool.bt, pool.lens, c, max_q=n))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:     # noqa: BLE001 -- reported by the thread that runs the test
+            faults.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not faults and pool.cache.read_error() == 0
+    for (_, _, _, want), outs in zip(jobs, got):
+        assert len(outs) == 50 and all(torch.equal(o, want) for o in outs)
