@@ -1304,3 +1304,48 @@ def test_attention_from_several_threads():
     assert not faults and pool.cache.read_error() == 0
     for (_, _, _, want), outs in zip(jobs, got):
         assert len(outs) == 50 and all(torch.equal(o, want) for o in outs)
+
+
+ORIG = dict(low_freq_factor=1.0, high_freq_factor=4.0, original_max_position=8192)
+
+
+@pytest.mark.parametrize("theta,rot", [(10000.0, 64), (500000.0, 128), (1000.0, 8)])
+@pytest.mark.parametrize("scaling", [None, dict(type="linear", factor=3.0), dict(type="ntk", factor=4.0),
+                                     dict(type="llama3", factor=8.0, **ORIG),
+                                     dict(type="yarn", factor=16.0, original_max_position=4096),
+                                     dict(type="yarn", factor=4.0, original_max_position=8192, beta_fast=16, beta_slow=2,
+                                          attention_factor=1.25)])
+def test_rope_table_is_the_formula(theta, rot, scaling):
+    """Every pair at a few positions against the formulas one number at a time in 64 bits.  An entry is rounded once
+    (half a step of a number below 2 mult); 64-bit frequencies are off by a few 2^-53, so an angle of up to 2^17 by 2^-33."""
+    t = paged.rope_table(131072, rot, theta, scaling, device="cpu")
+    kind = scaling["type"] if scaling else None
+    f = scaling["factor"] if scaling else 1.0
+    mult = 1.0
+    if kind == "yarn":
+        mult = scaling.get("attention_factor", 0.1 * math.log(f) + 1)
+    worst = (0.0,)
+    for i in range(rot // 2):
+        base = theta * f ** (rot / (rot - 2)) if kind == "ntk" else theta
+        w = base ** (-2 * i / rot)
+        if kind == "linear":
+            w /= f
+        elif kind == "llama3":
+            wave = 2 * math.pi / w
+            if wave > 8192 / 1.0:
+                w /= f
+            elif wave >= 8192 / 4.0:
+                smooth = (8192 / wave - 1.0) / (4.0 - 1.0)
+                w = (1 - smooth) * w / f + smooth * w
+        elif kind == "yarn":
+            orig = scaling["original_max_position"]
+            at = [rot * math.log(orig / (n * 2 * math.pi)) / (2 * math.log(theta))
+                  for n in (scaling.get("beta_fast", 32), scaling.get("beta_slow", 1))]
+            lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rot - 1)
+            share = min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0)
+            w = w * (1 - share) + w / f * share
+        for p in (0, 1, 2, 77, 4095, 8192, 100003, 131071):
+            for j, want in ((i, math.cos(p * w)), (rot // 2 + i, math.sin(p * w))):
+                d = abs(float(t[p, j]) - want * mult)
+                worst = max(worst, (d, p, i, float(t[p, j]), want * mult))
+    assert worst[0] <= mult * (2.0 ** -24 + 2.0 ** -32), worst     # (difference, position, pair, entry, formula)
