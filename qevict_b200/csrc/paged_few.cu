@@ -10,7 +10,7 @@
 // stage), so that no barrier couples the warps until their states join at the
 // end.  Blocks of four warps with 64 KB of rings: three share an SM (two with more
 // than eight rows), and one's start and end hide behind the others' loads.  64
-// sequences over up to 8192 INT8 tokens: 108 us, 122 us with two blocks and rings of
+// sequences over up to 8192 INT8 tokens: 109 us, 122 us with two blocks and rings of
 // three stages instead of two.  Short sequences that a block reads alone take eight
 // warps with 192 KB (512 keys 6.1 us, as four splits and their merge take with a
 // launch more; 8 uneven sequences of up to 1000 keys 9.2 against 9.5).
@@ -22,7 +22,9 @@
 // (movmatrix).  The reference m is set 2^7 below a maximum and moves only when a
 // logit exceeds it by 2^15, so that a tile needs no row maximum across lanes and
 // P spans fp16 down to 2^-31 of the largest.  With bf16 pages P is split into two
-// bf16 parts (P V is then exact to 2^-17; the tensor pipe is idle anyway).
+// bf16 parts (P V is then exact to 2^-17; the tensor pipe is idle anyway).  fp16's P is one
+// fp16 number, as precise as the output: outputs are 1.3-1.4 times as far from 64 bits as
+// fp32 arithmetic rounded once (bf16: as far).
 //
 // INT8 rows: the codes become exact fp16 integers in registers and the scales
 // stay in fp32,

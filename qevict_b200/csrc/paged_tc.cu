@@ -11,7 +11,7 @@
 // exponentials (16 per clock and SM) instead of their sum.  The (x, j) pairs take
 // two or three S buffers in turn (what O leaves of TMEM's 512 columns), so that at
 // D = 64, or once only one row tile has keys left, S of a later tile is ready when a
-// tile's softmax ends: 17 chunks and single tokens at D = 64 102 us (114 with one
+// tile's softmax ends: 17 chunks and single tokens at D = 64 103 us (114 with one
 // buffer per row tile), four 512-token chunks over INT8 pages 241 (272).
 //
 // m_x is a reference, not the running maximum: softmax is the same for any m, and
@@ -20,14 +20,18 @@
 // it and move it only where P would pass 2^24 (fp16: 2^15), rescaling O_x and l_x.
 // So almost no tile touches O in TMEM.
 //
-// (Measured and left out, 8192-token prompt at D = 128, 437-443 us: a quarter of
+// (Measured and left out, 8192-token prompt at D = 128, 437-443 us in a short run, 513-523
+// back to back at the clock that the power cap leaves: a quarter of
 // the exponentials as a polynomial on the FMA pipe, 462 us; the two tiles' softmax
 // warps taking turns at the exponentials, 456 us; two threads to a row, 494 us; no
 // row maximum, the reference moving where a tile's sum of P is too large, 455-468.
-// Without any exponentials it takes as long: the tensor pipe at the clock that its
-// power allows bounds it.  At D = 64 (347 us, 346 without exponentials) the bound
-// is the softmax warps' dependent instructions: two warps per scheduler issue in
-// 39 % of its cycles.)
+// Without any exponentials it takes as long, and the tensor pipe is active in 61 % of the
+// cycles: the hand-over between a tile's softmax and its products bounds it.  At D = 64
+// (347 us, 346 without exponentials) the bound is the softmax warps' dependent
+// instructions: two warps per scheduler issue in 34-39 % of its cycles.)
+//
+// P is one 16-bit number: outputs are 1.2-1.4 times as far from 64 bits as fp32 arithmetic
+// rounded once.
 //
 // INT8 pages: codes become exact 16-bit integers in shared memory (six extra
 // warps); the row scales ks, vs of a key stay in fp32: the logit is S c ks, and the

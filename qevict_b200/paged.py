@@ -218,7 +218,7 @@ def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=No
                  out=None):
     """RMS norm (where a weight is given) and rotation (where a table is) of each query and key head.
 
-    q [T, q_heads, D], k [T, kv_heads, D], heads contiguous within a token; positions [T] int32; table from
+    q [T, q_heads, D], k [T, kv_heads, D], heads contiguous within a token, tokens on 16-byte boundaries; positions [T] int32; table from
     rope_table, its rot_dim the part of the head that turns, in pairs (i, i + rot_dim/2), or (2i, 2i+1) with
     interleaved.  Returns contiguous (q, k), or fills out=(q_out, k_out), which may be q and k themselves
     where those are contiguous.  A position outside the table gives NaN.  (qv_qk_norm_rope)"""
@@ -315,8 +315,9 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
     kv_lens[b] (int32 [batch]) cached tokens; block_table int32 [batch, max_pages].  Causal: each token sees the
     keys up to its own.  A row that sees no key gives 0; rows of no chunk are left as they were (out) or
     undefined.  max_q / max_kv: upper bounds of the chunk and cached lengths, which size the launch (default:
-    T, and all that the block table can hold); a captured call serves any lengths below them.  out may be q
-    where that is contiguous.  scale (positive) defaults to D^-1/2.  (qv_paged_attention)"""
+    T, and all that the block table can hold); a captured call serves any lengths below them, fastest where they
+    are close: pass max_q=1 for a decode batch (without it more than 16 rows per kv head run as prompts do), and
+    max_kv near the longest.  out may be q where that is contiguous.  scale (positive) defaults to D^-1/2.  (qv_paged_attention)"""
     dt = q.dtype
     c, dev, H, S, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
     if D != 64 and D != 128:
