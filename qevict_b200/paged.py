@@ -218,10 +218,10 @@ def qk_norm_rope(q, k, positions=None, table=None, *, q_weight=None, k_weight=No
                  out=None):
     """RMS norm (where a weight is given) and rotation (where a table is) of each query and key head.
 
-    q [T, q_heads, D], k [T, kv_heads, D], heads contiguous within a token, tokens on 16-byte boundaries; positions [T] int32; table from
-    rope_table, its rot_dim the part of the head that turns, in pairs (i, i + rot_dim/2), or (2i, 2i+1) with
-    interleaved.  Returns contiguous (q, k), or fills out=(q_out, k_out), which may be q and k themselves
-    where those are contiguous.  A position outside the table gives NaN.  (qv_qk_norm_rope)"""
+    q [T, q_heads, D], k [T, kv_heads, D], heads contiguous within a token, tokens on 16-byte boundaries;
+    positions [T] int32; table from rope_table, its rot_dim the part of the head that turns, in pairs
+    (i, i + rot_dim/2), or (2i, 2i+1) with interleaved.  Returns contiguous (q, k), or fills out=(q_out, k_out),
+    which may be q and k themselves where those are contiguous.  A position outside the table gives NaN.  (qv_qk_norm_rope)"""
     dt, dev = q.dtype, q.device
     code = _DTYPES.get(dt)
     if not q.is_cuda or code is None or q.ndim != 3:
@@ -317,7 +317,8 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, k_scale=
     undefined.  max_q / max_kv: upper bounds of the chunk and cached lengths, which size the launch (default:
     T, and all that the block table can hold); a captured call serves any lengths below them, fastest where they
     are close: pass max_q=1 for a decode batch (without it more than 16 rows per kv head run as prompts do), and
-    max_kv near the longest.  out may be q where that is contiguous.  scale (positive) defaults to D^-1/2.  (qv_paged_attention)"""
+    max_kv near the longest.  out may be q where that is contiguous.  scale (positive) defaults to D^-1/2.
+    (qv_paged_attention)"""
     dt = q.dtype
     c, dev, H, S, D = _pool(k_pages, v_pages, k_scale, v_scale, dt, err)
     if D != 64 and D != 128:
